@@ -50,8 +50,9 @@ const char* lr_last_error(void);
  * Bit 0: an adaLN index was outside [0, table_rows) (that row used a zero
  * modulation); bit 1: a bounded wait inside the GEMM gave up; bit 2: a row
  * index of lr_gather_rows / lr_flash_restore was outside its source (that
- * output row was written from zeros). Bit 1 also covers the attention
- * kernel's bounded waits. Synchronises the device. */
+ * output row was written from zeros); bit 3: offsets of packed sequences went
+ * down or outside their tensor. Bit 1 also covers the bounded waits of the
+ * attention and 4-bit GEMM kernels. Synchronises the device. */
 int lr_device_status(unsigned int* bits, int clear);
 
 /* Arithmetic of the divisions and RMS reciprocal square roots of the
@@ -222,6 +223,75 @@ int lr_attention_bf16(const void* q, int64_t q_token_stride, const void* k, int6
                       const void* v, int64_t v_token_stride, int64_t batch, int64_t seq_q, int64_t seq_kv,
                       int64_t heads, int64_t head_dim, float scale, void* out, int64_t out_token_stride,
                       void* stream);
+
+/* A2 — attention over packed sequences of different lengths (bf16). Token t of
+ * sequence b is row cu_q[b] + t of q and out and, for keys, cu_k[b] + t of k and v
+ * (cu_q, cu_k: int32 device arrays [seqs + 1], cu[0] = 0, not decreasing). Query
+ * head h reads key/value head h / (heads / kv_heads):
+ *   out[i,h,:] = sum_j softmax_j(scale * q[i,h,:] . k[j,h',:]) * v[j,h',:]
+ * over the keys of i's sequence; with causal != 0 the queries are the last ones
+ * of their sequence: query i of Lq sees the keys j <= i + Lk - Lq of Lk. Rows
+ * without a visible key, and rows of q past cu_q[seqs], give zeros. fp32
+ * scores, softmax statistics and accumulation; probabilities rounded to bf16.
+ * head_dim 64 or 128; element strides of tokens and heads per operand, columns
+ * contiguous; pointers and strides 16-byte aligned; out contiguous
+ * [total_q, heads, head_dim]. Offsets outside the tensors raise device status
+ * bit 3 and are clamped. No counterpart in the reference. */
+int lr_attention_packed(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs,
+                        int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                        int causal, float scale, void* out, void* stream);
+
+/* R1 — rotary position embedding of q and k (bf16), no tables: the pair of
+ * frequency i of a token at position p is turned by p * inv_freq[i] radians
+ * (evaluated in turns to about 1e-7 for |p| < 2^36) and multiplied by `factor`;
+ * pairs are columns (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved
+ * != 0; columns from rotary_dim on are copied. positions: int32, or int64 with
+ * positions_64 != 0, one per token. q, k: element strides of tokens and heads,
+ * columns contiguous; q_out, k_out: contiguous [tokens, heads, head_dim]. Either
+ * of q, k may be left out with 0 heads. No counterpart in the reference (its
+ * rotary embedding is fused with a norm, lr_qk_norm_rope). */
+int lr_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, const void* k,
+            int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads, const void* positions,
+            int positions_64, const float* inv_freq, float factor, int64_t tokens, int64_t head_dim,
+            int64_t rotary_dim, int interleaved, void* q_out, void* k_out, void* stream);
+
+/* 4-bit floating-point formats: e2m1 codes, two a byte (the even column in the
+ * low nibble), under block scales. No counterpart in the reference.
+ *   LR_FP4_NV: blocks of 16 columns, e4m3 scales, and an fp32 scale per row:
+ *     A = max(max |x|, 1e-8), row scale A / 2688, block scale e = e4m3(448 max_b |x| / A),
+ *     code = e2m1(x * (2688 / (e A)));
+ *   LR_FP4_MX: blocks of 32 columns, e8m0 scales 2^e, e = floor(log2(max_b |x|)) - 2,
+ *     code = e2m1(x * 2^-e); no row scale.
+ * Nearest even, saturating. An infinity or NaN turns its row's (NV) or block's
+ * (MX) scale into NaN. Widths are multiples of 32.
+ * Scales lie in tiles of 128 rows x 4 blocks: uint8 [ceil(rows/128),
+ * ceil(blocks/4), 32, 4, 4], element [R, C, r, j, c] the scale of row
+ * 128 R + 32 j + r, block 4 C + c. Blocks past the row hold zeros; bytes of rows
+ * past the matrix are neither written nor read into a result. */
+#define LR_FP4_NV 0
+#define LR_FP4_MX 1
+
+/* Q4 — quantise bf16 rows (row stride in elements, rows 16-byte aligned):
+ * codes [rows, width/2], scales as above, row_scales fp32 [rows] (NV only). */
+int lr_fp4_quantize_rows(const void* x, int64_t rows, int64_t width, int64_t row_stride, int format,
+                         void* codes, void* scales, float* row_scales, void* stream);
+
+/* The values of such rows as bf16 [rows, width]: code * (scale * row_scale),
+ * rounded once; row_scales may be NULL (1). */
+int lr_fp4_dequantize_rows(const void* codes, const void* scales, const float* row_scales, int64_t rows,
+                           int64_t width, int format, void* out, void* stream);
+
+/* G4 — product of two 4-bit matrices with fp32 accumulation:
+ *   out[m,n] = bf16((sum_k A[m,k] B[n,k]) * row_scale[m] * col_scale[n] + bias[n])
+ * a: codes [M, K/2] with a_scales; b: codes [N, K/2] with b_scales (weights, one
+ * row per output); row_scale [M], col_scale [N] fp32 or NULL (1); bias bf16 [N]
+ * or NULL; out bf16 [M, N], row stride ldo. K a multiple of 32; codes and scales
+ * 16-byte aligned. */
+int lr_fp4_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t M,
+                int64_t N, int64_t K, int format, const float* row_scale, const float* col_scale,
+                const void* bias, void* out, int64_t ldo, void* stream);
 
 /* K10 (+K2 fused) — INT8 GEMM with int32 accumulation and a fused bf16 epilogue.
  * Replaces model/int8_gemm.py:96-163 `int8_matmul` (kernel `_gemm` :13-46),

@@ -24,6 +24,9 @@ LR_EPI_NONE = 0
 LR_EPI_GELU_TANH = 1
 LR_EPI_GATED_RESIDUAL = 2
 
+LR_FP4_NV = 0
+LR_FP4_MX = 1
+
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
@@ -51,6 +54,13 @@ SIGNATURES = {
     "lr_flash_restore": ([_p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _p, _p], _i32),
     "lr_flash_nearest_anchor": ([_p, _i64, _p, _i64, _p, _i64, _p, _p], _i32),
     "lr_attention_bf16": ([_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p], _i32),
+    "lr_attention_packed": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _i32, _f32, _p, _p], _i32),
+    "lr_rope": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _f32, _i64, _i64, _i64, _i32, _p, _p,
+                 _p], _i32),
+    "lr_fp4_quantize_rows": ([_p, _i64, _i64, _i64, _i32, _p, _p, _p, _p], _i32),
+    "lr_fp4_dequantize_rows": ([_p, _p, _p, _i64, _i64, _i32, _p, _p], _i32),
+    "lr_fp4_gemm": ([_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _p], _i32),
     "lr_int8_gemm": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i32, _p, _i64, _p,
                       _i64, _i64, _p, _i64, _i32, _p, _i64, _p], _i32),
     "lr_int8_gemm_workspace_bytes": ([_i64, _i64, _i64], _i64),
@@ -146,7 +156,8 @@ def arithmetic() -> str:
 
 
 def device_status(clear: bool = True) -> int:
-    """Device status bits (1: adaLN index out of range, 2: GEMM wait timeout)."""
+    """Device status bits (1: adaLN index out of range, 2: a bounded wait gave up, 4: row index out of range,
+    8: offsets of packed sequences out of range)."""
     bits = ctypes.c_uint(0)
     check(load().lr_device_status(ctypes.byref(bits), int(clear)), "device_status")
     return bits.value

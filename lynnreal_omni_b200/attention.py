@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import check, ptr, stream_of
 
-__all__ = ["attention_bshd"]
+__all__ = ["attention_bshd", "attention_packed"]
 
 
 def _token_view(t: torch.Tensor) -> torch.Tensor:
@@ -50,4 +50,55 @@ def attention_bshd(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     check(_lib.load().lr_attention_bf16(
         ptr(query), query.stride(1), ptr(key), key.stride(1), ptr(value), value.stride(1), b, sq, skv, h, d, sc,
         ptr(out), out.stride(1), stream_of(query)), "attention_bshd")
+    return out
+
+
+def _head_view(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, D] with contiguous columns and 16-byte aligned tokens and heads, else a contiguous copy."""
+    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: torch.Tensor | None = None, *, causal: bool = True,
+                     scale: float | None = None) -> torch.Tensor:
+    """Attention of packed sequences of different lengths -> bf16 [tokens, heads, D].
+
+    query [Tq, heads, D], key and value [Tk, kv_heads, D]: bf16, D 64 or 128, strided views are used in place; heads a
+    multiple of kv_heads (query head h reads key/value head h // (heads / kv_heads)). cu_seqlens_q, cu_seqlens_k: int32
+    [sequences + 1] offsets on the device (never read by the host); the keys' default to the queries'. ``causal``: the
+    queries are the last ones of their sequence, each sees the keys up to its own position (one query a sequence is a
+    decoding step). Rows without a visible key, and tokens past the last offset, give zeros. Values of other sequences
+    never reach a row; within a sequence, values of masked keys must be finite."""
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.dtype != torch.bfloat16 or not t.is_cuda or t.ndim != 3:
+            raise ValueError(f"attention_packed: {name} must be a CUDA bf16 [tokens, heads, D] tensor")
+        if t.device != query.device:
+            raise ValueError("attention_packed: query, key and value are on different devices")
+    tq, h, d = query.shape
+    tk, hk, _ = key.shape
+    if value.shape != key.shape or key.shape[2] != d:
+        raise ValueError("attention_packed: query/key/value shapes disagree")
+    if d not in (64, 128):
+        raise ValueError(f"attention_packed: head_dim {d} (the kernel handles 64 and 128)")
+    if hk == 0 or h == 0 or h % hk:
+        raise ValueError(f"attention_packed: {h} query heads do not share {hk} key/value heads evenly")
+    if cu_seqlens_k is None:
+        if tk != tq:
+            raise ValueError("attention_packed: cu_seqlens_k is needed where queries and keys differ in tokens")
+        cu_seqlens_k = cu_seqlens_q
+    for t in (cu_seqlens_q, cu_seqlens_k):
+        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() < 2 or t.device != query.device:
+            raise ValueError("attention_packed: cu_seqlens must be int32 [sequences + 1] on the query's device")
+    if cu_seqlens_k.numel() != cu_seqlens_q.numel():
+        raise ValueError("attention_packed: cu_seqlens_q and cu_seqlens_k differ in sequences")
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
+    query, key, value = _head_view(query), _head_view(key), _head_view(value)
+    out = torch.empty((tq, h, d), device=query.device, dtype=torch.bfloat16)
+    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    check(_lib.load().lr_attention_packed(
+        ptr(query), query.stride(0), query.stride(1), ptr(key), key.stride(0), key.stride(1), ptr(value),
+        value.stride(0), value.stride(1), ptr(cu_seqlens_q), ptr(cu_seqlens_k), cu_seqlens_q.numel() - 1, tq, tk, h, hk,
+        d, bool(causal), sc, ptr(out), stream_of(query)), "attention_packed")
     return out

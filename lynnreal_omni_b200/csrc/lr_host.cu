@@ -43,6 +43,7 @@ int read_status_elementwise(unsigned int* bits, int clear);
 int read_status_gemm(unsigned int* bits, int clear);
 int read_status_flash(unsigned int* bits, int clear);
 int read_status_attention(unsigned int* bits, int clear);
+int read_status_packed(unsigned int* bits, int clear);
 
 }  // namespace lr
 
@@ -60,7 +61,9 @@ extern "C" int lr_device_status(unsigned int* bits, int clear) {
   if (st) return st;
   st = lr::read_status_flash(bits, clear);
   if (st) return st;
-  return lr::read_status_attention(bits, clear);
+  st = lr::read_status_attention(bits, clear);
+  if (st) return st;
+  return lr::read_status_packed(bits, clear);
 }
 
 // ------------------------------------------------------------- CUDA IPC

@@ -1,0 +1,93 @@
+"""Rotary positions of queries and keys: half and interleaved layouts, part of the head, scaled for long contexts.
+
+``rope_frequencies`` makes the frequencies once; ``rope`` turns the queries and keys of a batch of tokens at any
+positions. Unlike ``kernels.qk_norm_rope`` there is no norm, no table per position, and queries and keys may differ
+in their number of heads.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr, stream_of
+
+__all__ = ["rope_frequencies", "rope"]
+
+
+def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                     original_length: int = 4096, fast_turns: float = 32.0, slow_turns: float = 1.0, device="cuda"):
+    """(inv_freq fp32 [rotary_dim / 2] in radians per position, output factor).
+
+    f_i = base^(-2 i / rotary_dim), for contexts ``factor`` times as long as the ``original_length``:
+      * None: unscaled;
+      * "linear": f_i / factor;
+      * "ntk": the base grown to base * factor^(R / (R - 2)), so that the slowest frequency is divided by the factor
+        and the fastest is kept;
+      * "yarn": frequencies that make more than ``fast_turns`` turns over the original length are kept, those below
+        ``slow_turns`` divided by the factor, a linear ramp over the index between; outputs times 0.1 ln(factor) + 1.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rope_frequencies: rotary_dim must be positive and even, got {rotary_dim}")
+    if not (base > 1 and factor >= 1 and original_length > 0 and fast_turns > slow_turns > 0):
+        raise ValueError("rope_frequencies: base > 1, factor >= 1, original_length > 0, fast_turns > slow_turns > 0")
+    half = rotary_dim // 2
+    index = torch.arange(half, dtype=torch.float64)
+    output = 1.0
+    if scaling == "ntk" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv = base ** (-index / half)
+    if scaling == "linear" or (scaling == "ntk" and rotary_dim == 2):
+        inv = inv / factor
+    elif scaling == "yarn":
+        def crossing(turns):  # the (real) index whose frequency makes that many turns over the original length
+            return half * math.log(original_length / (2 * math.pi * turns)) / math.log(base)
+        low, high = max(math.floor(crossing(fast_turns)), 0), min(math.ceil(crossing(slow_turns)), half - 1)
+        divided = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - divided) + inv / factor * divided
+        output = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rope_frequencies: scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    return inv.to(device=device, dtype=torch.float32), output
+
+
+def _tokens_view(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, head_dim] with contiguous columns; a view wherever the strides allow."""
+    if t.stride(-1) != 1:
+        t = t.contiguous()
+    return t if t.ndim == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
+
+
+def rope(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+         interleaved: bool = False, factor: float = 1.0):
+    """Rotated (query, key), contiguous, in the inputs' shapes.
+
+    query [..., heads, D] and key [..., kv_heads, D] (or None): bf16, strided views of a fused projection are fine;
+    positions: int32 or int64, one per token; inv_freq: fp32 [rotary_dim / 2]. The first rotary_dim columns of each
+    head are turned, as pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1); the others are copied.
+    """
+    for name, t in (("query", query), ("key", key)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.ndim < 3 or t.device != query.device):
+            raise ValueError(f"rope: {name} must be a bf16 [..., heads, head_dim] tensor on the query's device")
+    q = _tokens_view(query)
+    k = None if key is None else _tokens_view(key)
+    tokens, heads, d = q.shape
+    if k is not None and (k.shape[0] != tokens or k.shape[2] != d):
+        raise ValueError("rope: query and key differ in tokens or head_dim")
+    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or inv_freq.device != query.device:
+        raise ValueError("rope: inv_freq must be an fp32 vector on the query's device")
+    if 2 * inv_freq.numel() > d:
+        raise ValueError(f"rope: {2 * inv_freq.numel()} rotary columns do not fit head_dim {d}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != query.device:
+        raise ValueError("rope: positions must be int32 or int64 on the query's device")
+    if positions.numel() != tokens:
+        raise ValueError(f"rope: {positions.numel()} positions for {tokens} tokens")
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    q_out = torch.empty(query.shape, device=query.device, dtype=torch.bfloat16)
+    k_out = None if key is None else torch.empty(key.shape, device=query.device, dtype=torch.bfloat16)
+    check(_lib.load().lr_rope(
+        ptr(q), q.stride(0), q.stride(1), heads, ptr(k), 0 if k is None else k.stride(0), 0 if k is None else k.stride(1),
+        0 if k is None else k.shape[1], ptr(positions), positions.dtype == torch.int64, ptr(inv_freq), float(factor),
+        tokens, d, 2 * inv_freq.numel(), bool(interleaved), ptr(q_out), ptr(k_out), stream_of(query)), "rope")
+    return q_out, k_out
