@@ -44,6 +44,7 @@ int read_status_gemm(unsigned int* bits, int clear);
 int read_status_flash(unsigned int* bits, int clear);
 int read_status_attention(unsigned int* bits, int clear);
 int read_status_packed(unsigned int* bits, int clear);
+int read_status_fp4(unsigned int* bits, int clear);
 
 }  // namespace lr
 
@@ -63,7 +64,9 @@ extern "C" int lr_device_status(unsigned int* bits, int clear) {
   if (st) return st;
   st = lr::read_status_attention(bits, clear);
   if (st) return st;
-  return lr::read_status_packed(bits, clear);
+  st = lr::read_status_packed(bits, clear);
+  if (st) return st;
+  return lr::read_status_fp4(bits, clear);
 }
 
 // ------------------------------------------------------------- CUDA IPC
