@@ -14,10 +14,13 @@
 // order, so no wait stands between them.
 //
 // Two kernels:
-//   * gemm_kernel (more than kFewRows rows): persistent, 128 x 192 (a CTA) or
-//     256 x 192 (a CTA pair) output tiles, two accumulators of 192 columns, so
-//     that the epilogue of a tile overlaps the next one's MMAs; 192 leaves 128
-//     of the 512 TMEM columns for the scales, which 256 would not.
+//   * gemm_kernel (more than kFewRows rows): persistent over CTA pairs, 256 x
+//     192 H output tiles in H = 1 or 2 units of 192 columns. Two accumulators
+//     of 192 columns leave 128 of the 512 TMEM columns for the scales. H = 1
+//     alternates between them, so that the epilogue of a tile overlaps the next
+//     one's MMAs; H = 2 uses both for one tile, which reads 30 % fewer bytes
+//     from L2 a product, and drains each into registers as packed bf16 before
+//     it hands it back.
 //   * few_rows_kernel: the weight takes the 128-row side and the few
 //     activation rows the narrow side; bound by reading the weight, K is split
 //     over a cluster's CTAs and joined through distributed shared memory, in a
@@ -37,12 +40,14 @@ using bf16 = __nv_bfloat16;
 
 constexpr int KB = 128;          // bytes of codes per row and stage (256 columns)
 constexpr int TM = 128;          // rows a CTA
-constexpr int TN = 192;          // columns a tile
-constexpr int kEpiWarps = 4;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int TN = 192;          // columns a unit (an accumulator)
+constexpr int kGroupWarps = 4;   // epilogue warps a unit, one per TMEM lane quadrant
+constexpr int kThreads = 64 + 2 * 32 * kGroupWarps;
+constexpr int kFewThreads = 64 + 32 * kGroupWarps;
 constexpr int kOutChunk = 32 * 32 * 2;  // a warp's 32 rows x 32 columns of bf16
 constexpr int kBarBytes = 1024;
 constexpr int kFewRows = 128;
+constexpr int kMaxSplits = 8;  // the largest portable cluster
 
 struct Epilogue {
   const float* row_scale;
@@ -65,7 +70,7 @@ constexpr uint32_t idesc(int m, int n) {
 
 // Shared-memory descriptor of a 512-byte scale tile: no swizzle, 8 rows of 16 bytes contiguous.
 __device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) |
+  return (uint64_t)(saddr >> 4) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) |
          ((uint64_t)1u << 46);
 }
 template <bool PAIR>
@@ -96,19 +101,22 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   }
 }
 
-// One stage: scales to tensor memory, then four MMAs. RB: 128-row scale tiles
-// of B; sfa, sfb: their columns in tensor memory; shift: column at which the
-// tile's first B row stands.
+// A stage's scales of 128-row tiles to tensor memory: A's to sfa (four columns a
+// tile of blocks), B's RB row tiles to sfb (4 RB columns a tile of blocks).
 template <int FORMAT, bool PAIR, int RB>
-__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t a0, uint32_t b0, uint32_t sa0, uint32_t sb0,
-                                            uint32_t sfa, uint32_t sfb, uint32_t shift, uint32_t desc, bool first) {
+__device__ __forceinline__ void issue_scales(uint32_t sa0, uint32_t sb0, uint32_t sfa, uint32_t sfb) {
   constexpr int CT = kScaleTiles<FORMAT>;
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     copy_scales<PAIR>(sfa + c * 4, sa0 + c * 512);
 #pragma unroll
-    for (int r = 0; r < RB; ++r) copy_scales<PAIR>(sfb + c * 4 * RB + r * 4, sb0 + (r * CT + c) * 512);
+    for (int r = 0; r < RB; ++r) copy_scales<PAIR>(sfb + (c * RB + r) * 4, sb0 + (r * CT + c) * 512);
   }
+}
+// A stage's four MMAs. shift: column at which the unit's first B row stands.
+template <int FORMAT, bool PAIR, int RB>
+__device__ __forceinline__ void issue_mmas(uint32_t d, uint32_t a0, uint32_t b0, uint32_t sfa, uint32_t sfb,
+                                           uint32_t shift, uint32_t desc, bool first) {
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     const int c = FORMAT == kNv ? kk : kk / 2;
@@ -120,19 +128,20 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint32_t a0, uint32_t b0
 }
 
 // ------------------------------------------------------------------ many rows
-template <int FORMAT, bool PAIR>
+template <int FORMAT, int H>
 struct Tile {
-  static constexpr int kBRows = PAIR ? TN / 2 : TN;
-  static constexpr int kA = TM * KB, kB = kBRows * KB;
-  static constexpr int kSa = kScaleTiles<FORMAT> * 512, kSb = 2 * kScaleTiles<FORMAT> * 512;
+  static constexpr int kRows = 2 * TM, kCols = H * TN;
+  static constexpr int kRB = H == 1 ? 2 : 3;  // 128-row scale tiles that 192 H rows of B touch
+  static constexpr int kA = TM * KB, kB = kCols / 2 * KB;  // a CTA loads its rows of A and half the rows of B
+  static constexpr int kSa = kScaleTiles<FORMAT> * 512, kSb = kRB * kScaleTiles<FORMAT> * 512;
   static constexpr int kStage = kA + kB + kSa + kSb;
-  static constexpr int kStages = PAIR ? 6 : 4;
-  static constexpr int kOut = kEpiWarps * 2 * kOutChunk;
-  static constexpr int kCols = 2 * TN * 8;  // (column scale, bias) of two tiles
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kOut + kCols + kBarBytes;
+  static constexpr int kStages = H == 1 ? 5 : 4;
+  static constexpr int kOut = 2 * kGroupWarps * kOutChunk;
+  static constexpr int kColBytes = 4 * TN * 8;  // (column scale, bias), two units a group
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kOut + kColBytes + kBarBytes;
   static_assert(kStage % 1024 == 0 && kSmem <= 232448, "shared memory");
   // tensor memory: accumulators at 0 and TN, scales of two stages from 2 TN
-  static constexpr int kSfCols = kScaleTiles<FORMAT> * 12;
+  static constexpr int kSfCols = kScaleTiles<FORMAT> * 4 * (1 + kRB);
   static_assert(2 * TN + 2 * kSfCols <= 512, "tensor memory");
 };
 
@@ -147,45 +156,43 @@ __device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int gro
   nb = r / size;
 }
 
-// All epilogue warps meet; true if every one of them brought `ok`.
-__device__ __forceinline__ bool epilogue_barrier(bool ok) {
+// The 128 threads of an epilogue group meet; true if every one of them brought `ok`.
+__device__ __forceinline__ bool group_barrier(int group, bool ok) {
   uint32_t all;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.and.pred q, %1, 128, p;\n\t"
                "selp.u32 %0, 1, 0, q;\n\t}\n"
                : "=r"(all)
-               : "r"(ok ? 1u : 0u)
+               : "r"(1 + group), "r"(ok ? 1u : 0u)
                : "memory");
   return all != 0;
 }
 
-template <int FORMAT, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int FORMAT, int H>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                 const __grid_constant__ CUtensorMap map_out, int M, int N, int K, int group, int tma_out,
                 const Epilogue ep) {
-  using C = Tile<FORMAT, PAIR>;
+  using C = Tile<FORMAT, H>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* out_stage = smem + C::kStages * C::kStage;
   float2* cols = reinterpret_cast<float2*>(out_stage + C::kOut);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(out_stage + C::kOut + C::kCols);
-  uint64_t* full = bars;                   // copies landed (the leader's, of both CTAs)
-  uint64_t* empty = bars + C::kStages;     // MMAs have read the stage
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_stage + C::kOut + C::kColBytes);
+  uint64_t* full = bars;                    // the leader's: both CTAs' copies landed
+  uint64_t* empty = bars + C::kStages;      // MMAs have read the stage
   uint64_t* tfull = bars + 2 * C::kStages;  // [2] accumulator ready
-  uint64_t* tempty = tfull + 2;             // [2] accumulator drained (the leader's)
+  uint64_t* tempty = tfull + 2;             // [2] the leader's: accumulator drained
   uint64_t* drain = tfull + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   const Watch watch{tmem_slot + 1, &g_fp4_status};
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0;
-  constexpr int kRows = PAIR ? 2 * TM : TM;
-  const int num_m = (M + kRows - 1) / kRows, num_n = (N + TN - 1) / TN;
+  const uint32_t rank = cluster_rank();
+  const int num_m = (M + C::kRows - 1) / C::kRows, num_n = (N + C::kCols - 1) / C::kCols;
   const int tiles = num_m * num_n;
   const int kblocks = (K / 2 + KB - 1) / KB;
-  const int first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-  const int step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int first_tile = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&tfull[a]), 1);
-      mbar_init(smem_u32(&tempty[a]), (PAIR ? 2 : 1) * kEpiWarps);
+      mbar_init(smem_u32(&tempty[a]), 2 * kGroupWarps);
     }
     mbar_init(smem_u32(drain), 1);
     *watch.abort_flag = 0u;
@@ -204,163 +211,164 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_sa);
     prefetch_map(&map_sb);
   }
-  if (warp == 1) tmem_alloc<PAIR ? 2 : 1>(smem_u32(tmem_slot), 512);
+  if (warp == 1) tmem_alloc<2>(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();
+  cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ------------------------------------------------------ copies
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true, any = false;
-      for (int t = first_tile; t < tiles && ok; t += step) {
-        int mb, nb;
-        tile_coords(t, num_m, num_n, group, mb, nb);
-        const int m0 = mb * kRows + (int)rank * TM, n0 = nb * TN;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, watch)) {
-            ok = false;
-            break;
-          }
-          const uint32_t a = smem_u32(smem + stage * C::kStage), b = a + C::kA, sa = b + C::kB, sb = sa + C::kSa;
-          uint32_t bar = smem_u32(&full[stage]);
-          if (rank == 0) mbar_expect_tx(bar, (PAIR ? 2 : 1) * C::kStage);
-          if (PAIR) {
-            bar = map_to_rank(bar, 0);
-            tma_load_2d_pair(a, &map_a, bar, kb * KB, m0);
-            tma_load_2d_pair(b, &map_b, bar, kb * KB, n0 + (int)rank * C::kBRows);
-            tma_load_3d_pair(sa, &map_sa, bar, 0, kb * kScaleTiles<FORMAT>, m0 / 128);
-            tma_load_3d_pair(sb, &map_sb, bar, 0, kb * kScaleTiles<FORMAT>, n0 / 128);
-          } else {
-            tma_load_2d(a, &map_a, bar, kb * KB, m0);
-            tma_load_2d(b, &map_b, bar, kb * KB, n0);
-            tma_load_3d(sa, &map_sa, bar, 0, kb * kScaleTiles<FORMAT>, m0 / 128);
-            tma_load_3d(sb, &map_sb, bar, 0, kb * kScaleTiles<FORMAT>, n0 / 128);
-          }
-          any = true;
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      if (!ok && any) {
-        // giving up: time for the copies in flight to land before the CTA can exit
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 100000ull) {
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      // ------------------------------------------------------ MMAs
-      int stage = 0, local = 0;
-      uint32_t phase = 0, buffer = 0;
-      bool ok = true;
-      constexpr uint32_t kDesc = idesc<FORMAT>(kRows, TN);
-      for (int t = first_tile; t < tiles && ok; t += step, ++local) {
-        int mb, nb;
-        tile_coords(t, num_m, num_n, group, mb, nb);
-        const uint32_t shift = (uint32_t)(nb * TN % 128 / 32);  // a tile starts at row 0 or 64 of B's scale tile
-        const int acc = local & 1;
-        if (!wait_bounded(smem_u32(&tempty[acc]), ((uint32_t)(local >> 1) & 1u) ^ 1u, watch)) {
+    // -------------------------------------------------------- copies
+    const bool el = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = first_tile; t < tiles && ok; t += step) {
+      int mb, nb;
+      tile_coords(t, num_m, num_n, group, mb, nb);
+      const int m0 = mb * C::kRows + (int)rank * TM, n0 = nb * C::kCols;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!warp_wait(smem_u32(&empty[stage]), phase ^ 1u, watch, lane)) {
           ok = false;
           break;
         }
-        tc_fence_after();
+        if (el) {
+          const uint32_t a = smem_u32(smem + stage * C::kStage), b = a + C::kA, sa = b + C::kB, sb = sa + C::kSa;
+          const uint32_t own = smem_u32(&full[stage]);
+          if (rank == 0) mbar_expect_tx(own, 2 * C::kStage);
+          const uint32_t bar = map_to_rank(own, 0);
+          tma_load_2d_pair(a, &map_a, bar, kb * KB, m0);
+          // unit u of B (192 rows): rows [96 rank, +96) of it
+#pragma unroll
+          for (int u = 0; u < H; ++u)
+            tma_load_2d_pair(b + u * (TN / 2) * KB, &map_b, bar, kb * KB, n0 + u * TN + (int)rank * (TN / 2));
+          tma_load_3d_pair(sa, &map_sa, bar, 0, kb * kScaleTiles<FORMAT>, m0 / 128);
+          tma_load_3d_pair(sb, &map_sb, bar, 0, kb * kScaleTiles<FORMAT>, n0 / 128);
+        }
+        __syncwarp();
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      // giving up: time for the copies in flight to land before the CTA can exit
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 100000ull) {
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      // ------------------------------------------------------ MMAs
+      const bool el = elect_one();
+      int stage = 0, local = 0;
+      uint32_t phase = 0, buffer = 0;
+      bool ok = true;
+      constexpr uint32_t kDesc = idesc<FORMAT>(C::kRows, TN);
+      for (int t = first_tile; t < tiles && ok; t += step, ++local) {
+        int mb, nb;
+        tile_coords(t, num_m, num_n, group, mb, nb);
+        // H = 1: a unit starts at row 0 or 64 of its scale tile. H = 2: unit 1 starts 192 rows in.
+        const uint32_t shift = H == 1 ? (uint32_t)(nb * TN % 128 / 32) : 0u;
+        const int acc = H == 1 ? local & 1 : 0;
+        const uint32_t parity = (H == 1 ? (uint32_t)(local >> 1) & 1u : (uint32_t)local & 1u) ^ 1u;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_bounded(smem_u32(&full[stage]), phase, watch)) {
+          if (!warp_wait(smem_u32(&full[stage]), phase, watch, lane) ||
+              (kb == 0 && !warp_wait(smem_u32(&tempty[acc]), parity, watch, lane))) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t a = smem_u32(smem + stage * C::kStage), b = a + C::kA, sa = b + C::kB, sb = sa + C::kSa;
-          const uint32_t sf = tmem + 2 * TN + buffer * C::kSfCols;
-          issue_stage<FORMAT, PAIR, 2>(tmem + acc * TN, a, b, sa, sb, sf, sf + kScaleTiles<FORMAT> * 4, shift, kDesc,
-                                       kb == 0);
-          buffer ^= 1u;
-          if (PAIR)
+          const uint32_t sfa = tmem + 2 * TN + buffer * C::kSfCols, sfb = sfa + kScaleTiles<FORMAT> * 4;
+          if (el) {
+            issue_scales<FORMAT, true, C::kRB>(sa, sb, sfa, sfb);
+            issue_mmas<FORMAT, true, C::kRB>(tmem + acc * TN, a, b, sfa, sfb, shift, kDesc, kb == 0);
+          }
+          if (H == 2) {
+            if (kb == 0) {
+              if (!warp_wait(smem_u32(&tempty[1]), parity, watch, lane)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+            }
+            if (el) {
+              if (kb == kblocks - 1) mma_commit_pair(smem_u32(&tfull[0]), (uint16_t)3);
+              issue_mmas<FORMAT, true, C::kRB>(tmem + TN, a, b + (TN / 2) * KB, sfa, sfb, TN / 32, kDesc, kb == 0);
+            }
+          }
+          if (el) {
             mma_commit_pair(smem_u32(&empty[stage]), (uint16_t)3);
-          else
-            mma_commit(smem_u32(&empty[stage]));
+            if (kb == kblocks - 1) mma_commit_pair(smem_u32(&tfull[H == 1 ? acc : 1]), (uint16_t)3);
+          }
+          __syncwarp();
+          buffer ^= 1u;
           if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) {
-          if (PAIR)
-            mma_commit_pair(smem_u32(&tfull[acc]), (uint16_t)3);
-          else
-            mma_commit(smem_u32(&tfull[acc]));
-        }
       }
       if (!ok) {
-        if (PAIR)
-          mma_commit_pair(smem_u32(drain), (uint16_t)1);
-        else
-          mma_commit(smem_u32(drain));
+        if (el) mma_commit_pair(smem_u32(drain), (uint16_t)1);
+        __syncwarp();
         drain_bounded(smem_u32(drain), 0u);
       }
     }
   } else {
     // -------------------------------------------------------- epilogue
-    const int quad = warp & 3;  // TMEM lanes 32 quad .. + 32
-    uint8_t* staging = out_stage + (warp - 2) * 2 * kOutChunk;
-    uint32_t chunk = 0;
-    int local = 0;
-    for (int t = first_tile; t < tiles; t += step, ++local) {
-      const int acc = local & 1;
+    // Group g drains accumulator g: every other tile (H = 1) or unit g of every tile (H = 2).
+    const int g = (warp - 2) / kGroupWarps, quad = warp & 3;  // TMEM lanes 32 quad .. + 32
+    uint8_t* buf = out_stage + (warp - 2) * kOutChunk;
+    int turn = 0;
+    for (int t = first_tile + (H == 1 ? g * step : 0); t < tiles; t += H == 1 ? 2 * step : step, ++turn) {
       int mb, nb;
       tile_coords(t, num_m, num_n, group, mb, nb);
-      const int n0 = nb * TN;
-      const int row0 = mb * kRows + (int)rank * TM + quad * 32, row = row0 + lane;
-      float2* cs = cols + acc * TN;
-      for (int i = threadIdx.x - 64; i < TN; i += 32 * kEpiWarps) {
+      const int n0 = nb * C::kCols + (H == 1 ? 0 : g * TN);
+      const int row0 = mb * C::kRows + (int)rank * TM + quad * 32, row = row0 + lane;
+      float2* cs = cols + (g * 2 + (turn & 1)) * TN;
+      for (int i = quad * 32 + lane; i < TN; i += 32 * kGroupWarps) {
         const int n = n0 + i;
         cs[i] = make_float2(n < N && ep.col_scale ? ep.col_scale[n] : 1.0f,
                             n < N && ep.bias ? __bfloat162float(ep.bias[n]) : 0.0f);
       }
       const float rs = row < M && ep.row_scale ? ep.row_scale[row] : 1.0f;
-      const bool ok = warp_wait(smem_u32(&tfull[acc]), (uint32_t)(local >> 1) & 1u, watch, lane);
-      if (!epilogue_barrier(ok)) break;
+      const bool ok = warp_wait(smem_u32(&tfull[g]), (uint32_t)turn & 1u, watch, lane);
+      if (!group_barrier(g, ok)) break;
       tc_fence_after();
-      const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * TN);
-#pragma unroll 1
+      uint32_t y[TN / 2];
+      const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(g * TN);
+#pragma unroll
       for (int c = 0; c < TN / 32; ++c) {
         uint32_t r[32];
         tmem_ld32(tbase + (uint32_t)(c * 32), r);
         if (c == TN / 32 - 1) {  // everything is in registers: hand the accumulator back
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if (PAIR)
-              mbar_arrive_cluster(smem_u32(&tempty[acc]), 0u);
-            else
-              mbar_arrive(smem_u32(&tempty[acc]));
-          }
+          if (lane == 0) mbar_arrive_cluster(smem_u32(&tempty[g]), 0u);
         }
-        const int col0 = n0 + c * 32;
-        if (col0 >= N) continue;
-        uint32_t y[16];
         const float4* c4 = reinterpret_cast<const float4*>(cs + c * 32);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float4 f = c4[e];  // two columns' (scale, bias)
-          y[e] = cvt2(fmaf(__uint_as_float(r[2 * e]) * rs, f.x, f.y), fmaf(__uint_as_float(r[2 * e + 1]) * rs, f.z, f.w));
+          y[c * 16 + e] =
+              cvt2(fmaf(__uint_as_float(r[2 * e]) * rs, f.x, f.y), fmaf(__uint_as_float(r[2 * e + 1]) * rs, f.z, f.w));
         }
+      }
+#pragma unroll
+      for (int c = 0; c < TN / 32; ++c) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= N) break;
         // rows to this warp's staging buffer, 64-byte swizzle: conflict-free 16-byte writes
-        uint8_t* buf = staging + (chunk & 1u) * kOutChunk;
-        if (tma_out && lane == 0) bulk_wait_read1();
+        if (tma_out && lane == 0) bulk_wait_read();
         __syncwarp();
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
-              make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+          *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(
+              y[c * 16 + 4 * q], y[c * 16 + 4 * q + 1], y[c * 16 + 4 * q + 2], y[c * 16 + 4 * q + 3]);
         if (tma_out) {
           fence_async_smem();
           __syncwarp();
@@ -375,7 +383,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               ep.out[(int64_t)(row0 + i) * ep.ldo + col0 + lane] = *reinterpret_cast<const bf16*>(
                   buf + i * 64 + ((((uint32_t)lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2);
         }
-        ++chunk;
       }
     }
     if (tma_out && lane == 0) bulk_wait_all();
@@ -384,10 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<PAIR ? 2 : 1>(tmem, 512);
+    tmem_dealloc<2>(tmem, 512);
   }
 }
 
@@ -397,18 +404,18 @@ struct Few {
   static constexpr int kA = TM * KB, kB = NT * KB;
   static constexpr int kS = kScaleTiles<FORMAT> * 512;
   static constexpr int kStage = kA + kB + 2 * kS;
-  static constexpr int kStages = 4;
+  static constexpr int kStages = NT <= 32 ? 4 : 3;  // two CTAs an SM
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kBarBytes;
   static constexpr int kSfCols = kScaleTiles<FORMAT> * 8;
   static constexpr int kTmem = NT <= 64 ? 128 : 256;
-  static_assert(kStage % 1024 == 0 && NT + 2 * kSfCols <= kTmem && kSmem <= 232448, "budgets");
+  static_assert(kStage % 1024 == 0 && NT + 2 * kSfCols <= kTmem && 2 * (kSmem + 1024) <= 233472, "two CTAs an SM");
   static_assert(TM * NT * 4 <= kStages * kStage, "the partial tile reuses the stages");
 };
 
-// Weight rows [128 x, +128) against activation rows [NT y, +NT); the cluster's
+// Weight rows [128 x, +128) against the M <= NT activation rows; the cluster's
 // CTAs take consecutive slices of K.
 template <int FORMAT, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kFewThreads)
     few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_sx, int M, int N,
                     int K, int splits, const Epilogue ep) {
@@ -425,7 +432,7 @@ __global__ void __launch_bounds__(kThreads)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
-  const int n0 = (int)(blockIdx.x / splits) * TM, m0 = (int)blockIdx.y * NT;
+  const int n0 = (int)(blockIdx.x / splits) * TM;
   const int kblocks = (K / 2 + KB - 1) / KB;
   const int kb0 = (int)((int64_t)kblocks * rank / splits), kb1 = (int)((int64_t)kblocks * (rank + 1) / splits);
 
@@ -449,73 +456,76 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  bool ok = true;
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, watch)) {
-          ok = false;
-          break;
-        }
+    const bool el = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(smem_u32(&empty[stage]), phase ^ 1u, watch, lane)) {
+        ok = false;
+        break;
+      }
+      if (el) {
         const uint32_t a = smem_u32(smem + stage * C::kStage), b = a + C::kA, sa = b + C::kB, sb = sa + C::kS;
         const uint32_t bar = smem_u32(&full[stage]);
         mbar_expect_tx(bar, C::kStage);
         tma_load_2d(a, &map_w, bar, kb * KB, n0);
-        tma_load_2d(b, &map_x, bar, kb * KB, m0);
+        tma_load_2d(b, &map_x, bar, kb * KB, 0);
         tma_load_3d(sa, &map_sw, bar, 0, kb * kScaleTiles<FORMAT>, n0 / 128);
-        tma_load_3d(sb, &map_sx, bar, 0, kb * kScaleTiles<FORMAT>, m0 / 128);
-        if (++stage == C::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        tma_load_3d(sb, &map_sx, bar, 0, kb * kScaleTiles<FORMAT>, 0);
       }
-      if (!ok) {
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 100000ull) {
-        }
+      __syncwarp();
+      if (++stage == C::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (!ok) {
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 100000ull) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, buffer = 0;
-      constexpr uint32_t kDesc = idesc<FORMAT>(TM, NT);
-      const uint32_t shift = (uint32_t)(m0 % 128 / 32);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait_bounded(smem_u32(&full[stage]), phase, watch)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+    const bool el = elect_one();
+    int stage = 0;
+    uint32_t phase = 0, buffer = 0;
+    bool ok = true;
+    constexpr uint32_t kDesc = idesc<FORMAT>(TM, NT);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(smem_u32(&full[stage]), phase, watch, lane)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (el) {
         const uint32_t a = smem_u32(smem + stage * C::kStage), b = a + C::kA, sa = b + C::kB, sb = sa + C::kS;
-        const uint32_t sf = tmem + NT + buffer * C::kSfCols;
-        issue_stage<FORMAT, false, 1>(tmem, a, b, sa, sb, sf, sf + kScaleTiles<FORMAT> * 4, shift, kDesc, kb == kb0);
-        buffer ^= 1u;
+        const uint32_t sfa = tmem + NT + buffer * C::kSfCols, sfb = sfa + kScaleTiles<FORMAT> * 4;
+        issue_scales<FORMAT, false, 1>(sa, sb, sfa, sfb);
+        issue_mmas<FORMAT, false, 1>(tmem, a, b, sfa, sfb, 0u, kDesc, kb == kb0);
         mma_commit(smem_u32(&empty[stage]));
-        if (++stage == C::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (kb == kb1 - 1) mma_commit(smem_u32(done));
       }
-      if (ok) {
-        mma_commit(smem_u32(done));
-      } else {
-        mma_commit(smem_u32(drain));
-        drain_bounded(smem_u32(drain), 0u);
+      __syncwarp();
+      buffer ^= 1u;
+      if (++stage == C::kStages) {
+        stage = 0;
+        phase ^= 1u;
       }
+    }
+    if (!ok) {
+      if (el) mma_commit(smem_u32(drain));
+      __syncwarp();
+      drain_bounded(smem_u32(drain), 0u);
     }
   } else {
     // The partial tile, [activation row][weight row] fp32, over the stages (every copy into them has been read).
     const int quad = warp & 3;
-    ok = warp_wait(smem_u32(done), 0u, watch, lane);
-    if (ok) {
+    if (warp_wait(smem_u32(done), 0u, watch, lane)) {
       tc_fence_after();
       float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
-      const int live = min(NT, M - m0);
-#pragma unroll 1
-      for (int c = 0; c < live; c += 16) {
+      #pragma unroll 1
+      for (int c = 0; c < M; c += 16) {
         uint32_t r[16];
         tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, r);
 #pragma unroll
@@ -528,23 +538,41 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   if (splits > 1) cluster_sync_all();
   if (warp >= 2) {
-    // Activation rows rank, rank + splits, ...: the slices' sums added in order.
-    const int quad = warp & 3, n = n0 + quad * 32 + lane;
-    const float cs = n < N && ep.col_scale ? ep.col_scale[n] : 1.0f;
-    const float b = n < N && ep.bias ? __bfloat162float(ep.bias[n]) : 0.0f;
-    const uint32_t part = smem_u32(smem) + (uint32_t)(quad * 32 + lane) * 4;
-    for (int i = rank; i < NT && m0 + i < M; i += splits) {
-      float y = 0.0f;
-      for (int s = 0; s < splits; ++s) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                     : "=f"(v)
-                     : "r"(map_to_rank(part + (uint32_t)i * TM * 4, (uint32_t)s))
-                     : "memory");
-        y += v;
+    // A warp an activation row, a lane four outputs; the slices' sums are fetched together and added in order.
+    const int n = n0 + lane * 4;
+    float cs[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cs[e] = n + e < N && ep.col_scale ? ep.col_scale[n + e] : 1.0f;
+      b[e] = n + e < N && ep.bias ? __bfloat162float(ep.bias[n + e]) : 0.0f;
+    }
+    const bool whole = n + 4 <= N && ep.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(ep.out) & 7) == 0;
+    for (int i = rank + (warp - 2) * splits; i < M; i += kGroupWarps * splits) {
+      const uint32_t part = smem_u32(smem) + (uint32_t)(i * TM + lane * 4) * 4;
+      float4 v[kMaxSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) {
+        v[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (s < splits)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                       : "r"(map_to_rank(part, (uint32_t)s))
+                       : "memory");
       }
-      if (ep.row_scale) y *= ep.row_scale[m0 + i];
-      if (n < N) ep.out[(int64_t)(m0 + i) * ep.ldo + n] = __float2bfloat16_rn(fmaf(y, cs, b));
+      float y[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int s = 1; s < kMaxSplits; ++s) y[0] += v[s].x, y[1] += v[s].y, y[2] += v[s].z, y[3] += v[s].w;
+      const float rs = ep.row_scale ? ep.row_scale[i] : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e] * rs, cs[e], b[e]);
+      bf16* dst = ep.out + (int64_t)i * ep.ldo + n;
+      if (whole) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(cvt2(y[0], y[1]), cvt2(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < N) dst[e] = __float2bfloat16_rn(y[e]);
+      }
     }
   }
   __syncwarp();
@@ -576,13 +604,13 @@ struct Operands {
   int M, N, K;
 };
 
-template <int FORMAT, bool PAIR>
+template <int FORMAT, int H>
 int launch_many(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
-  using C = Tile<FORMAT, PAIR>;
+  using C = Tile<FORMAT, H>;
   CUtensorMap ma, mb, msa, msb, mo{};
   int st;
-  if ((st = code_map(&ma, o.a, o.M, o.K, TM)) || (st = code_map(&mb, o.b, o.N, o.K, C::kBRows)) ||
-      (st = scale_map<FORMAT>(&msa, o.as, o.M, o.K, 1)) || (st = scale_map<FORMAT>(&msb, o.bs, o.N, o.K, 2)))
+  if ((st = code_map(&ma, o.a, o.M, o.K, TM)) || (st = code_map(&mb, o.b, o.N, o.K, TN / 2)) ||
+      (st = scale_map<FORMAT>(&msa, o.as, o.M, o.K, 1)) || (st = scale_map<FORMAT>(&msb, o.bs, o.N, o.K, C::kRB)))
     return st;
   const int tma_out = ep.ldo % 8 == 0 && aligned(ep.out, 16);
   if (tma_out) {
@@ -592,26 +620,13 @@ int launch_many(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
       return st;
   }
   static bool done[64] = {};
-  if ((st = configure_smem(gemm_kernel<FORMAT, PAIR>, C::kSmem, done))) return st;
-  constexpr int kRows = PAIR ? 2 * TM : TM;
-  const int num_m = (o.M + kRows - 1) / kRows, num_n = (o.N + TN - 1) / TN;
-  const int64_t tiles = (int64_t)num_m * num_n;
-  const int workers = PAIR ? sm_count() / 2 : sm_count();
-  const int grid = (PAIR ? 2 : 1) * (int)(tiles < workers ? tiles : workers);
-  int64_t group = (24ll << 20) / ((int64_t)kRows * o.K / 2);  // 24 MB of A's codes
+  if ((st = configure_smem(gemm_kernel<FORMAT, H>, C::kSmem, done))) return st;
+  const int num_m = (o.M + C::kRows - 1) / C::kRows, num_n = (o.N + C::kCols - 1) / C::kCols;
+  const int tiles = num_m * num_n, pairs = sm_count() / 2;
+  int64_t group = (24ll << 20) / ((int64_t)C::kRows * o.K / 2);  // 24 MB of A's codes
   if (group < 1) group = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {PAIR ? 2u : 1u, 1, 1};
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, gemm_kernel<FORMAT, PAIR>, ma, mb, msa, msb, mo, o.M, o.N, o.K,
-                     (int)(group < num_m ? group : num_m), tma_out, ep);
+  gemm_kernel<FORMAT, H><<<2 * (tiles < pairs ? tiles : pairs), kThreads, C::kSmem, stream>>>(
+      ma, mb, msa, msb, mo, o.M, o.N, o.K, (int)(group < num_m ? group : num_m), tma_out, ep);
   return launch_status("fp4 gemm");
 }
 
@@ -625,14 +640,14 @@ int launch_few(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
     return st;
   static bool done[64] = {};
   if ((st = configure_smem(few_rows_kernel<FORMAT, NT>, C::kSmem, done))) return st;
-  const int tiles = ((o.N + TM - 1) / TM) * ((o.M + NT - 1) / NT);
+  const int tiles = (o.N + TM - 1) / TM;
   const int kblocks = (o.K / 2 + KB - 1) / KB;
   // as many slices as fill the GPU with two CTAs an SM and leave each two stages
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * sm_count() && kblocks >= 4 * splits) splits *= 2;
+  while (splits < kMaxSplits && tiles * splits * 2 <= 2 * sm_count() && kblocks >= 4 * splits) splits *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((o.N + TM - 1) / TM * splits), (unsigned)((o.M + NT - 1) / NT));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(tiles * splits));
+  cfg.blockDim = dim3(kFewThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute at{};
@@ -650,7 +665,12 @@ int gemm(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
   if (o.M <= 32) return launch_few<FORMAT, 32>(o, ep, stream);
   if (o.M <= 64) return launch_few<FORMAT, 64>(o, ep, stream);
   if (o.M <= kFewRows) return launch_few<FORMAT, 128>(o, ep, stream);
-  return launch_many<FORMAT, true>(o, ep, stream);
+  // a wide tile takes about 1.4 times a narrow one's time for twice its columns
+  const int64_t pairs = sm_count() / 2, num_m = (o.M + 2 * TM - 1) / (2 * TM);
+  const int64_t narrow = (num_m * ((o.N + TN - 1) / TN) + pairs - 1) / pairs;
+  const int64_t wide = (num_m * ((o.N + 2 * TN - 1) / (2 * TN)) + pairs - 1) / pairs;
+  if (wide * 7 <= narrow * 5) return launch_many<FORMAT, 2>(o, ep, stream);
+  return launch_many<FORMAT, 1>(o, ep, stream);
 }
 
 }  // namespace

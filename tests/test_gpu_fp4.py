@@ -186,7 +186,8 @@ def check_product(m, n, k, format, seed=0, scales=True, bias=True):
 @pytest.mark.parametrize("format", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 200, 64), (3, 129, 96), (17, 192, 256), (64, 193, 288), (65, 384, 512),
                                    (127, 64, 1024), (128, 128, 128), (129, 576, 320), (200, 1000, 160), (257, 40, 2080),
-                                   (300, 777, 544), (1, 4099, 1056), (33, 640, 4096), (513, 385, 256)])
+                                   (300, 777, 544), (1, 4099, 1056), (33, 640, 4096), (513, 385, 256), (1500, 12000, 96),
+                                   (1300, 12003, 544)])
 def test_product(m, n, k, format):
     check_product(m, n, k, format, seed=m + n + k)
 
