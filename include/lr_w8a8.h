@@ -241,7 +241,13 @@ int lr_attention_packed(const void* q, int64_t q_token_stride, int64_t q_head_st
                         int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                         int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs,
                         int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                        int causal, float scale, void* out, void* stream);
+                        int causal, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* Bytes of workspace that lr_attention_packed needs for these counts (0: none;
+ * only calls with a few queries a sequence split their keys and need some). */
+int64_t lr_attention_packed_workspace_bytes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads,
+                                            int64_t kv_heads, int64_t head_dim);
 
 /* R1 — rotary position embedding of q and k (bf16), no tables: the pair of
  * frequency i of a token at position p is turned by p * inv_freq[i] radians

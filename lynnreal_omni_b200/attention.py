@@ -97,8 +97,11 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     query, key, value = _head_view(query), _head_view(key), _head_view(value)
     out = torch.empty((tq, h, d), device=query.device, dtype=torch.bfloat16)
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    check(_lib.load().lr_attention_packed(
+    lib, seqs = _lib.load(), cu_seqlens_q.numel() - 1
+    need = lib.lr_attention_packed_workspace_bytes(seqs, tq, tk, h, hk, d)
+    workspace = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None
+    check(lib.lr_attention_packed(
         ptr(query), query.stride(0), query.stride(1), ptr(key), key.stride(0), key.stride(1), ptr(value),
-        value.stride(0), value.stride(1), ptr(cu_seqlens_q), ptr(cu_seqlens_k), cu_seqlens_q.numel() - 1, tq, tk, h, hk,
-        d, bool(causal), sc, ptr(out), stream_of(query)), "attention_packed")
+        value.stride(0), value.stride(1), ptr(cu_seqlens_q), ptr(cu_seqlens_k), seqs, tq, tk, h, hk, d, bool(causal), sc,
+        ptr(out), ptr(workspace), need, stream_of(query)), "attention_packed")
     return out
