@@ -85,15 +85,41 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // ------------------------------------------------------------------ prompts
 constexpr int kRows = 128;    // rows of a query tile (TMEM lanes)
 constexpr int kKeys = 128;    // keys of a tile
+constexpr int kHalf = 64;     // keys whose probabilities are handed over together
 constexpr int kAtom = 128 * 128;  // 128 rows x 64 columns, 128-byte swizzle
 constexpr int kPromptThreads = 384;
+
+// Largest scaled score of 64 (of the first `valid` of them).
+template <bool MASKED>
+__device__ __forceinline__ float half_maximum(const uint32_t* s, float scale, int valid) {
+  if constexpr (MASKED) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+      if (e < valid) mx = fmaxf(mx, __uint_as_float(s[e]) * scale);
+    return mx;
+  } else {
+  float m4[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m4[e] = __uint_as_float(s[e]);
+  if (scale >= 0.0f) {
+#pragma unroll
+    for (int e = 4; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(s[e]));
+    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
+  }
+#pragma unroll
+  for (int e = 4; e < 64; ++e) m4[e & 3] = fminf(m4[e & 3], __uint_as_float(s[e]));
+  return fminf(fminf(m4[0], m4[1]), fminf(m4[2], m4[3])) * scale;
+  }
+}
 
 template <int D>
 struct Prompt {
   static constexpr int kTile = D / 64 * kAtom;
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kQ = 0, kRing = 2 * kTile, kBars = kRing + kSlots * kTile;
-  static constexpr size_t kSmem = 1024 + kBars + 512;
+  static constexpr int kBarBytes = 768;  // barriers and items
+  static constexpr size_t kSmem = 1024 + kBars + kBarBytes;
   static constexpr uint32_t kColO = 256;  // scores of tile t at 128 t, output of tile t at 256 + D t
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -175,27 +201,85 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// Of every kEvery pairs of a full tile, one goes through exp2_poly2 (the special
-// function unit is as busy as the tensor core otherwise).
-#ifndef LR_PACKED_EMU
-#define LR_PACKED_EMU 4
-#endif
+// One pair in `kPolyEvery` of a full tile goes through exp2_poly2: the special
+// function unit (16 values a cycle) is as busy as the tensor core otherwise. At
+// 64 columns, where the products take half as long, one in three (8192 tokens:
+// 452 us without, 418 us one in four, 410 us one in three), at 128 one in four
+// (16384 tokens: 2066, 1955, 2030 us).
+template <int D>
+constexpr int kPolyEvery = D == 64 ? 3 : 4;
 
 struct PromptShape {
   int tokens_tile;  // query tokens of a tile
   int tile_heads;   // query heads of a tile (the group, or a part of a group above 128)
   int head_parts;   // tiles that a group is cut into
   int slots;
+  int items;        // slots * kv_heads * head_parts
+  int wide_out;     // out is 32-byte aligned
 };
 
+// A block of work: two query tiles of one key/value head (or a part of its group).
+struct PromptItem {
+  int q_row;       // first query token
+  int tok0;        // the same within its sequence
+  int lq, lk;      // lengths of the sequence
+  int k_row;       // first key
+  int kv_head, head0, heads_here;
+  int tiles[2];    // key tiles that each query tile sees
+};
+constexpr int kItemSlots = 4;
+
+// Work item `index`, or false for an empty slot. Later blocks of a sequence
+// see more keys and come first; the heads of a block stand side by side.
+__device__ __forceinline__ bool prompt_item(const Args& a, const PromptShape& ps, int index, int lane, PromptItem& w) {
+  const int parts = a.kv_heads * ps.head_parts;
+  const int part = index % parts;
+  const int slot = ps.slots - 1 - index / parts;
+  w.kv_head = part / ps.head_parts;
+  const int in_group = part % ps.head_parts * ps.tile_heads;
+  w.heads_here = min(ps.tile_heads, a.group - in_group);
+  w.head0 = w.kv_head * a.group + in_group;
+  const int block = 2 * ps.tokens_tile;
+  // "Sequence" a.seqs is what lies past the last offset: queries without keys.
+  int b, qs, qe, ke;
+  if (a.seqs < 32) {  // every offset in one lane: one round of loads
+    const int q = clamped(a.cu_q, min(lane, a.seqs), a.total_q), k = clamped(a.cu_k, min(lane, a.seqs), a.total_k);
+    const bool at = lane <= a.seqs && (int)((uint32_t)q / (uint32_t)block) + lane <= slot;
+    b = max(__popc(__ballot_sync(0xffffffffu, at)) - 1, 0);
+    qs = __shfl_sync(0xffffffffu, q, b);
+    qe = __shfl_sync(0xffffffffu, q, min(b + 1, a.seqs));
+    w.k_row = __shfl_sync(0xffffffffu, k, b);
+    ke = __shfl_sync(0xffffffffu, k, min(b + 1, a.seqs));
+  } else {
+    b = find_sequence(a.cu_q, a.seqs, a.total_q, block, slot, lane);
+    qs = clamped(a.cu_q, b, a.total_q);
+    qe = clamped(a.cu_q, min(b + 1, a.seqs), a.total_q);
+    w.k_row = clamped(a.cu_k, b, a.total_k);
+    ke = clamped(a.cu_k, min(b + 1, a.seqs), a.total_k);
+  }
+  if (b == a.seqs) qe = a.total_q;
+  w.lk = max(ke - w.k_row, 0);
+  w.lq = max(qe - qs, 0);
+  w.tok0 = (slot - (int)((uint32_t)qs / (uint32_t)block) - b) * block;
+  w.q_row = qs + w.tok0;
+  if (w.tok0 < 0 || w.tok0 >= w.lq) return false;  // below 0: offsets that go down
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = w.tok0 + t * ps.tokens_tile, last = min(first + ps.tokens_tile, w.lq) - 1;
+    const int seen = first >= w.lq ? 0 : a.causal ? min(max(last + w.lk - w.lq + 1, 0), w.lk) : w.lk;
+    w.tiles[t] = (seen + kKeys - 1) / kKeys;
+  }
+  return true;
+}
+
 // Probabilities of 64 scores (bf16 pairs into s[0..31]) and their sum.
-template <bool MASKED>
+template <bool MASKED, int D>
 __device__ __forceinline__ void probabilities(uint32_t* s, float2 sc2, float2 nm2, int valid, float2& sum) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, nm2);
     float2 p;
-    if (!MASKED && LR_PACKED_EMU > 0 && i % LR_PACKED_EMU == LR_PACKED_EMU - 1)
+    if (!MASKED && i % kPolyEvery<D> == kPolyEvery<D> - 1)
       p = exp2_poly2(x);
     else
       p = make_float2(ex2(x.x), ex2(x.y));
@@ -208,6 +292,22 @@ __device__ __forceinline__ void probabilities(uint32_t* s, float2 sc2, float2 nm
   }
 }
 
+// 16 bf16 values; rows lie far apart, so a lane's store should fill a 32-byte sector.
+__device__ __forceinline__ void store_16(bf16* dst, const uint32_t* y, int wide) {
+  if (wide)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(y[0]), "r"(y[1]), "r"(y[2]),
+                 "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                 : "memory");
+  else
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+}
+
+// Persistent, one CTA an SM; warp roles: 0 copies, 1 MMAs, 3 finds the items,
+// 4-7 and 8-11 the softmax of query tiles 0 and 1. While one item's last
+// products and its output are under way, the next one's queries and keys load
+// and its first scores are computed.
 template <int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -216,288 +316,329 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
-  uint64_t* q_full = bars;                    // [tile]
-  uint64_t* full = bars + 2;                  // [slot] K or V tile landed
-  uint64_t* empty = full + C::kSlots;         // [slot] read by all its MMAs
-  uint64_t* s_full = empty + C::kSlots;       // [tile] scores ready; the previous P V is done, too
-  uint64_t* p_full = s_full + 2;              // [tile] probabilities written, output rescaled
-  uint64_t* o_done = p_full + 2;              // [tile] last P V done
-  uint64_t* drain = o_done + 2;
+  uint64_t* q_full = bars;               // [tile] queries landed
+  uint64_t* q_empty = bars + 2;          // [tile] read by their last scores
+  uint64_t* full = bars + 4;             // [slot] K or V tile landed
+  uint64_t* empty = full + C::kSlots;    // [slot] read by all its MMAs
+  uint64_t* s_full = empty + C::kSlots;  // [tile] scores ready; the previous P V is done, too
+  uint64_t* p_half = s_full + 2;         // [tile] the second half's probabilities written, output rescaled
+  uint64_t* p_full = s_full + 4;         // [tile] all of them
+  uint64_t* o_done = s_full + 6;         // [tile] last P V of the item done
+  uint64_t* o_empty = s_full + 8;        // [tile] output read
+  uint64_t* i_full = s_full + 10;        // [item slot] published
+  uint64_t* i_empty = i_full + kItemSlots;  // [item slot] read by every role
+  uint64_t* drain = i_empty + kItemSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  PromptItem* items = reinterpret_cast<PromptItem*>(tmem_slot + 2);
+  static_assert((14 + 2 * C::kSlots + 2 * kItemSlots + 1) * 8 + 8 + kItemSlots * sizeof(PromptItem) <= C::kBarBytes, "barriers");
   const Watch watch{tmem_slot + 1, &g_packed_status};
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (blockIdx.x == 0 && warp == 3) check_offsets(a, lane, 32);
-
-  // Later blocks of a sequence see more keys and come first.
-  const int parts = a.kv_heads * ps.head_parts;
-  const int part = blockIdx.x % parts;
-  const int slot = ps.slots - 1 - (int)(blockIdx.x / parts);
-  const int kv_head = part / ps.head_parts;
-  const int head_in_group = part % ps.head_parts * ps.tile_heads;
-  const int heads_here = min(ps.tile_heads, a.group - head_in_group);
-  const int head0 = kv_head * a.group + head_in_group;
-  const int block = 2 * ps.tokens_tile;
-  // "Sequence" a.seqs is what lies past the last offset: queries without keys.
-  const int b = find_sequence(a.cu_q, a.seqs, a.total_q, block, slot, lane);
-  const int qs = clamped(a.cu_q, b, a.total_q);
-  const int qe = b < a.seqs ? max(clamped(a.cu_q, b + 1, a.total_q), qs) : a.total_q;
-  const int ks = b < a.seqs ? clamped(a.cu_k, b, a.total_k) : 0;
-  const int lq = qe - qs;
-  const int lk = b < a.seqs ? max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0) : 0;
-  const int tok0 = (slot - (int)((uint32_t)qs / (uint32_t)block) - b) * block;  // of the block, in the sequence
-  if (tok0 < 0 || tok0 >= lq) return;  // an empty slot (below 0: offsets that go down)
-  // Keys that a tile's last token sees, in tiles of keys.
-  int tiles[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = tok0 + t * ps.tokens_tile, last = min(first + ps.tokens_tile, lq) - 1;
-    const int seen = first >= lq ? 0 : a.causal ? min(max(last + lk - lq + 1, 0), lk) : lk;
-    tiles[t] = (seen + kKeys - 1) / kKeys;
-  }
-  const int most = max(tiles[0], tiles[1]);
-
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    prefetch_map(&map_q);
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&q_full[t]), 1);
+      mbar_init(smem_u32(&q_empty[t]), 1);
       mbar_init(smem_u32(&s_full[t]), 1);
+      mbar_init(smem_u32(&p_half[t]), 4);
       mbar_init(smem_u32(&p_full[t]), 4);
       mbar_init(smem_u32(&o_done[t]), 1);
+      mbar_init(smem_u32(&o_empty[t]), 4);
     }
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
     }
+    for (int s = 0; s < kItemSlots; ++s) {
+      mbar_init(smem_u32(&i_full[s]), 1);
+      mbar_init(smem_u32(&i_empty[s]), 10);  // copies, MMAs, eight softmax warps
+    }
     mbar_init(smem_u32(drain), 1);
     *watch.abort_flag = 0u;
     mbar_init_fence();
-    prefetch_map(&map_q);
-    prefetch_map(&map_k);
-    prefetch_map(&map_v);
   }
   if (warp == 1) tmem_alloc<1>(smem_u32(tmem_slot), 512);
+  // Items are dealt out forth and back, so that every CTA gets as many heavy ones.
+  auto item_index = [&](int round) {
+    return round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  };
+  PromptItem first{};
+  bool first_there = false;
+  if (warp == 3) first_there = prompt_item(a, ps, item_index(0), lane, first);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  // The ring holds K_0 V_0 K_1 V_1 ...; entry e is in slot e % kSlots.
-  auto entry_bar = [&](uint64_t* set, int e) { return smem_u32(&set[e % C::kSlots]); };
-  auto entry_addr = [&](int e) { return smem_u32(smem + C::kRing + (e % C::kSlots) * C::kTile); };
-  auto entry_phase = [&](int e) { return (uint32_t)(e / C::kSlots) & 1u; };
-  // The softmax warps hold a row of scores each: of the launch's 384 x 168 registers 128 x 72 stay here, 256 x 208 go there.
+  const uint32_t tmem = uniform(*tmem_slot);
+  // The ring holds K_0 V_0 K_1 V_1 ... of all items in turn; entry e is in slot e % kSlots.
+  auto entry_bar = [&](uint64_t* set, uint32_t e) { return smem_u32(&set[e % C::kSlots]); };
+  auto entry_addr = [&](uint32_t e) { return smem_u32(smem + C::kRing + (e % C::kSlots) * C::kTile); };
+  auto entry_phase = [&](uint32_t e) { return (e / C::kSlots) & 1u; };
+  // The next item, the number-th of this CTA; false at the end (no keys and no queries) or when giving up.
+  auto next_item = [&](uint32_t number, PromptItem& w) {
+    const uint32_t s = number % kItemSlots;
+    if (!warp_wait(smem_u32(&i_full[s]), (number / kItemSlots) & 1u, watch, lane)) return false;
+    w = items[s];
+    w.lk = uniform(w.lk);
+    w.tiles[0] = uniform(w.tiles[0]);
+    w.tiles[1] = uniform(w.tiles[1]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&i_empty[s]));
+    return w.lq > 0;
+  };
+
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0) {
-    // ---------------------------------------------------------- copies
-    const bool el = elect_one();
-    if (el && most > 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (tiles[t] == 0) continue;
-        const uint32_t bar = smem_u32(&q_full[t]), dst = smem_u32(smem + C::kQ + t * C::kTile);
-        mbar_expect_tx(bar, (uint32_t)(D / 64 * 128 * ps.tile_heads * ps.tokens_tile));
-#pragma unroll
-        for (int x = 0; x < D / 64; ++x)
-          tma_load_3d(dst + x * kAtom, &map_q, bar, x * 64, head0, qs + tok0 + t * ps.tokens_tile);
-      }
-    }
-    __syncwarp();
-    bool ok = true;
-    for (int e = 0; e < 2 * most; ++e) {
-      if (!warp_wait(entry_bar(empty, e), entry_phase(e) ^ 1u, watch, lane)) {
-        ok = false;
-        break;
-      }
-      if (el) {
-        const uint32_t bar = entry_bar(full, e), dst = entry_addr(e);
-        mbar_expect_tx(bar, C::kTile);
-#pragma unroll
-        for (int x = 0; x < D / 64; ++x)
-          tma_load_3d(dst + x * kAtom, e & 1 ? &map_v : &map_k, bar, x * 64, kv_head, ks + (e >> 1) * kKeys);
-      }
-      __syncwarp();
-    }
-    if (!ok) {  // giving up: time for the copies in flight to land before the CTA can exit
-      const unsigned long long t0 = globaltimer();
-      while (globaltimer() - t0 < 100000ull) {
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMAs
-    // Per key tile j: P_0 V_j, Q_0 K_{j+1}, P_1 V_j, Q_1 K_{j+1}: the softmax of one query tile runs under the
-    // other's MMAs.
-    const bool el = elect_one();
-    bool ok = true;
-    for (int j = -1; j < most && ok; ++j) {
-      if (j >= 0 && j == most - 1 && most * kKeys > lk) {
-        // The last V tile ends past the sequence: its rows there, another sequence's, become zeros (their
-        // probabilities are 0, but 0 times an infinity is not).
-        const int e = 2 * j + 1, from = lk - j * kKeys;
-        if (!warp_wait(entry_bar(full, e), entry_phase(e), watch, lane)) break;
-        uint8_t* tile = smem + C::kRing + (e % C::kSlots) * C::kTile;
-#pragma unroll
-        for (int x = 0; x < D / 64; ++x)
-          for (int i = from * 8 + lane; i < kKeys * 8; i += 32)
-            *reinterpret_cast<uint4*>(tile + x * kAtom + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        fence_async_smem();
+    if (warp == 3) {
+      // ------------------------------------------------------- items
+      if (blockIdx.x == 0) check_offsets(a, lane, 32);
+      uint32_t number = 0;
+      for (int round = 0;; ++round) {
+        PromptItem w{};
+        const bool end = round * (int64_t)gridDim.x >= ps.items;
+        if (round == 0) {
+          if (!first_there) continue;
+          w = first;
+        } else if (!end && (item_index(round) >= ps.items || !prompt_item(a, ps, item_index(round), lane, w))) {
+          continue;
+        }
+        const uint32_t s = number % kItemSlots;
+        if (!warp_wait(smem_u32(&i_empty[s]), ((number / kItemSlots) & 1u) ^ 1u, watch, lane)) break;
+        if (lane == 0) {
+          items[s] = w;  // all zeros at the end
+          mbar_arrive(smem_u32(&i_full[s]));
+        }
         __syncwarp();
+        ++number;
+        if (end) break;
       }
+    } else if (warp == 0) {
+      // ------------------------------------------------------ copies
+      const bool el = elect_one();
+      uint32_t e = 0, uses[2] = {0, 0};
+      bool ok = true;
+      PromptItem w;
+      for (uint32_t number = 0; ok && next_item(number, w); ++number) {
+        const int most = max(w.tiles[0], w.tiles[1]);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t s_col = tmem + (uint32_t)(t * 128), o_col = tmem + C::kColO + (uint32_t)(t * D);
-        if (j >= 0 && j < tiles[t]) {
-          if (!warp_wait(smem_u32(&p_full[t]), (uint32_t)j & 1u, watch, lane) ||
-              !warp_wait(entry_bar(full, 2 * j + 1), entry_phase(2 * j + 1), watch, lane)) {
-            ok = false;
-            break;
+        for (int t = 0; t < 2; ++t) {
+          if (w.tiles[t] == 0) continue;
+          ok = ok && warp_wait(smem_u32(&q_empty[t]), (uses[t] & 1u) ^ 1u, watch, lane);
+          if (el && ok) {
+            const uint32_t bar = smem_u32(&q_full[t]), dst = smem_u32(smem + C::kQ + t * C::kTile);
+            mbar_expect_tx(bar, (uint32_t)(D / 64 * 128 * ps.tile_heads * ps.tokens_tile));
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x)
+              tma_load_3d(dst + x * kAtom, &map_q, bar, x * 64, w.head0, w.q_row + t * ps.tokens_tile);
           }
-          tc_fence_after();
-          if (el) {
-            const uint32_t v = entry_addr(2 * j + 1);
+          __syncwarp();
+          ++uses[t];
+        }
+        for (int i = 0; i < 2 * most && ok; ++i, ++e) {
+          ok = warp_wait(entry_bar(empty, e), entry_phase(e) ^ 1u, watch, lane);
+          if (el && ok) {
+            const uint32_t bar = entry_bar(full, e), dst = entry_addr(e);
+            mbar_expect_tx(bar, C::kTile);
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_ts(o_col, s_col + kk * 8, desc_mnmajor(v + kk * 16 * 128, kAtom), kDescPV<D>, (j | kk) != 0 ? 1u : 0u);
-            if (j == tiles[t] - 1) mma_commit(smem_u32(&o_done[t]));
-            if (t == 1 || j >= tiles[1]) mma_commit(entry_bar(empty, 2 * j + 1));
+            for (int x = 0; x < D / 64; ++x)
+              tma_load_3d(dst + x * kAtom, i & 1 ? &map_v : &map_k, bar, x * 64, w.kv_head, w.k_row + (i >> 1) * kKeys);
           }
           __syncwarp();
         }
-        if (j + 1 < tiles[t]) {
-          if ((j < 0 && !warp_wait(smem_u32(&q_full[t]), 0u, watch, lane)) ||
-              !warp_wait(entry_bar(full, 2 * j + 2), entry_phase(2 * j + 2), watch, lane)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (el) {
-            const uint32_t q = smem_u32(smem + C::kQ + t * C::kTile), k = entry_addr(2 * j + 2);
+      }
+      if (!ok) {  // giving up: time for the copies in flight to land before the CTA can exit
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 100000ull) {
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------- MMAs
+      // Per key tile j: P_0 V_j, Q_0 K_{j+1}, P_1 V_j, Q_1 K_{j+1}: the softmax of one query tile runs under the
+      // other's MMAs. P V starts on the second half of the keys while the first half's probabilities are computed.
+      const bool el = elect_one();
+      bool ok = true;
+      uint32_t e0 = 0, done[2] = {0, 0}, uses[2] = {0, 0};  // ring entries, key tiles and items so far
+      PromptItem w;
+      for (uint32_t number = 0; ok && next_item(number, w); ++number) {
+        const int most = max(w.tiles[0], w.tiles[1]);
+        for (int j = -1; j < most && ok; ++j) {
+          const uint32_t ev = e0 + 2 * j + 1, ek = ev + 1;  // V_j, K_{j+1}
+          if (j >= 0 && !(ok = warp_wait(entry_bar(full, ev), entry_phase(ev), watch, lane))) break;
+          if (j >= 0 && j == most - 1 && most * kKeys > w.lk) {
+            // The last V tile ends past the sequence: its rows there, another sequence's, become zeros (their
+            // probabilities are 0, but 0 times an infinity is not).
+            uint8_t* tile = smem + C::kRing + (ev % C::kSlots) * C::kTile;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (uint32_t)((kk >> 2) * kAtom + (kk & 3) * 32);
-              mma_ss(s_col, desc_kmajor(q + off), desc_kmajor(k + off), kDescQK, kk != 0 ? 1u : 0u);
+            for (int x = 0; x < D / 64; ++x)
+              for (int i = (w.lk - j * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
+                *reinterpret_cast<uint4*>(tile + x * kAtom + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            fence_async_smem();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t s_col = tmem + (uint32_t)(t * 128), o_col = tmem + C::kColO + (uint32_t)(t * D);
+            if (j >= 0 && j < w.tiles[t]) {
+              const uint32_t parity = (done[t] + (uint32_t)j) & 1u;
+              if (!(ok = warp_wait(smem_u32(&p_half[t]), parity, watch, lane))) break;
+              // the item's first product writes over the previous item's output
+              if (j == 0 && !(ok = warp_wait(smem_u32(&o_empty[t]), (uses[t] & 1u) ^ 1u, watch, lane))) break;
+              const uint32_t v = entry_addr(ev);
+#pragma unroll
+              for (int h = 1; h >= 0; --h) {
+                if (h == 0 && !(ok = warp_wait(smem_u32(&p_full[t]), parity, watch, lane))) break;
+                tc_fence_after();
+                if (el) {
+#pragma unroll
+                  for (int kk = 0; kk < kHalf / 16; ++kk)
+                    mma_ts(o_col, s_col + h * kHalf + kk * 8, desc_mnmajor(v + (h * kHalf + kk * 16) * 128, kAtom),
+                           kDescPV<D>, j > 0 || h == 0 || kk > 0 ? 1u : 0u);
+                }
+                __syncwarp();
+              }
+              if (!ok) break;
+              if (el && j == w.tiles[t] - 1) mma_commit(smem_u32(&o_done[t]));
             }
-            mma_commit(smem_u32(&s_full[t]));
-            if (t == 1 || j + 1 >= tiles[1]) mma_commit(entry_bar(empty, 2 * j + 2));
+            if (j + 1 < w.tiles[t]) {
+              if (j < 0 && !(ok = warp_wait(smem_u32(&q_full[t]), uses[t] & 1u, watch, lane))) break;
+              if (!(ok = warp_wait(entry_bar(full, ek), entry_phase(ek), watch, lane))) break;
+              tc_fence_after();
+              if (el) {
+                const uint32_t q = smem_u32(smem + C::kQ + t * C::kTile), k = entry_addr(ek);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint32_t off = (uint32_t)((kk >> 2) * kAtom + (kk & 3) * 32);
+                  mma_ss(s_col, desc_kmajor(q + off), desc_kmajor(k + off), kDescQK, kk != 0 ? 1u : 0u);
+                }
+                mma_commit(smem_u32(&s_full[t]));
+                if (j + 1 == w.tiles[t] - 1) mma_commit(smem_u32(&q_empty[t]));
+              }
+            }
+            __syncwarp();
+          }
+          if (el && ok) {
+            if (j >= 0) mma_commit(entry_bar(empty, ev));
+            if (j + 1 < most) mma_commit(entry_bar(empty, ek));
           }
           __syncwarp();
         }
+        e0 += 2 * (uint32_t)most;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          done[t] += (uint32_t)w.tiles[t];
+          uses[t] += w.tiles[t] > 0 ? 1u : 0u;
+        }
       }
-    }
-    // Every MMA is done before tensor memory can be released.
-    if (el) mma_commit(smem_u32(drain));
-    __syncwarp();
-    drain_bounded(smem_u32(drain), 0u);
+      // Every MMA is done before tensor memory can be released.
+      if (el) mma_commit(smem_u32(drain));
+      __syncwarp();
+      drain_bounded(smem_u32(drain), 0u);
     }
   } else {
     // ---------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = (warp - 4) >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const int in_tile = row / ps.tile_heads, head = row - in_tile * ps.tile_heads;
-    const int token = tok0 + t * ps.tokens_tile + in_tile;
-    const bool live = in_tile < ps.tokens_tile && head < heads_here && token < lq;
-    const int seen = !live ? 0 : a.causal ? min(max(token + lk - lq + 1, 0), lk) : lk;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t s_col = tmem + lanes + (uint32_t)(t * 128), o_col = tmem + lanes + C::kColO + (uint32_t)(t * D);
-    const int n = tiles[t];
-    float m_run = -INFINITY, l_run = 0.0f;
+    uint32_t done = 0, uses = 0;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      if (!warp_wait(smem_u32(&s_full[t]), (uint32_t)j & 1u, watch, lane)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t s[128];
-      tmem_ld32_nowait(s_col, s);
-      tmem_ld32_nowait(s_col + 32u, s + 32);
-      tmem_ld32_nowait(s_col + 64u, s + 64);
-      tmem_ld32_nowait(s_col + 96u, s + 96);
-      tmem_wait32(s);
-      tmem_wait32(s + 32);
-      tmem_wait32(s + 64);
-      tmem_wait32(s + 96);
-      const int valid = seen - j * kKeys;
-      const bool full_tile = __all_sync(0xffffffffu, valid >= kKeys);
-      // The running maximum moves only when it would grow by more than 2^8: probabilities stay below 2^8 and the
-      // output is rescaled rarely, exactly.
-      float mx;
-      if (full_tile) {
-        float m4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m4[e] = __uint_as_float(s[e]);
-        if (a.scale_log2 >= 0.0f) {
-#pragma unroll
-          for (int e = 4; e < 128; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(s[e]));
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
-        } else {
-#pragma unroll
-          for (int e = 4; e < 128; ++e) m4[e & 3] = fminf(m4[e & 3], __uint_as_float(s[e]));
-          mx = fminf(fminf(m4[0], m4[1]), fminf(m4[2], m4[3])) * a.scale_log2;
+    PromptItem w;
+    for (uint32_t number = 0; ok && next_item(number, w); ++number) {
+      // keys that this row sees, -1 for a row that stands for nothing
+      int seen = -1;
+      bf16* dst = a.out;
+      {
+        const int offset = t * ps.tokens_tile + in_tile;  // of this row's token in the block
+        const int token = w.tok0 + offset;
+        if (in_tile < ps.tokens_tile && head < w.heads_here && token < w.lq) {
+          seen = a.causal ? min(max(token + w.lk - w.lq + 1, 0), w.lk) : w.lk;
+          dst += ((int64_t)(w.q_row + offset) * a.heads + w.head0 + head) * D;
         }
-      } else {
-        mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 128; ++e)
-          if (e < valid) mx = fmaxf(mx, __uint_as_float(s[e]) * a.scale_log2);
       }
-      const bool move = mx > m_run + 8.0f;
-      const float m_use = move ? mx : m_run;
-      const float alpha = move ? ex2(m_run - m_use) : 1.0f;
-      const float m_sub = m_use == -INFINITY ? 0.0f : m_use;
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
+      const int n = w.tiles[t];
+      float m_run = -INFINITY, l_run = 0.0f;
+      for (int j = 0; j < n; ++j, ++done) {
+        if (!(ok = warp_wait(smem_u32(&s_full[t]), done & 1u, watch, lane))) break;
+        tc_fence_after();
+        // Both halves for the maximum; the second stays in registers, the first is read again for its probabilities.
+        const int valid = seen - j * kKeys;
+        const bool full_tile = __all_sync(0xffffffffu, valid >= kKeys);
+        uint32_t s[kHalf];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_ld32_nowait(s_col + (uint32_t)(h * kHalf), s);
+          tmem_ld32_nowait(s_col + (uint32_t)(h * kHalf) + 32u, s + 32);
+          tmem_wait32(s);
+          tmem_wait32(s + 32);
+          mx = fmaxf(mx, full_tile ? half_maximum<false>(s, a.scale_log2, kHalf)
+                                   : half_maximum<true>(s, a.scale_log2, valid - h * kHalf));
+        }
+        // The running maximum moves only when it would grow by more than 2^8: probabilities stay below 2^8 and the
+        // output is rescaled rarely, exactly.
+        const bool move = mx > m_run + 8.0f;
+        const float m_use = move ? mx : m_run;
+        const float alpha = move ? ex2(m_run - m_use) : 1.0f;
+        const float m_sub = m_use == -INFINITY ? 0.0f : m_use;
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_col + (uint32_t)c, o);
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_col + (uint32_t)c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(o_col + (uint32_t)c, o);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(o_col + (uint32_t)c, o);
+          }
         }
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_sub, -m_sub);
+        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int h = 1; h >= 0; --h) {
+          if (h == 0) {
+            tmem_ld32_nowait(s_col, s);
+            tmem_ld32_nowait(s_col + 32u, s + 32);
+            tmem_wait32(s);
+            tmem_wait32(s + 32);
+          }
+          if (full_tile)
+            probabilities<false, D>(s, sc2, nm2, kHalf, sum);
+          else
+            probabilities<true, D>(s, sc2, nm2, valid - h * kHalf, sum);
+          tmem_st32(s_col + (uint32_t)(h * kHalf), s);  // over the first of the half's own columns
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(h == 1 ? &p_half[t] : &p_full[t]));
+        }
+        l_run = fmaf(l_run, alpha, sum.x + sum.y);
+        m_run = m_use;
       }
-      const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_sub, -m_sub);
-      float2 sum = make_float2(0.0f, 0.0f);
-      if (full_tile) {
-        probabilities<false>(s, sc2, nm2, 64, sum);
-        tmem_st32(s_col, s);
-        probabilities<false>(s + 64, sc2, nm2, 64, sum);
-        tmem_st32(s_col + 32u, s + 64);
-      } else {
-        probabilities<true>(s, sc2, nm2, valid, sum);
-        tmem_st32(s_col, s);
-        probabilities<true>(s + 64, sc2, nm2, valid - 64, sum);
-        tmem_st32(s_col + 32u, s + 64);
+      if (n > 0) {
+        ok = ok && warp_wait(smem_u32(&o_done[t]), uses & 1u, watch, lane);
+        ++uses;
       }
-      l_run = fmaf(l_run, alpha, sum.x + sum.y);
-      m_run = m_use;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
-    }
-    if (ok && n > 0) ok = warp_wait(smem_u32(&o_done[t]), 0u, watch, lane);
-    if (ok) {
+      if (!ok) break;
       tc_fence_after();
-      const float inv = seen == 0 ? 0.0f : 1.0f / l_run;
-      bf16* dst = a.out + ((int64_t)(qs + token) * a.heads + head0 + head) * D;
+      const float inv = 1.0f / l_run;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
         if (n > 0) {
           tmem_ld32(o_col + (uint32_t)c, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
-        if (live) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = seen == 0 ? 0.0f : __uint_as_float(o[8 * x + e]) * inv;
-            *reinterpret_cast<uint4*>(dst + c + 8 * x) = pack8(f);
+          if (c == D - 32) {  // the output is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&o_empty[t]));
           }
         }
+        if (seen < 0) continue;
+        uint32_t y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          y[e] = seen == 0 ? 0u : cvt2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) store_16(dst + c + 16 * x, y + 8 * x, ps.wide_out);
       }
     }
   }
@@ -836,8 +977,10 @@ int launch_prompt(const Args& a, cudaStream_t stream) {
   ps.tile_heads = (a.group + ps.head_parts - 1) / ps.head_parts;
   ps.tokens_tile = kRows / ps.tile_heads;
   ps.slots = a.total_q / (2 * ps.tokens_tile) + a.seqs + 1;
-  const int64_t grid = (int64_t)ps.slots * a.kv_heads * ps.head_parts;
-  LR_REQUIRE(grid <= INT32_MAX, "attention_packed: too many blocks");
+  const int64_t items = (int64_t)ps.slots * a.kv_heads * ps.head_parts;
+  LR_REQUIRE(items <= INT32_MAX - 65536, "attention_packed: too many blocks");
+  ps.items = (int)items;
+  ps.wide_out = aligned(a.out, 32);
   CUtensorMap mq, mk{}, mv{};
   int st = head_map<D>(&mq, a.q, a.heads, a.total_q, a.q_ts, a.q_hs, (uint32_t)ps.tile_heads, (uint32_t)ps.tokens_tile);
   if (st) return st;
@@ -846,7 +989,7 @@ int launch_prompt(const Args& a, cudaStream_t stream) {
     return st;
   static bool done[64] = {};
   if ((st = configure_smem(prompt_kernel<D>, C::kSmem, done))) return st;
-  prompt_kernel<D><<<(unsigned)grid, kPromptThreads, C::kSmem, stream>>>(mq, mk, mv, a, ps);
+  prompt_kernel<D><<<(unsigned)(items < sm_count() ? items : sm_count()), kPromptThreads, C::kSmem, stream>>>(mq, mk, mv, a, ps);
   return launch_status("attention_packed (prompts)");
 }
 

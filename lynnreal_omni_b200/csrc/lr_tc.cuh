@@ -93,6 +93,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
+// A value that is the same in the whole warp, marked as such: loops and branches
+// on it keep the operands of the MMAs between them in uniform registers.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 // Drain after an abort: wait, for a quarter of the limit at most.
 __device__ __forceinline__ void drain_bounded(uint32_t bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer();
