@@ -832,6 +832,7 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
         }
       }
     }
+    allow_dependent();  // join_kernel looks its row up meanwhile
     // The warps' parts to shared memory, added in order.
     __syncthreads();
 #pragma unroll
@@ -889,49 +890,59 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
   }
 }
 
-// The parts of the sequences whose keys were split, in order: a warp a row.
-template <int D>
-__global__ void __launch_bounds__(128) join_kernel(const Args a, const StepShape ss) {
+// The parts of the sequences whose keys were split: a block a row, a thread a
+// column and every THREADS / D-th part; the groups' sums are added in order.
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepShape ss) {
+  constexpr int kGroups = THREADS / D;
+  __shared__ float sh_y[kGroups][D], sh_l[kGroups];
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.total_q * a.heads) return;
+  const int col = threadIdx.x % D, group = threadIdx.x / D;
+  const int64_t item = blockIdx.x;
   const int tok = (int)(item / a.heads), head = (int)(item % a.heads);
-  // with blocks of one token a sequence's first slot is its offset plus its number
-  int lo = 0, n = a.seqs;
+  int b = 0, n = a.seqs;  // the last sequence that starts at or before the token
   while (n > 1) {
-    const int stride = (n + 31) / 32, at = lo + lane * stride;
-    const int hits = __popc(__ballot_sync(0xffffffffu, at < lo + n && a.cu_q[at] <= tok));
+    const int stride = (n + 31) / 32, at = b + lane * stride;
+    const int hits = __popc(__ballot_sync(0xffffffffu, at < b + n && a.cu_q[at] <= tok));
     const int step = max(hits - 1, 0) * stride;
     n = min(stride, n - step);
-    lo += step;
+    b += step;
   }
-  const int b = lo;
   const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
   const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
   const int pieces = (int)((lk + (int64_t)ss.chunk - 1) / ss.chunk);
-  if (pieces <= 1 || lq * a.group > ss.max_rows || tok < qs || tok >= qs + lq) return;
+  if (pieces <= 1 || (int64_t)lq * a.group > ss.max_rows || tok < qs || tok >= qs + lq) {
+    wait_for_predecessor();
+    return;
+  }
   const int row = (tok - qs) * a.group + head % a.group;
   const int seen = a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
   const int64_t stride = (int64_t)a.kv_heads * ss.max_rows;
   const int64_t at = ((int64_t)((uint32_t)ks / (uint32_t)ss.chunk + b) * a.kv_heads + head / a.group) * ss.max_rows + row;
+  wait_for_predecessor();
   float top = -INFINITY;
   for (int p = lane; p < pieces; p += 32) top = fmaxf(top, ss.part_ml[at + p * stride].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float sub = top == -INFINITY ? 0.0f : top;
-  float y[D / 32] = {}, sum = 0.0f;
-#pragma unroll 4
-  for (int p = 0; p < pieces; ++p) {
+  float y = 0.0f, sum = 0.0f;
+#pragma unroll 8
+  for (int p = group; p < pieces; p += kGroups) {
     const float2 ml = ss.part_ml[at + p * stride];
     const float f = ex2(ml.x - sub);
     sum = fmaf(ml.y, f, sum);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) y[c] = fmaf(ss.part_o[(at + p * stride) * D + c * 32 + lane], f, y[c]);
+    y = fmaf(ss.part_o[(at + p * stride) * D + col], f, y);
   }
-  const float inv = 1.0f / sum;
+  sh_y[group][col] = y;
+  if (col == 0) sh_l[group] = sum;
+  __syncthreads();
+  if (group != 0) return;
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c)
-    a.out[item * D + c * 32 + lane] = __float2bfloat16_rn(seen > 0 ? y[c] * inv : 0.0f);
+  for (int w = 1; w < kGroups; ++w) {
+    y += sh_y[w][col];
+    sum += sh_l[w];
+  }
+  a.out[item * D + col] = __float2bfloat16_rn(seen > 0 ? y * (1.0f / sum) : 0.0f);
 }
 
 // ------------------------------------------------------------------ host
@@ -946,8 +957,8 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   const int64_t queries = (total_q + seqs - 1) / seqs;  // a sequence, on average
   p.step = queries * group <= 64;
   if (!p.step) return p;
-  // one slot's CTAs are few: about three waves of three CTAs an SM, whole when there is one sequence
-  const int64_t want = (int64_t)sm_count() * 3 * (seqs > 1 ? 3 : 1) / kv_heads;
+  // slots for three waves of four CTAs an SM, for one whole wave when there is one sequence
+  const int64_t want = (int64_t)sm_count() * 4 * (seqs > 1 ? 3 : 1) / kv_heads;
   int64_t chunk = (total_k + (want > 0 ? want : 1) - 1) / (want > 0 ? want : 1);
   chunk = (chunk + 63) / 64 * 64;
   if (chunk < 256) chunk = 256;
@@ -1010,8 +1021,13 @@ int launch_step(const Args& a, const Plan& p, void* workspace, cudaStream_t stre
   int st = launch_status("attention_packed (steps)");
   if (st || p.bytes == 0) return st;
   const int64_t rows = (int64_t)a.total_q * a.heads;
-  join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a, ss);
-  return launch_status("attention_packed (join)");
+  LR_REQUIRE(rows <= INT32_MAX, "attention_packed: too many rows");
+  // a thread takes about eight parts at most: one token against 32768 keys 33.8 us with 256 threads, 30.2 us with 512
+  // (64 requests of a few parts each, 139 us, lose 5 us to the larger blocks)
+  const int parts_each = p.slots / a.seqs;
+  const auto join = parts_each > 32 ? join_kernel<D, 1024> : parts_each > 8 ? join_kernel<D, 512> : join_kernel<D, 128>;
+  const unsigned threads = parts_each > 32 ? 1024 : parts_each > 8 ? 512 : 128;
+  return launch("attention_packed (join)", join, dim3((unsigned)rows), threads, 0, stream, 1, true, a, ss);
 }
 
 }  // namespace

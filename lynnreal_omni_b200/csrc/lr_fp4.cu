@@ -18,6 +18,7 @@
 // loads, 8-byte stores); the two halves of an mxfp4 block are two lanes.
 #include "lr_fp4.cuh"
 #include "lr_host.h"
+#include "lr_tc.cuh"
 
 namespace lr {
 namespace fp4 {
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       }
     }
   }
+  tc::allow_dependent();  // a product may set itself up
   // zeros in the last tile's blocks past the row (they meet zero codes)
   if (live && t < (int)(ctiles * 4 - blocks)) scales[scale_offset(row, blocks + t, ctiles)] = 0;
 }

@@ -217,6 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_predecessor();
 
   if (warp == 0) {
     // -------------------------------------------------------- copies
@@ -455,6 +456,7 @@ __global__ void __launch_bounds__(kFewThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_predecessor();
 
   if (warp == 0) {
     const bool el = elect_one();
@@ -625,9 +627,8 @@ int launch_many(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
   const int tiles = num_m * num_n, pairs = sm_count() / 2;
   int64_t group = (24ll << 20) / ((int64_t)C::kRows * o.K / 2);  // 24 MB of A's codes
   if (group < 1) group = 1;
-  gemm_kernel<FORMAT, H><<<2 * (tiles < pairs ? tiles : pairs), kThreads, C::kSmem, stream>>>(
-      ma, mb, msa, msb, mo, o.M, o.N, o.K, (int)(group < num_m ? group : num_m), tma_out, ep);
-  return launch_status("fp4 gemm");
+  return launch("fp4 gemm", gemm_kernel<FORMAT, H>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), kThreads, C::kSmem,
+                stream, 1, true, ma, mb, msa, msb, mo, o.M, o.N, o.K, (int)(group < num_m ? group : num_m), tma_out, ep);
 }
 
 template <int FORMAT, int NT>
@@ -645,18 +646,8 @@ int launch_few(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
   // as many slices as fill the GPU with two CTAs an SM and leave each two stages
   int splits = 1;
   while (splits < kMaxSplits && tiles * splits * 2 <= 2 * sm_count() && kblocks >= 4 * splits) splits *= 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * splits));
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {(unsigned)splits, 1, 1};
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, few_rows_kernel<FORMAT, NT>, mw, mx, msw, msx, o.M, o.N, o.K, splits, ep);
-  return launch_status("fp4 gemm (few rows)");
+  return launch("fp4 gemm (few rows)", few_rows_kernel<FORMAT, NT>, dim3((unsigned)(tiles * splits)), kFewThreads, C::kSmem,
+                stream, (unsigned)splits, true, mw, mx, msw, msx, o.M, o.N, o.K, splits, ep);
 }
 
 template <int FORMAT>

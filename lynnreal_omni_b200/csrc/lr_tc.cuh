@@ -233,7 +233,40 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ------------------------------------------------------------------ dependent launches
+// A kernel launched with launch_dependent may start when its predecessor's
+// blocks have all called allow_dependent (or ended); it must call
+// wait_for_predecessor, in every block, before it touches global memory or
+// ends: until then only its own set-up may run.
+__device__ __forceinline__ void allow_dependent() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------ host
+// Launch in clusters of `cluster` blocks, `dependent` on the stream's last kernel as above.
+template <typename... Params, typename... Args>
+int launch(const char* what, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+           unsigned cluster, bool dependent, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2]{};
+  unsigned n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n++].val.clusterDim = {cluster, 1, 1};
+  }
+  if (dependent) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return launch_status(what);
+}
+
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
