@@ -86,6 +86,9 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   __shared__ float red[kThreads / 32];
   const int t = threadIdx.x % TPR;
   const int row = blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
+  // A product that follows may set itself up: at once beside a grid that leaves room, else when this one ends.
+  const bool early = gridDim.x <= 296;
+  if (early) tc::allow_dependent();
   const bool live = row < rows;
   const int units = width / 16;
   const int blocks = FORMAT == kNv ? units : units / 2;
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       }
     }
   }
-  tc::allow_dependent();  // a product may set itself up
+  if (!early) tc::allow_dependent();
   // zeros in the last tile's blocks past the row (they meet zero codes)
   if (live && t < (int)(ctiles * 4 - blocks)) scales[scale_offset(row, blocks + t, ctiles)] = 0;
 }

@@ -340,6 +340,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool ok = warp_wait(smem_u32(&tfull[g]), (uint32_t)turn & 1u, watch, lane);
       if (!group_barrier(g, ok)) break;
       tc_fence_after();
+      // 32 columns to this warp's staging buffer (64-byte swizzle: conflict-free 16-byte writes) and out.
+      auto store = [&](int c, const uint32_t* y) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= N) return;
+        if (tma_out && lane == 0) bulk_wait_read();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+        if (tma_out) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_out, smem_u32(buf), col0, row0);
+            bulk_commit();
+          }
+        } else {  // rows that start off 16-byte boundaries: a row a step, a lane a column
+          __syncwarp();
+          if (col0 + lane < N)
+            for (int i = 0; i < 32 && row0 + i < M; ++i)
+              ep.out[(int64_t)(row0 + i) * ep.ldo + col0 + lane] = *reinterpret_cast<const bf16*>(
+                  buf + i * 64 + ((((uint32_t)lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2);
+        }
+      };
+      // The next tile's MMAs wait for this accumulator where H = 2: it is emptied before anything is stored. The last
+      // tile's columns are stored as they come (512 x 4096 to 12288: 1.5 of 17 us).
+      const bool hold = H == 2 && t + step < tiles;
       uint32_t y[TN / 2];
       const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(g * TN);
 #pragma unroll
@@ -358,32 +386,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           y[c * 16 + e] =
               cvt2(fmaf(__uint_as_float(r[2 * e]) * rs, f.x, f.y), fmaf(__uint_as_float(r[2 * e + 1]) * rs, f.z, f.w));
         }
+        if (!hold) store(c, y + c * 16);
       }
+      if (hold) {
 #pragma unroll
-      for (int c = 0; c < TN / 32; ++c) {
-        const int col0 = n0 + c * 32;
-        if (col0 >= N) break;
-        // rows to this warp's staging buffer, 64-byte swizzle: conflict-free 16-byte writes
-        if (tma_out && lane == 0) bulk_wait_read();
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(
-              y[c * 16 + 4 * q], y[c * 16 + 4 * q + 1], y[c * 16 + 4 * q + 2], y[c * 16 + 4 * q + 3]);
-        if (tma_out) {
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&map_out, smem_u32(buf), col0, row0);
-            bulk_commit();
-          }
-        } else {  // rows that start off 16-byte boundaries: a row a step, a lane a column
-          __syncwarp();
-          if (col0 + lane < N)
-            for (int i = 0; i < 32 && row0 + i < M; ++i)
-              ep.out[(int64_t)(row0 + i) * ep.ldo + col0 + lane] = *reinterpret_cast<const bf16*>(
-                  buf + i * 64 + ((((uint32_t)lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2);
-        }
+        for (int c = 0; c < TN / 32; ++c) store(c, y + c * 16);
       }
     }
     if (tma_out && lane == 0) bulk_wait_all();
