@@ -156,6 +156,22 @@ __device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int gro
   nb = r / size;
 }
 
+// A staged 32 x 32 chunk to rows of any alignment: a row a store, a column a lane. (Pairs of columns in 4-byte stores
+// took half as many and twice the time: the odd rows' pairs straddle the staged words.)
+__device__ __forceinline__ void store_rows(const uint8_t* buf, bf16* dst, int64_t ld, int rows, bool inside, int lane) {
+  uint16_t* to = reinterpret_cast<uint16_t*>(dst) + lane;
+#pragma unroll
+  for (int i0 = 0; i0 < 32; i0 += 8) {
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      v[k] = *reinterpret_cast<const uint16_t*>(buf + (i0 + k) * 64 + (((lane >> 3) ^ (((i0 + k) >> 1) & 3)) << 4) + (lane & 7) * 2);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (inside && i0 + k < rows) to[(i0 + k) * ld] = v[k];
+  }
+}
+
 // The 128 threads of an epilogue group meet; true if every one of them brought `ok`.
 __device__ __forceinline__ bool group_barrier(int group, bool ok) {
   uint32_t all;
@@ -167,11 +183,12 @@ __device__ __forceinline__ bool group_barrier(int group, bool ok) {
   return all != 0;
 }
 
-template <int FORMAT, int H>
+// TMA_OUT: out's rows start on 16-byte boundaries.
+template <int FORMAT, int H, bool TMA_OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
-                const __grid_constant__ CUtensorMap map_out, int M, int N, int K, int group, int tma_out,
+                const __grid_constant__ CUtensorMap map_out, int M, int N, int K, int group,
                 const Epilogue ep) {
   using C = Tile<FORMAT, H>;
   extern __shared__ uint8_t smem_raw[];
@@ -344,25 +361,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto store = [&](int c, const uint32_t* y) {
         const int col0 = n0 + c * 32;
         if (col0 >= N) return;
-        if (tma_out && lane == 0) bulk_wait_read();
+        if (TMA_OUT && lane == 0) bulk_wait_read();
         __syncwarp();
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
               make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-        if (tma_out) {
+        if constexpr (TMA_OUT) {
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
             tma_store_2d(&map_out, smem_u32(buf), col0, row0);
             bulk_commit();
           }
-        } else {  // rows that start off 16-byte boundaries: a row a step, a lane a column
+        } else {  // rows that start off 16-byte boundaries
           __syncwarp();
-          if (col0 + lane < N)
-            for (int i = 0; i < 32 && row0 + i < M; ++i)
-              ep.out[(int64_t)(row0 + i) * ep.ldo + col0 + lane] = *reinterpret_cast<const bf16*>(
-                  buf + i * 64 + ((((uint32_t)lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2);
+          store_rows(buf, ep.out + (int64_t)row0 * ep.ldo + col0, ep.ldo, M - row0, col0 + lane < N, lane);
         }
       };
       // The next tile's MMAs wait for this accumulator where H = 2: it is emptied before anything is stored. The last
@@ -393,7 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int c = 0; c < TN / 32; ++c) store(c, y + c * 16);
       }
     }
-    if (tma_out && lane == 0) bulk_wait_all();
+    if (TMA_OUT && lane == 0) bulk_wait_all();
   }
 
   __syncwarp();
@@ -613,29 +627,33 @@ struct Operands {
   int M, N, K;
 };
 
-template <int FORMAT, int H>
-int launch_many(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
+template <int FORMAT, int H, bool TMA_OUT>
+int launch_many_to(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
   using C = Tile<FORMAT, H>;
   CUtensorMap ma, mb, msa, msb, mo{};
   int st;
   if ((st = code_map(&ma, o.a, o.M, o.K, TM)) || (st = code_map(&mb, o.b, o.N, o.K, TN / 2)) ||
       (st = scale_map<FORMAT>(&msa, o.as, o.M, o.K, 1)) || (st = scale_map<FORMAT>(&msb, o.bs, o.N, o.K, C::kRB)))
     return st;
-  const int tma_out = ep.ldo % 8 == 0 && aligned(ep.out, 16);
-  if (tma_out) {
+  if (TMA_OUT) {
     const cuuint64_t dims[2] = {(cuuint64_t)o.N, (cuuint64_t)o.M}, strides[1] = {(cuuint64_t)ep.ldo * 2};
     const cuuint32_t box[2] = {32, 32};
     if ((st = make_map(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ep.out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)))
       return st;
   }
   static bool done[64] = {};
-  if ((st = configure_smem(gemm_kernel<FORMAT, H>, C::kSmem, done))) return st;
+  if ((st = configure_smem(gemm_kernel<FORMAT, H, TMA_OUT>, C::kSmem, done))) return st;
   const int num_m = (o.M + C::kRows - 1) / C::kRows, num_n = (o.N + C::kCols - 1) / C::kCols;
   const int tiles = num_m * num_n, pairs = sm_count() / 2;
   int64_t group = (24ll << 20) / ((int64_t)C::kRows * o.K / 2);  // 24 MB of A's codes
   if (group < 1) group = 1;
-  return launch("fp4 gemm", gemm_kernel<FORMAT, H>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), kThreads, C::kSmem,
-                stream, 1, true, ma, mb, msa, msb, mo, o.M, o.N, o.K, (int)(group < num_m ? group : num_m), tma_out, ep);
+  return launch("fp4 gemm", gemm_kernel<FORMAT, H, TMA_OUT>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), kThreads, C::kSmem,
+                stream, 1, true, ma, mb, msa, msb, mo, o.M, o.N, o.K, (int)(group < num_m ? group : num_m), ep);
+}
+template <int FORMAT, int H>
+int launch_many(const Operands& o, const Epilogue& ep, cudaStream_t stream) {
+  if (ep.ldo % 8 == 0 && aligned(ep.out, 16)) return launch_many_to<FORMAT, H, true>(o, ep, stream);
+  return launch_many_to<FORMAT, H, false>(o, ep, stream);
 }
 
 template <int FORMAT, int NT>
