@@ -155,29 +155,49 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   if (live && t < (int)(ctiles * 4 - blocks)) scales[scale_offset(row, blocks + t, ctiles)] = 0;
 }
 
-template <int FORMAT>
+// A warp a row and kUnits units a lane, 32 apart; a block eight rows, whose scales
+// lie in the same 32-byte sectors.
+constexpr int kUnits = 2;
+template <int FORMAT, bool WIDE>
 __global__ void __launch_bounds__(256)
     dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                       const float* __restrict__ row_scales, int rows, int width, bf16* __restrict__ out) {
-  const int units = width / 16;
+  const int units = width / 16, lane = threadIdx.x & 31;
   const int64_t ctiles = ((FORMAT == kNv ? units : units / 2) + 3) / 4;
-  const int64_t total = (int64_t)rows * units;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / units;
-    const int unit = (int)(i - row * units);
-    const uint2 c = *reinterpret_cast<const uint2*>(codes + i * 8);
-    float s = scale_value<FORMAT>(scales[scale_offset(row, FORMAT == kNv ? unit : unit / 2, ctiles)]);
-    if (row_scales != nullptr) s = __fmul_rn(s, row_scales[row]);
-    float f[8];
-    unpack_e2m1(c.x, f);
+  const int unit0 = blockIdx.x * (32 * kUnits) + lane;
+  for (int64_t row = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.y * 8) {
+    uint2 c[kUnits];
+    uint32_t byte[kUnits];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], s);
-    uint4* dst = reinterpret_cast<uint4*>(out + i * 16);
-    dst[0] = pack8(f);
-    unpack_e2m1(c.y, f);
+    for (int i = 0; i < kUnits; ++i) {
+      const int unit = unit0 + 32 * i;
+      if (unit < units) {
+        c[i] = __ldcs(reinterpret_cast<const uint2*>(codes + row * (width / 2) + unit * 8));
+        byte[i] = scales[scale_offset(row, FORMAT == kNv ? unit : unit / 2, ctiles)];
+      }
+    }
+    const float rs = row_scales != nullptr ? row_scales[row] : 1.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], s);
-    dst[1] = pack8(f);
+    for (int i = 0; i < kUnits; ++i) {
+      const int unit = unit0 + 32 * i;
+      if (unit >= units) break;
+      const float s = __fmul_rn(scale_value<FORMAT>(byte[i]), rs);
+      float lo[8], hi[8];
+      unpack_e2m1(c[i].x, lo);
+      unpack_e2m1(c[i].y, hi);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = __fmul_rn(lo[e], s), hi[e] = __fmul_rn(hi[e], s);
+      const uint4 u = pack8(lo), v = pack8(hi);
+      bf16* dst = out + row * width + unit * 16;
+      if (WIDE) {
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(u.x), "r"(u.y), "r"(u.z),
+                     "r"(u.w), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
+      } else {
+        reinterpret_cast<uint4*>(dst)[0] = u;
+        reinterpret_cast<uint4*>(dst)[1] = v;
+      }
+    }
   }
 }
 
@@ -246,16 +266,14 @@ extern "C" int lr_fp4_dequantize_rows(const void* codes, const void* scales, con
   LR_REQUIRE(codes && scales && out, "fp4_dequantize_rows: null pointer");
   if (!aligned(codes, 16) || !aligned(out, 16))
     return set_error(LR_ERR_UNSUPPORTED, "fp4_dequantize_rows: rows must start on 16-byte boundaries");
-  const int64_t units = rows * (width / 16);
-  const int64_t want = (units + 255) / 256, most = (int64_t)sm_count() * 32;
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  auto* s = static_cast<cudaStream_t>(stream);
-  auto* c = static_cast<const uint8_t*>(codes);
-  auto* sc = static_cast<const uint8_t*>(scales);
-  auto* o = static_cast<__nv_bfloat16*>(out);
-  if (format == LR_FP4_NV)
-    fp4::dequantize_kernel<fp4::kNv><<<grid, 256, 0, s>>>(c, sc, row_scales, (int)rows, (int)width, o);
-  else
-    fp4::dequantize_kernel<fp4::kMx><<<grid, 256, 0, s>>>(c, sc, row_scales, (int)rows, (int)width, o);
+  const int64_t blocks = (rows + 7) / 8;
+  const dim3 grid((unsigned)((width / 16 + 32 * fp4::kUnits - 1) / (32 * fp4::kUnits)), (unsigned)(blocks < 65535 ? blocks : 65535));
+  const auto kernel = format == LR_FP4_NV ? aligned(out, 32) ? fp4::dequantize_kernel<fp4::kNv, true>
+                                                             : fp4::dequantize_kernel<fp4::kNv, false>
+                      : aligned(out, 32)  ? fp4::dequantize_kernel<fp4::kMx, true>
+                                          : fp4::dequantize_kernel<fp4::kMx, false>;
+  kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), row_scales, (int)rows, (int)width,
+      static_cast<__nv_bfloat16*>(out));
   return launch_status("fp4 dequantize");
 }

@@ -21,7 +21,7 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 256;
+constexpr int kMaxThreads = 512;
 
 struct RopeArgs {
   const bf16* src[2];  // query, key
@@ -58,81 +58,130 @@ __device__ __forceinline__ float2 rotation(int64_t p, float f, float factor) {
   return make_float2(c * factor, s * factor);
 }
 
-// Tokens blockIdx.x * tpb .. + tpb. VEC: eight values (16 bytes) an access.
-// An item is one access of each half of the pairs (half layout) or one access
-// (interleaved, copied columns).
-template <bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a, int tpb) {
-  extern __shared__ float2 turn[];  // [tpb][rotary / 2]
-  const int half = a.rotary / 2;
-  const int64_t token0 = (int64_t)blockIdx.x * tpb;
-  const int here = (int)min((int64_t)tpb, a.tokens - token0);
-  for (int i = threadIdx.x; i < here * half; i += kThreads) {
-    const int64_t n = token0 + i / half;
-    const int64_t p = a.positions_64 ? static_cast<const int64_t*>(a.positions)[n]
-                                     : (int64_t) static_cast<const int32_t*>(a.positions)[n];
-    turn[i] = rotation(p, a.inv_freq[i % half], a.factor);
-  }
-  __syncthreads();
+template <bool VEC>
+struct Value {
+  using type = uint4;  // eight columns
+};
+template <>
+struct Value<false> {
+  using type = uint16_t;
+};
+__device__ __forceinline__ uint4 load(const bf16* p, uint4) { return ld_stream(p); }
+__device__ __forceinline__ uint16_t load(const bf16* p, uint16_t) { return *reinterpret_cast<const uint16_t*>(p); }
+
+// (a, b) turned by r.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float2 r) {
+  const float u = a, v = b;
+  a = u * r.x - v * r.y;
+  b = v * r.x + u * r.y;
+}
+
+// TPB consecutive tokens. An item is what one thread moves of one head: eight
+// columns (VEC; else one) of each half of the pairs (half layout), the columns
+// of four (one) pairs (interleaved), or eight (one) copied columns. Rotated
+// items come first, so that few warps hold both kinds; a thread keeps its item
+// over the block's tokens and has all their loads under way before the first
+// product, and the first ones before the angles.
+template <bool VEC, bool INTERLEAVED, int TPB>
+__global__ void __launch_bounds__(kMaxThreads) rope_kernel(const RopeArgs a) {
+  extern __shared__ float2 turn[];  // [TPB][rotary / 2]
+  using V = typename Value<VEC>::type;
   constexpr int W = VEC ? 8 : 1;
-  const int rot_items = INTERLEAVED ? a.rotary / (VEC ? 8 : 2) : half / W;
-  const int items = rot_items + (a.head_dim - a.rotary) / W;
+  const int half = a.rotary / 2;
+  const int64_t token0 = (int64_t)blockIdx.x * TPB;
+  const int here = (int)min((int64_t)TPB, a.tokens - token0);
   const int heads = a.heads[0] + a.heads[1];
-  const int total = here * heads * items;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int row = i / items, item = i - row * items;
-    const int t = row / heads, h = row - t * heads;
+  constexpr int kStep = INTERLEAVED ? (VEC ? 8 : 2) : W;  // columns from one item to the next
+  const int rot_items = (INTERLEAVED ? a.rotary : half) / kStep, copy_items = (a.head_dim - a.rotary) / W;
+  const int rotated = heads * rot_items, total = rotated + heads * copy_items;
+
+  bool first = true;
+  for (int i = threadIdx.x; first || i < total; i += blockDim.x) {
+    const bool any = i < total, turned = i < rotated;
+    const int j = turned ? i : i - rotated, per = turned ? rot_items : copy_items;
+    int h = any ? j / per : 0;
+    const int item = any ? j - h * per : 0;
     const int which = h >= a.heads[0];
-    const int head = which ? h - a.heads[0] : h;
-    const bf16* src = a.src[which] + (token0 + t) * a.token_stride[which] + head * a.head_stride[which];
-    bf16* dst = a.dst[which] + ((token0 + t) * a.heads[which] + head) * (int64_t)a.head_dim;
-    const float2* tt = turn + t * half;
-    if (item >= rot_items) {
-      const int col = a.rotary + (item - rot_items) * W;
-      if (VEC)
-        *reinterpret_cast<uint4*>(dst + col) = ld_stream(src + col);
-      else
-        dst[col] = src[col];
-    } else if (INTERLEAVED) {
-      if (VEC) {
-        float f[8];
-        unpack8(ld_stream(src + item * 8), f);
+    h -= which ? a.heads[0] : 0;
+    const int col = turned ? item * kStep : a.rotary + item * W;
+    const int second = INTERLEAVED ? 1 : half;  // column distance of a pair, where a thread loads both apart
+    const int64_t src_stride = which ? a.token_stride[1] : a.token_stride[0];
+    const int64_t dst_stride = (int64_t)(which ? a.heads[1] : a.heads[0]) * a.head_dim;
+    const bf16* src = (which ? a.src[1] : a.src[0]) + token0 * src_stride + h * (which ? a.head_stride[1] : a.head_stride[0]) + col;
+    bf16* dst = (which ? a.dst[1] : a.dst[0]) + token0 * dst_stride + h * (int64_t)a.head_dim + col;
+    const bool two = turned && !(INTERLEAVED && VEC);
+    V x[TPB], y[TPB];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 r = tt[item * 4 + e];
-          const float x = f[2 * e], y = f[2 * e + 1];
-          f[2 * e] = x * r.x - y * r.y;
-          f[2 * e + 1] = y * r.x + x * r.y;
-        }
-        *reinterpret_cast<uint4*>(dst + item * 8) = pack8(f);
-      } else {
-        const float2 r = tt[item];
-        const float x = __bfloat162float(src[2 * item]), y = __bfloat162float(src[2 * item + 1]);
-        dst[2 * item] = __float2bfloat16_rn(x * r.x - y * r.y);
-        dst[2 * item + 1] = __float2bfloat16_rn(y * r.x + x * r.y);
+    for (int t = 0; t < TPB; ++t)
+      if (any && t < here) {
+        x[t] = load(src + t * src_stride, V{});
+        if (two) y[t] = load(src + t * src_stride + second, V{});
       }
-    } else {
-      if (VEC) {
-        float x[8], y[8];
-        unpack8(ld_stream(src + item * 8), x);
-        unpack8(ld_stream(src + half + item * 8), y);
+    if (first) {
+      for (int n = threadIdx.x; n < here * half; n += blockDim.x) {
+        const int64_t at = token0 + n / half;
+        const int64_t p = a.positions_64 ? static_cast<const int64_t*>(a.positions)[at]
+                                         : (int64_t) static_cast<const int32_t*>(a.positions)[at];
+        turn[n] = rotation(p, a.inv_freq[n % half], a.factor);
+      }
+      __syncthreads();
+      first = false;
+      if (!any) break;
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 r = tt[item * 8 + e];
-          const float u = x[e], v = y[e];
-          x[e] = u * r.x - v * r.y;
-          y[e] = v * r.x + u * r.y;
+    for (int t = 0; t < TPB; ++t) {
+      if (t >= here) break;
+      bf16* to = dst + t * dst_stride;
+      if constexpr (VEC) {
+        if (turned) {
+          const float4* r4 = reinterpret_cast<const float4*>(turn + t * half + (INTERLEAVED ? item * 4 : item * 8));
+          float u[8], v[8];
+          unpack8(x[t], u);
+          if (!INTERLEAVED) unpack8(y[t], v);
+#pragma unroll
+          for (int e = 0; e < (INTERLEAVED ? 4 : 8); e += 2) {
+            const float4 r = r4[e / 2];
+            if (INTERLEAVED) {
+              turn_pair(u[2 * e], u[2 * e + 1], make_float2(r.x, r.y));
+              turn_pair(u[2 * e + 2], u[2 * e + 3], make_float2(r.z, r.w));
+            } else {
+              turn_pair(u[e], v[e], make_float2(r.x, r.y));
+              turn_pair(u[e + 1], v[e + 1], make_float2(r.z, r.w));
+            }
+          }
+          *reinterpret_cast<uint4*>(to) = pack8(u);
+          if (!INTERLEAVED) *reinterpret_cast<uint4*>(to + half) = pack8(v);
+        } else {
+          *reinterpret_cast<uint4*>(to) = x[t];
         }
-        *reinterpret_cast<uint4*>(dst + item * 8) = pack8(x);
-        *reinterpret_cast<uint4*>(dst + half + item * 8) = pack8(y);
       } else {
-        const float2 r = tt[item];
-        const float x = __bfloat162float(src[item]), y = __bfloat162float(src[half + item]);
-        dst[item] = __float2bfloat16_rn(x * r.x - y * r.y);
-        dst[half + item] = __float2bfloat16_rn(y * r.x + x * r.y);
+        uint16_t* raw = reinterpret_cast<uint16_t*>(to);
+        if (turned) {
+          float u = bf_bits(x[t]), v = bf_bits(y[t]);
+          turn_pair(u, v, turn[t * half + item]);
+          raw[0] = f2bf_bits(u);
+          raw[second] = f2bf_bits(v);
+        } else {
+          raw[0] = x[t];
+        }
       }
     }
   }
+}
+
+template <bool VEC, bool INTERLEAVED>
+int launch_rope(const RopeArgs& a, cudaStream_t stream) {
+  // Four tokens a block (128 columns: 256 angles), where that many blocks fill the GPU and their angles fit.
+  const int tpb = a.tokens >= 8 * sm_count() && a.rotary <= 1024 ? 4 : 1;
+  const int64_t items = (int64_t)(a.heads[0] + a.heads[1]) * (a.head_dim / (VEC ? 8 : 1));
+  const int64_t threads = (items / (a.rotary > 0 && !(VEC && INTERLEAVED) ? 2 : 1) + 31) / 32 * 32;
+  const unsigned block = (unsigned)(threads < 128 ? 128 : threads > kMaxThreads ? kMaxThreads : threads);
+  const size_t smem = (size_t)tpb * (a.rotary / 2) * sizeof(float2);
+  if (tpb == 4)
+    rope_kernel<VEC, INTERLEAVED, 4><<<(unsigned)((a.tokens + 3) / 4), block, smem, stream>>>(a);
+  else
+    rope_kernel<VEC, INTERLEAVED, 1><<<(unsigned)a.tokens, block, smem, stream>>>(a);
+  return launch_status("rope");
 }
 
 }  // namespace
@@ -172,19 +221,7 @@ extern "C" int lr_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
     if (a.heads[w])
       vec = vec && a.token_stride[w] % 8 == 0 && a.head_stride[w] % 8 == 0 && aligned(a.src[w], 16) &&
             aligned(a.dst[w], 16);
-  // Four tokens a block share the launch of their angles (one angle a thread
-  // at 128 columns); fewer while the blocks would not fill the GPU twice.
-  const int tpb = tokens >= 8 * sm_count() && rotary_dim <= 1024 ? 4 : 1;
-  const unsigned grid = (unsigned)((tokens + tpb - 1) / tpb);
-  const size_t smem = (size_t)tpb * (rotary_dim / 2) * sizeof(float2);
   auto* st = static_cast<cudaStream_t>(stream);
-  if (vec && interleaved)
-    rope_kernel<true, true><<<grid, kThreads, smem, st>>>(a, tpb);
-  else if (vec)
-    rope_kernel<true, false><<<grid, kThreads, smem, st>>>(a, tpb);
-  else if (interleaved)
-    rope_kernel<false, true><<<grid, kThreads, smem, st>>>(a, tpb);
-  else
-    rope_kernel<false, false><<<grid, kThreads, smem, st>>>(a, tpb);
-  return launch_status("rope");
+  if (vec) return interleaved ? launch_rope<true, true>(a, st) : launch_rope<true, false>(a, st);
+  return interleaved ? launch_rope<false, true>(a, st) : launch_rope<false, false>(a, st);
 }
