@@ -128,9 +128,9 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 
 def stream_of(tensor: torch.Tensor) -> int:
     """The caller's current CUDA stream on the tensor's device (launch target)."""
-    if tensor.device.type != "cuda":
+    if not tensor.is_cuda:
         raise ValueError("the W8A8 ops run on CUDA tensors only")
-    return torch.cuda.current_stream(tensor.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 ARITHMETIC = {"reference_gpu": 1, "ieee": 0}

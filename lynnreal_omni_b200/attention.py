@@ -71,10 +71,11 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     queries are the last ones of their sequence, each sees the keys up to its own position (one query a sequence is a
     decoding step). Rows without a visible key, and tokens past the last offset, give zeros. Values of other sequences
     never reach a row; within a sequence, values of masked keys must be finite."""
+    device = query.device
     for name, t in (("query", query), ("key", key), ("value", value)):
         if t.dtype != torch.bfloat16 or not t.is_cuda or t.ndim != 3:
             raise ValueError(f"attention_packed: {name} must be a CUDA bf16 [tokens, heads, D] tensor")
-        if t.device != query.device:
+        if t.device != device:
             raise ValueError("attention_packed: query, key and value are on different devices")
     tq, h, d = query.shape
     tk, hk, _ = key.shape
@@ -89,17 +90,17 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
             raise ValueError("attention_packed: cu_seqlens_k is needed where queries and keys differ in tokens")
         cu_seqlens_k = cu_seqlens_q
     for t in (cu_seqlens_q, cu_seqlens_k):
-        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() < 2 or t.device != query.device:
+        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() < 2 or t.device != device:
             raise ValueError("attention_packed: cu_seqlens must be int32 [sequences + 1] on the query's device")
     if cu_seqlens_k.numel() != cu_seqlens_q.numel():
         raise ValueError("attention_packed: cu_seqlens_q and cu_seqlens_k differ in sequences")
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     query, key, value = _head_view(query), _head_view(key), _head_view(value)
-    out = torch.empty((tq, h, d), device=query.device, dtype=torch.bfloat16)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
     lib, seqs = _lib.load(), cu_seqlens_q.numel() - 1
     need = lib.lr_attention_packed_workspace_bytes(seqs, tq, tk, h, hk, d)
-    workspace = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None
+    workspace = query.new_empty(need, dtype=torch.uint8) if need else None
     check(lib.lr_attention_packed(
         ptr(query), query.stride(0), query.stride(1), ptr(key), key.stride(0), key.stride(1), ptr(value),
         value.stride(0), value.stride(1), ptr(cu_seqlens_q), ptr(cu_seqlens_k), seqs, tq, tk, h, hk, d, bool(causal), sc,

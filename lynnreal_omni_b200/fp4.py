@@ -34,12 +34,12 @@ def _check_packed(name: str, what: str, codes: torch.Tensor, scales: torch.Tenso
     """(rows, width) of a packed matrix whose codes and scales fit each other."""
     if codes.dtype != torch.uint8 or codes.ndim != 2 or not codes.is_contiguous():
         raise ValueError(f"{name}: {what} codes must be a contiguous uint8 [rows, width / 2] tensor")
-    rows, width = codes.shape[0], codes.shape[1] * 2
-    if (scales.dtype != torch.uint8 or tuple(scales.shape) != _scale_shape(rows, width, block)
-            or not scales.is_contiguous() or scales.device != codes.device):
-        raise ValueError(f"{name}: {what} scales must be contiguous uint8 {_scale_shape(rows, width, block)} on the "
-                         f"codes' device, got {tuple(scales.shape)}")
-    return rows, width
+    rows, half = codes.shape
+    shape = _scale_shape(rows, 2 * half, block)
+    if scales.dtype != torch.uint8 or scales.shape != shape or not scales.is_contiguous() or scales.device != codes.device:
+        raise ValueError(f"{name}: {what} scales must be contiguous uint8 {shape} on the codes' device, "
+                         f"got {scales.dtype} {tuple(scales.shape)}")
+    return rows, 2 * half
 
 
 def _vector(name: str, what: str, t: torch.Tensor | None, count: int, dtype: torch.dtype, device):
@@ -73,9 +73,9 @@ def quantize_rows_fp4(value: torch.Tensor, *, format: str = "nvfp4"):
         raise ValueError(f"quantize_rows_fp4: the width must be a positive multiple of 32, got {width}")
     if value.stride(1) != 1 or (rows > 1 and (value.stride(0) % 8 or value.stride(0) < width)) or value.data_ptr() % 16:
         value = value.clone(memory_format=torch.contiguous_format)
-    codes = torch.empty((rows, width // 2), device=value.device, dtype=torch.uint8)
-    scales = torch.empty(_scale_shape(rows, width, block), device=value.device, dtype=torch.uint8)
-    row_scale = torch.empty((rows, 1), device=value.device, dtype=torch.float32) if block == 16 else None
+    codes = value.new_empty((rows, width // 2), dtype=torch.uint8)
+    scales = value.new_empty(_scale_shape(rows, width, block), dtype=torch.uint8)
+    row_scale = value.new_empty((rows, 1), dtype=torch.float32) if block == 16 else None
     check(_lib.load().lr_fp4_quantize_rows(ptr(value), rows, width, value.stride(0), code, ptr(codes), ptr(scales),
                                            ptr(row_scale), stream_of(value)), "quantize_rows_fp4")
     return codes, scales, row_scale
@@ -87,7 +87,7 @@ def dequantize_rows_fp4(codes: torch.Tensor, scales: torch.Tensor, row_scale: to
     code, block = _format("dequantize_rows_fp4", format)
     rows, width = _check_packed("dequantize_rows_fp4", "the", codes, scales, block)
     row_scale = _vector("dequantize_rows_fp4", "row_scale", row_scale, rows, torch.float32, codes.device)
-    output = torch.empty((rows, width), device=codes.device, dtype=torch.bfloat16)
+    output = codes.new_empty((rows, width), dtype=torch.bfloat16)
     check(_lib.load().lr_fp4_dequantize_rows(ptr(codes), ptr(scales), ptr(row_scale), rows, width, code, ptr(output),
                                              stream_of(codes)), "dequantize_rows_fp4")
     return output
@@ -106,10 +106,11 @@ def fp4_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: torch.Ten
         raise ValueError(f"fp4_matmul: operands of widths {k} and {kb} (and one device) are wanted to be alike")
     if n == 0 or k == 0:
         raise ValueError("fp4_matmul: empty weight")
-    row_scale = _vector("fp4_matmul", "row_scale", row_scale, m, torch.float32, a_codes.device)
-    column_scale = _vector("fp4_matmul", "column_scale", column_scale, n, torch.float32, a_codes.device)
-    bias = _vector("fp4_matmul", "bias", bias, n, torch.bfloat16, a_codes.device)
-    output = torch.empty((m, n), device=a_codes.device, dtype=torch.bfloat16)
+    device = a_codes.device
+    row_scale = _vector("fp4_matmul", "row_scale", row_scale, m, torch.float32, device)
+    column_scale = _vector("fp4_matmul", "column_scale", column_scale, n, torch.float32, device)
+    bias = _vector("fp4_matmul", "bias", bias, n, torch.bfloat16, device)
+    output = a_codes.new_empty((m, n), dtype=torch.bfloat16)
     check(_lib.load().lr_fp4_gemm(ptr(a_codes), ptr(a_scales), ptr(b_codes), ptr(b_scales), m, n, k, code,
                                   ptr(row_scale), ptr(column_scale), ptr(bias), ptr(output), n, stream_of(a_codes)),
           "fp4_matmul")

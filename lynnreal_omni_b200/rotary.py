@@ -67,27 +67,32 @@ def rope(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
     positions: int32 or int64, one per token; inv_freq: fp32 [rotary_dim / 2]. The first rotary_dim columns of each
     head are turned, as pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1); the others are copied.
     """
+    device = query.device
     for name, t in (("query", query), ("key", key)):
-        if t is not None and (t.dtype != torch.bfloat16 or t.ndim < 3 or t.device != query.device):
+        if t is not None and (t.dtype != torch.bfloat16 or t.ndim < 3 or t.device != device):
             raise ValueError(f"rope: {name} must be a bf16 [..., heads, head_dim] tensor on the query's device")
     q = _tokens_view(query)
-    k = None if key is None else _tokens_view(key)
     tokens, heads, d = q.shape
-    if k is not None and (k.shape[0] != tokens or k.shape[2] != d):
-        raise ValueError("rope: query and key differ in tokens or head_dim")
-    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or inv_freq.device != query.device:
+    rotary = 2 * inv_freq.numel()
+    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or inv_freq.device != device:
         raise ValueError("rope: inv_freq must be an fp32 vector on the query's device")
-    if 2 * inv_freq.numel() > d:
-        raise ValueError(f"rope: {2 * inv_freq.numel()} rotary columns do not fit head_dim {d}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != query.device:
+    if rotary > d:
+        raise ValueError(f"rope: {rotary} rotary columns do not fit head_dim {d}")
+    wide = positions.dtype == torch.int64
+    if not (wide or positions.dtype == torch.int32) or positions.device != device:
         raise ValueError("rope: positions must be int32 or int64 on the query's device")
     if positions.numel() != tokens:
         raise ValueError(f"rope: {positions.numel()} positions for {tokens} tokens")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    q_out = torch.empty(query.shape, device=query.device, dtype=torch.bfloat16)
-    k_out = None if key is None else torch.empty(key.shape, device=query.device, dtype=torch.bfloat16)
+    q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    k_out, k_args = None, (None, 0, 0, 0)
+    if key is not None:
+        k = _tokens_view(key)
+        if k.shape[0] != tokens or k.shape[2] != d:
+            raise ValueError("rope: query and key differ in tokens or head_dim")
+        k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
+        k_args = (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1])
     check(_lib.load().lr_rope(
-        ptr(q), q.stride(0), q.stride(1), heads, ptr(k), 0 if k is None else k.stride(0), 0 if k is None else k.stride(1),
-        0 if k is None else k.shape[1], ptr(positions), positions.dtype == torch.int64, ptr(inv_freq), float(factor),
-        tokens, d, 2 * inv_freq.numel(), bool(interleaved), ptr(q_out), ptr(k_out), stream_of(query)), "rope")
+        q.data_ptr(), q.stride(0), q.stride(1), heads, *k_args, positions.data_ptr(), wide, inv_freq.data_ptr(),
+        float(factor), tokens, d, rotary, bool(interleaved), q_out.data_ptr(), ptr(k_out), stream_of(query)), "rope")
     return q_out, k_out
