@@ -336,8 +336,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_map(&map_q);
-    prefetch_map(&map_k);
-    prefetch_map(&map_v);
+    if (a.total_k > 0) {  // else there is no map
+      prefetch_map(&map_k);
+      prefetch_map(&map_v);
+    }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&q_full[t]), 1);
       mbar_init(smem_u32(&q_empty[t]), 1);
@@ -667,9 +669,12 @@ struct StepShape {
   int chunk;      // keys of a slot
   int slots;
   int max_rows;   // rows a sequence up to which its keys are split
-  float* part_o;  // [slots][kv_heads][max_rows][D] unnormalised
-  float2* part_ml;  // maximum (base 2, scaled) and sum
+  float* part_o;    // [parts][kv_heads][max_rows][D] unnormalised
+  float2* part_ml;  // [parts][kv_heads][max_rows] maximum (base 2, scaled) and sum
 };
+// First part of a sequence of more than `chunk` keys that starts at key `ks`: such a sequence of l keys has
+// ceil(l / chunk) <= floor(2 l / chunk) pieces, so the next one's parts start behind them.
+__device__ __forceinline__ int64_t first_part(int ks, int chunk) { return (2 * (int64_t)ks + chunk - 1) / chunk; }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -874,7 +879,7 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
       }
       const int row = r0 + r;
       if (split) {
-        const int64_t at = ((int64_t)slot * a.kv_heads + kv_head) * ss.max_rows + row;
+        const int64_t at = ((first_part(ks, ss.chunk) + index) * a.kv_heads + kv_head) * ss.max_rows + row;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) ss.part_o[at * D + c * 32 + lane] = y[c];
         if (lane == 0) ss.part_ml[at] = make_float2(top, sum);
@@ -918,7 +923,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
   const int row = (tok - qs) * a.group + head % a.group;
   const int seen = a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
   const int64_t stride = (int64_t)a.kv_heads * ss.max_rows;
-  const int64_t at = ((int64_t)((uint32_t)ks / (uint32_t)ss.chunk + b) * a.kv_heads + head / a.group) * ss.max_rows + row;
+  const int64_t at = (first_part(ks, ss.chunk) * a.kv_heads + head / a.group) * ss.max_rows + row;
   wait_for_predecessor();
   float top = -INFINITY;
   for (int p = lane; p < pieces; p += 32) top = fmaxf(top, ss.part_ml[at + p * stride].x);
@@ -950,6 +955,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
 struct Plan {
   bool step;
   int chunk, slots, max_rows;
+  int64_t parts;  // room for parts, 0 where no sequence can be long enough to be split
   int64_t bytes;  // of workspace
 };
 Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t kv_heads, int64_t head_dim) {
@@ -967,7 +973,8 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   int64_t most = 1;
   while (most < queries) most *= 2;
   p.max_rows = (int)(most * group);
-  if (total_k > chunk) p.bytes = (int64_t)p.slots * kv_heads * p.max_rows * (head_dim + 2) * 4;
+  p.parts = total_k > chunk ? 2 * total_k / chunk + 2 : 0;
+  p.bytes = p.parts * kv_heads * p.max_rows * (head_dim + 2) * 4;
   return p;
 }
 
@@ -1007,10 +1014,9 @@ int launch_prompt(const Args& a, cudaStream_t stream) {
 template <int D>
 int launch_step(const Args& a, const Plan& p, void* workspace, cudaStream_t stream) {
   StepShape ss{p.chunk, p.slots, p.max_rows, nullptr, nullptr};
-  const int64_t parts = (int64_t)p.slots * a.kv_heads * p.max_rows;
   if (p.bytes > 0) {
     ss.part_o = static_cast<float*>(workspace);
-    ss.part_ml = reinterpret_cast<float2*>(ss.part_o + parts * D);
+    ss.part_ml = reinterpret_cast<float2*>(ss.part_o + p.parts * a.kv_heads * p.max_rows * D);
   }
   const int nt = p.max_rows <= 8 ? 1 : 2;
   const dim3 grid((unsigned)p.slots, (unsigned)a.kv_heads, (unsigned)((p.max_rows + 8 * nt - 1) / (8 * nt)));

@@ -101,6 +101,15 @@ def test_long_sequences():
     check([1, 3], [9000, 20000], 8, 2, 64, seed=2)
 
 
+def test_workspace_is_bounded_by_the_keys():
+    """Split sequences among many short ones: the parts lie close together, whatever the number of sequences."""
+    need = _lib.load().lr_attention_packed_workspace_bytes
+    assert need(100000, 100000, 10 ** 8, 32, 8, 128) == need(2, 2, 10 ** 8, 32, 8, 128) < 1 << 24
+    lk = [700, 3, 2900, 257, 1, 513, 0, 4000] + [5] * 50 + [1200]
+    check([1] * len(lk), lk, 8, 2, 128)
+    check([1, 2] * (len(lk) // 2) + [1], lk, 4, 2, 64, seed=3)
+
+
 @pytest.mark.parametrize("spread", [0.0, 30.0])
 def test_flat_and_peaked_scores(spread):
     check([260, 40], [260, 40], 4, 2, 128, spread=spread)
@@ -208,6 +217,8 @@ def test_empty_and_refusals():
     cu = offsets([8])
     assert attention_packed(q[:0], k, v, offsets([0]), cu).shape == (0, 4, 64)
     assert not bool(attention_packed(q, k[:0], v[:0], cu, offsets([0])).any())
+    many = torch.ones(700, 4, 64, device=DEV, dtype=torch.bfloat16)
+    assert not bool(attention_packed(many, k[:0], v[:0], offsets([700]), offsets([0])).any())
     with pytest.raises(ValueError, match="bf16"):
         attention_packed(q.float(), k, v, cu)
     with pytest.raises(ValueError, match="head_dim"):
