@@ -95,6 +95,13 @@ def test_fewer_or_more_queries_than_keys(lq, lk, causal, d):
         assert not bool(got[4:].any())
 
 
+@pytest.mark.parametrize("seqs", [31, 32, 33, 255, 256, 400])
+def test_many_sequences(seqs):
+    """Both ways of finding a block's sequence, at the edges of their ranges; every third sequence is empty."""
+    lengths = [0 if i % 3 == 2 else 40 + 53 * i % 97 for i in range(seqs)]
+    check(lengths, lengths, 2, 1, 64, seed=seqs)
+
+
 def test_long_sequences():
     check([4100], [4100], 2, 1, 128)
     check([1], [70000], 8, 1, 128, seed=1)
