@@ -1,4 +1,4 @@
-"""Attention core of the fused DiT block on the sm_100a tcgen05 kernel.
+"""Attention on the sm_100a tcgen05 kernels: the core of the fused DiT block, and packed prompts.
 
 ``attention_bshd(query, key, value)`` computes softmax(scale * Q K^T) V for
 bf16 [B, S, H, 128] tensors (heads contiguous within a token; the strided
@@ -7,6 +7,10 @@ softmax, bf16 output [B, S, H, 128]. It stands where FusedAttention calls
 diffusers' attention dispatcher (model/fusion.py:55-57). Unsupported inputs
 (a mask, another head size, another dtype) raise ValueError; torch's SDPA
 remains available as ``fusion.sdpa_bshd`` for callers that need those.
+
+``attention_packed`` is the attention of prompts of different lengths, packed
+without padding: causal or full, with grouped key/value heads, and with fewer
+queries than keys (a decoding step, a piece of a prompt).
 """
 from __future__ import annotations
 
