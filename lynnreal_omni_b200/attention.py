@@ -58,8 +58,11 @@ def attention_bshd(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
 
 
 def _head_view(t: torch.Tensor) -> torch.Tensor:
-    """[tokens, heads, D] with contiguous columns and 16-byte aligned tokens and heads, else a contiguous copy."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+    """[tokens, heads, D] with contiguous columns and 16-byte aligned tokens and heads that do not overlap (what TMA maps
+    address), else a contiguous copy."""
+    d = t.shape[2]
+    ts, hs = t.stride(0), t.stride(1)
+    if t.stride(2) == 1 and ts % 8 == 0 and hs % 8 == 0 and ts >= d and hs >= d and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -58,16 +58,32 @@ __device__ __forceinline__ float2 rotation(int64_t p, float f, float factor) {
   return make_float2(c * factor, s * factor);
 }
 
-template <bool VEC>
-struct Value {
-  using type = uint4;  // eight columns
+// W columns as they lie in memory.
+template <int W>
+struct Columns {
+  uint4 v[W / 8];
 };
 template <>
-struct Value<false> {
-  using type = uint16_t;
+struct Columns<1> {
+  uint16_t v;
 };
-__device__ __forceinline__ uint4 load(const bf16* p, uint4) { return ld_stream(p); }
-__device__ __forceinline__ uint16_t load(const bf16* p, uint16_t) { return *reinterpret_cast<const uint16_t*>(p); }
+__device__ __forceinline__ Columns<16> load(const bf16* p, Columns<16>) {
+  Columns<16> c;
+  asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(c.v[0].x), "=r"(c.v[0].y), "=r"(c.v[0].z), "=r"(c.v[0].w), "=r"(c.v[1].x), "=r"(c.v[1].y),
+                 "=r"(c.v[1].z), "=r"(c.v[1].w)
+               : "l"(p));
+  return c;
+}
+__device__ __forceinline__ Columns<8> load(const bf16* p, Columns<8>) { return {{ld_stream(p)}}; }
+__device__ __forceinline__ Columns<1> load(const bf16* p, Columns<1>) { return {*reinterpret_cast<const uint16_t*>(p)}; }
+__device__ __forceinline__ void store(bf16* p, const Columns<16>& c) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(c.v[0].x), "r"(c.v[0].y),
+               "r"(c.v[0].z), "r"(c.v[0].w), "r"(c.v[1].x), "r"(c.v[1].y), "r"(c.v[1].z), "r"(c.v[1].w)
+               : "memory");
+}
+__device__ __forceinline__ void store(bf16* p, const Columns<8>& c) { *reinterpret_cast<uint4*>(p) = c.v[0]; }
+__device__ __forceinline__ void store(bf16* p, const Columns<1>& c) { *reinterpret_cast<uint16_t*>(p) = c.v; }
 
 // (a, b) turned by r.
 __device__ __forceinline__ void turn_pair(float& a, float& b, float2 r) {
@@ -76,22 +92,22 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float2 r) {
   b = v * r.x + u * r.y;
 }
 
-// TPB consecutive tokens. An item is what one thread moves of one head: eight
-// columns (VEC; else one) of each half of the pairs (half layout), the columns
-// of four (one) pairs (interleaved), or eight (one) copied columns. Rotated
+// TPB consecutive tokens. An item is what one thread moves of one head: W
+// columns (16 in 32-byte accesses, 8, or 1) of each half of the pairs (half
+// layout), W columns of pairs side by side (interleaved; 2 where W is 1), or W
+// copied columns. Rotated
 // items come first, so that few warps hold both kinds; a thread keeps its item
 // over the block's tokens and has all their loads under way before the first
 // product, and the first ones before the angles.
-template <bool VEC, bool INTERLEAVED, int TPB>
+template <int W, bool INTERLEAVED, int TPB>
 __global__ void __launch_bounds__(kMaxThreads) rope_kernel(const RopeArgs a) {
   extern __shared__ float2 turn[];  // [TPB][rotary / 2]
-  using V = typename Value<VEC>::type;
-  constexpr int W = VEC ? 8 : 1;
+  using V = Columns<W>;
   const int half = a.rotary / 2;
   const int64_t token0 = (int64_t)blockIdx.x * TPB;
   const int here = (int)min((int64_t)TPB, a.tokens - token0);
   const int heads = a.heads[0] + a.heads[1];
-  constexpr int kStep = INTERLEAVED ? (VEC ? 8 : 2) : W;  // columns from one item to the next
+  constexpr int kStep = INTERLEAVED && W == 1 ? 2 : W;  // columns from one item to the next
   const int rot_items = (INTERLEAVED ? a.rotary : half) / kStep, copy_items = (a.head_dim - a.rotary) / W;
   const int rotated = heads * rot_items, total = rotated + heads * copy_items;
 
@@ -109,7 +125,7 @@ __global__ void __launch_bounds__(kMaxThreads) rope_kernel(const RopeArgs a) {
     const int64_t dst_stride = (int64_t)(which ? a.heads[1] : a.heads[0]) * a.head_dim;
     const bf16* src = (which ? a.src[1] : a.src[0]) + token0 * src_stride + h * (which ? a.head_stride[1] : a.head_stride[0]) + col;
     bf16* dst = (which ? a.dst[1] : a.dst[0]) + token0 * dst_stride + h * (int64_t)a.head_dim + col;
-    const bool two = turned && !(INTERLEAVED && VEC);
+    const bool two = turned && !(INTERLEAVED && W > 1);
     V x[TPB], y[TPB];
 #pragma unroll
     for (int t = 0; t < TPB; ++t)
@@ -132,55 +148,58 @@ __global__ void __launch_bounds__(kMaxThreads) rope_kernel(const RopeArgs a) {
     for (int t = 0; t < TPB; ++t) {
       if (t >= here) break;
       bf16* to = dst + t * dst_stride;
-      if constexpr (VEC) {
+      if constexpr (W > 1) {
         if (turned) {
-          const float4* r4 = reinterpret_cast<const float4*>(turn + t * half + (INTERLEAVED ? item * 4 : item * 8));
-          float u[8], v[8];
-          unpack8(x[t], u);
-          if (!INTERLEAVED) unpack8(y[t], v);
+          // angles of the item: W / 2 (interleaved) or W of them
+          const float4* r4 = reinterpret_cast<const float4*>(turn + t * half + item * (INTERLEAVED ? W / 2 : W));
 #pragma unroll
-          for (int e = 0; e < (INTERLEAVED ? 4 : 8); e += 2) {
-            const float4 r = r4[e / 2];
-            if (INTERLEAVED) {
-              turn_pair(u[2 * e], u[2 * e + 1], make_float2(r.x, r.y));
-              turn_pair(u[2 * e + 2], u[2 * e + 3], make_float2(r.z, r.w));
-            } else {
-              turn_pair(u[e], v[e], make_float2(r.x, r.y));
-              turn_pair(u[e + 1], v[e + 1], make_float2(r.z, r.w));
+          for (int q = 0; q < W / 8; ++q) {
+            float u[8], v[8];
+            unpack8(x[t].v[q], u);
+            if (!INTERLEAVED) unpack8(y[t].v[q], v);
+#pragma unroll
+            for (int e = 0; e < (INTERLEAVED ? 4 : 8); e += 2) {
+              const float4 r = r4[(q * (INTERLEAVED ? 4 : 8) + e) / 2];
+              if (INTERLEAVED) {
+                turn_pair(u[2 * e], u[2 * e + 1], make_float2(r.x, r.y));
+                turn_pair(u[2 * e + 2], u[2 * e + 3], make_float2(r.z, r.w));
+              } else {
+                turn_pair(u[e], v[e], make_float2(r.x, r.y));
+                turn_pair(u[e + 1], v[e + 1], make_float2(r.z, r.w));
+              }
             }
+            x[t].v[q] = pack8(u);
+            if (!INTERLEAVED) y[t].v[q] = pack8(v);
           }
-          *reinterpret_cast<uint4*>(to) = pack8(u);
-          if (!INTERLEAVED) *reinterpret_cast<uint4*>(to + half) = pack8(v);
-        } else {
-          *reinterpret_cast<uint4*>(to) = x[t];
+          if (!INTERLEAVED) store(to + half, y[t]);
         }
+        store(to, x[t]);
       } else {
-        uint16_t* raw = reinterpret_cast<uint16_t*>(to);
         if (turned) {
-          float u = bf_bits(x[t]), v = bf_bits(y[t]);
+          float u = bf_bits(x[t].v), v = bf_bits(y[t].v);
           turn_pair(u, v, turn[t * half + item]);
-          raw[0] = f2bf_bits(u);
-          raw[second] = f2bf_bits(v);
-        } else {
-          raw[0] = x[t];
+          x[t].v = f2bf_bits(u);
+          y[t].v = f2bf_bits(v);
+          store(to + second, y[t]);
         }
+        store(to, x[t]);
       }
     }
   }
 }
 
-template <bool VEC, bool INTERLEAVED>
+template <int W, bool INTERLEAVED>
 int launch_rope(const RopeArgs& a, cudaStream_t stream) {
   // Four tokens a block (128 columns: 256 angles), where that many blocks fill the GPU and their angles fit.
   const int tpb = a.tokens >= 8 * sm_count() && a.rotary <= 1024 ? 4 : 1;
-  const int64_t items = (int64_t)(a.heads[0] + a.heads[1]) * (a.head_dim / (VEC ? 8 : 1));
-  const int64_t threads = (items / (a.rotary > 0 && !(VEC && INTERLEAVED) ? 2 : 1) + 31) / 32 * 32;
+  const int64_t items = (int64_t)(a.heads[0] + a.heads[1]) * (a.head_dim / W);
+  const int64_t threads = (items / (a.rotary > 0 && !(W > 1 && INTERLEAVED) ? 2 : 1) + 31) / 32 * 32;
   const unsigned block = (unsigned)(threads < 128 ? 128 : threads > kMaxThreads ? kMaxThreads : threads);
   const size_t smem = (size_t)tpb * (a.rotary / 2) * sizeof(float2);
   if (tpb == 4)
-    rope_kernel<VEC, INTERLEAVED, 4><<<(unsigned)((a.tokens + 3) / 4), block, smem, stream>>>(a);
+    rope_kernel<W, INTERLEAVED, 4><<<(unsigned)((a.tokens + 3) / 4), block, smem, stream>>>(a);
   else
-    rope_kernel<VEC, INTERLEAVED, 1><<<(unsigned)a.tokens, block, smem, stream>>>(a);
+    rope_kernel<W, INTERLEAVED, 1><<<(unsigned)a.tokens, block, smem, stream>>>(a);
   return launch_status("rope");
 }
 
@@ -216,12 +235,16 @@ extern "C" int lr_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
   a.inv_freq = inv_freq;
   a.factor = factor;
   a.tokens = (int)tokens, a.head_dim = (int)head_dim, a.rotary = (int)rotary_dim;
-  bool vec = head_dim % 8 == 0 && (interleaved ? rotary_dim % 8 == 0 : rotary_dim % 16 == 0);
-  for (int w = 0; w < 2; ++w)
-    if (a.heads[w])
-      vec = vec && a.token_stride[w] % 8 == 0 && a.head_stride[w] % 8 == 0 && aligned(a.src[w], 16) &&
-            aligned(a.dst[w], 16);
+  // The widest access that divides the head, the rotary part and every row's start.
+  auto fits = [&](int64_t w) {
+    bool ok = head_dim % w == 0 && rotary_dim % (interleaved ? w : 2 * w) == 0;
+    for (int i = 0; i < 2; ++i)
+      if (a.heads[i])
+        ok = ok && a.token_stride[i] % w == 0 && a.head_stride[i] % w == 0 && aligned(a.src[i], 2 * w) && aligned(a.dst[i], 2 * w);
+    return ok;
+  };
   auto* st = static_cast<cudaStream_t>(stream);
-  if (vec) return interleaved ? launch_rope<true, true>(a, st) : launch_rope<true, false>(a, st);
-  return interleaved ? launch_rope<false, true>(a, st) : launch_rope<false, false>(a, st);
+  if (fits(16)) return interleaved ? launch_rope<16, true>(a, st) : launch_rope<16, false>(a, st);
+  if (fits(8)) return interleaved ? launch_rope<8, true>(a, st) : launch_rope<8, false>(a, st);
+  return interleaved ? launch_rope<1, true>(a, st) : launch_rope<1, false>(a, st);
 }

@@ -163,6 +163,9 @@ def test_strided_views():
     assert torch.equal(attention_packed(q, k, v, offsets(lengths)), expected)
     heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
     assert torch.equal(attention_packed(*heads_first, offsets(lengths)), expected)
+    shared = [t[:, :1].expand(-1, 4, -1) for t in (k, v)]  # broadcast heads
+    assert torch.equal(attention_packed(q, *shared, offsets(lengths)),
+                       attention_packed(q, k[:, :1], v[:, :1], offsets(lengths)))
     odd = torch.cat((fused[:, :1], fused), 1)[:, 1:]  # 2-byte aligned
     views = [t.unflatten(1, (-1, 128)) for t in odd.split([512, 256, 256], 1)]
     assert torch.equal(attention_packed(*views, offsets(lengths)), expected)
