@@ -57,14 +57,15 @@ def attention_bshd(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     return out
 
 
-def _head_view(t: torch.Tensor) -> torch.Tensor:
-    """[tokens, heads, D] with contiguous columns and 16-byte aligned tokens and heads that do not overlap (what TMA maps
-    address), else a contiguous copy."""
+def _head_view(t: torch.Tensor):
+    """(t, token stride, head stride) of [tokens, heads, D] with contiguous columns and 16-byte aligned tokens and heads
+    that do not overlap (what TMA maps address); of a contiguous copy where t is not so."""
+    ts, hs, cs = t.stride()
     d = t.shape[2]
-    ts, hs = t.stride(0), t.stride(1)
-    if t.stride(2) == 1 and ts % 8 == 0 and hs % 8 == 0 and ts >= d and hs >= d and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    if cs == 1 and ts % 8 == 0 and hs % 8 == 0 and ts >= d and hs >= d and t.data_ptr() % 16 == 0:
+        return t, ts, hs
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.shape[1] * d, d
 
 
 def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -80,13 +81,13 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     never reach a row; within a sequence, values of masked keys must be finite."""
     device = query.device
     for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.dtype != torch.bfloat16 or not t.is_cuda or t.ndim != 3:
+        if t.dtype != torch.bfloat16 or t.ndim != 3 or not t.is_cuda:
             raise ValueError(f"attention_packed: {name} must be a CUDA bf16 [tokens, heads, D] tensor")
-        if t.device != device:
-            raise ValueError("attention_packed: query, key and value are on different devices")
+    if key.device != device or value.device != device:
+        raise ValueError("attention_packed: query, key and value are on different devices")
     tq, h, d = query.shape
-    tk, hk, _ = key.shape
-    if value.shape != key.shape or key.shape[2] != d:
+    tk, hk, dk = key.shape
+    if value.shape != key.shape or dk != d:
         raise ValueError("attention_packed: query/key/value shapes disagree")
     if d not in (64, 128):
         raise ValueError(f"attention_packed: head_dim {d} (the kernel handles 64 and 128)")
@@ -96,20 +97,21 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if tk != tq:
             raise ValueError("attention_packed: cu_seqlens_k is needed where queries and keys differ in tokens")
         cu_seqlens_k = cu_seqlens_q
+    count = cu_seqlens_q.numel()
     for t in (cu_seqlens_q, cu_seqlens_k):
-        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() < 2 or t.device != device:
+        if t.dtype != torch.int32 or t.ndim != 1 or count < 2 or t.device != device:
             raise ValueError("attention_packed: cu_seqlens must be int32 [sequences + 1] on the query's device")
-    if cu_seqlens_k.numel() != cu_seqlens_q.numel():
+    if cu_seqlens_k.numel() != count:
         raise ValueError("attention_packed: cu_seqlens_q and cu_seqlens_k differ in sequences")
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
-    query, key, value = _head_view(query), _head_view(key), _head_view(value)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    (query, q_ts, q_hs), (key, k_ts, k_hs), (value, v_ts, v_hs) = _head_view(query), _head_view(key), _head_view(value)
+    out = torch.empty(tq, h, d, dtype=torch.bfloat16, device=device)
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    lib, seqs = _lib.load(), cu_seqlens_q.numel() - 1
+    lib, seqs = _lib.load(), count - 1
     need = lib.lr_attention_packed_workspace_bytes(seqs, tq, tk, h, hk, d)
-    workspace = query.new_empty(need, dtype=torch.uint8) if need else None
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     check(lib.lr_attention_packed(
-        ptr(query), query.stride(0), query.stride(1), ptr(key), key.stride(0), key.stride(1), ptr(value),
-        value.stride(0), value.stride(1), ptr(cu_seqlens_q), ptr(cu_seqlens_k), seqs, tq, tk, h, hk, d, bool(causal), sc,
-        ptr(out), ptr(workspace), need, stream_of(query)), "attention_packed")
+        query.data_ptr(), q_ts, q_hs, key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, cu_seqlens_q.data_ptr(),
+        cu_seqlens_k.data_ptr(), seqs, tq, tk, h, hk, d, bool(causal), sc, out.data_ptr(), ptr(workspace), need,
+        stream_of(query)), "attention_packed")
     return out

@@ -42,9 +42,7 @@ def _check_packed(name: str, what: str, codes: torch.Tensor, scales: torch.Tenso
     return rows, 2 * half
 
 
-def _vector(name: str, what: str, t: torch.Tensor | None, count: int, dtype: torch.dtype, device):
-    if t is None:
-        return None
+def _vector(name: str, what: str, t: torch.Tensor, count: int, dtype: torch.dtype, device):
     if t.dtype != dtype or t.numel() != count or t.device != device:
         raise ValueError(f"{name}: {what} must hold {count} {dtype} values on the codes' device")
     return t.contiguous()
@@ -71,12 +69,14 @@ def quantize_rows_fp4(value: torch.Tensor, *, format: str = "nvfp4"):
     rows, width = value.shape
     if width == 0 or width % 32:
         raise ValueError(f"quantize_rows_fp4: the width must be a positive multiple of 32, got {width}")
-    if value.stride(1) != 1 or (rows > 1 and (value.stride(0) % 8 or value.stride(0) < width)) or value.data_ptr() % 16:
-        value = value.clone(memory_format=torch.contiguous_format)
-    codes = value.new_empty((rows, width // 2), dtype=torch.uint8)
-    scales = value.new_empty(_scale_shape(rows, width, block), dtype=torch.uint8)
-    row_scale = value.new_empty((rows, 1), dtype=torch.float32) if block == 16 else None
-    check(_lib.load().lr_fp4_quantize_rows(ptr(value), rows, width, value.stride(0), code, ptr(codes), ptr(scales),
+    stride, column_stride = value.stride()
+    if column_stride != 1 or (rows > 1 and (stride % 8 or stride < width)) or value.data_ptr() % 16:
+        value, stride = value.clone(memory_format=torch.contiguous_format), width
+    device = value.device
+    codes = torch.empty(rows, width // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(*_scale_shape(rows, width, block), dtype=torch.uint8, device=device)
+    row_scale = torch.empty(rows, 1, dtype=torch.float32, device=device) if block == 16 else None
+    check(_lib.load().lr_fp4_quantize_rows(value.data_ptr(), rows, width, stride, code, codes.data_ptr(), scales.data_ptr(),
                                            ptr(row_scale), stream_of(value)), "quantize_rows_fp4")
     return codes, scales, row_scale
 
@@ -86,8 +86,9 @@ def dequantize_rows_fp4(codes: torch.Tensor, scales: torch.Tensor, row_scale: to
     """The values of packed rows: bf16 [rows, width], code * (scale * row_scale) rounded once."""
     code, block = _format("dequantize_rows_fp4", format)
     rows, width = _check_packed("dequantize_rows_fp4", "the", codes, scales, block)
-    row_scale = _vector("dequantize_rows_fp4", "row_scale", row_scale, rows, torch.float32, codes.device)
-    output = codes.new_empty((rows, width), dtype=torch.bfloat16)
+    if row_scale is not None:
+        row_scale = _vector("dequantize_rows_fp4", "row_scale", row_scale, rows, torch.float32, codes.device)
+    output = torch.empty(rows, width, dtype=torch.bfloat16, device=codes.device)
     check(_lib.load().lr_fp4_dequantize_rows(ptr(codes), ptr(scales), ptr(row_scale), rows, width, code, ptr(output),
                                              stream_of(codes)), "dequantize_rows_fp4")
     return output
@@ -107,13 +108,16 @@ def fp4_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: torch.Ten
     if n == 0 or k == 0:
         raise ValueError("fp4_matmul: empty weight")
     device = a_codes.device
-    row_scale = _vector("fp4_matmul", "row_scale", row_scale, m, torch.float32, device)
-    column_scale = _vector("fp4_matmul", "column_scale", column_scale, n, torch.float32, device)
-    bias = _vector("fp4_matmul", "bias", bias, n, torch.bfloat16, device)
-    output = a_codes.new_empty((m, n), dtype=torch.bfloat16)
-    check(_lib.load().lr_fp4_gemm(ptr(a_codes), ptr(a_scales), ptr(b_codes), ptr(b_scales), m, n, k, code,
-                                  ptr(row_scale), ptr(column_scale), ptr(bias), ptr(output), n, stream_of(a_codes)),
-          "fp4_matmul")
+    if row_scale is not None:
+        row_scale = _vector("fp4_matmul", "row_scale", row_scale, m, torch.float32, device)
+    if column_scale is not None:
+        column_scale = _vector("fp4_matmul", "column_scale", column_scale, n, torch.float32, device)
+    if bias is not None:
+        bias = _vector("fp4_matmul", "bias", bias, n, torch.bfloat16, device)
+    output = torch.empty(m, n, dtype=torch.bfloat16, device=device)
+    check(_lib.load().lr_fp4_gemm(a_codes.data_ptr(), a_scales.data_ptr(), b_codes.data_ptr(), b_scales.data_ptr(), m, n, k,
+                                  code, ptr(row_scale), ptr(column_scale), ptr(bias), output.data_ptr(), n,
+                                  stream_of(a_codes)), "fp4_matmul")
     return output
 
 

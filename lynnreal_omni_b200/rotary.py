@@ -52,11 +52,14 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | N
     return inv.to(device=device, dtype=torch.float32), output
 
 
-def _tokens_view(t: torch.Tensor) -> torch.Tensor:
-    """[tokens, heads, head_dim] with contiguous columns; a view wherever the strides allow."""
+def _tokens_view(t: torch.Tensor):
+    """(t, token stride, head stride) of [tokens, heads, head_dim] with contiguous columns; a view wherever the strides
+    allow."""
     if t.stride(-1) != 1:
         t = t.contiguous()
-    return t if t.ndim == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
+    if t.ndim != 3:
+        t = t.reshape(-1, t.shape[-2], t.shape[-1])
+    return t, *t.stride()[:2]
 
 
 def rope(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -71,7 +74,7 @@ def rope(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
     for name, t in (("query", query), ("key", key)):
         if t is not None and (t.dtype != torch.bfloat16 or t.ndim < 3 or t.device != device):
             raise ValueError(f"rope: {name} must be a bf16 [..., heads, head_dim] tensor on the query's device")
-    q = _tokens_view(query)
+    q, q_ts, q_hs = _tokens_view(query)
     tokens, heads, d = q.shape
     rotary = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or inv_freq.device != device:
@@ -84,15 +87,15 @@ def rope(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
     if positions.numel() != tokens:
         raise ValueError(f"rope: {positions.numel()} positions for {tokens} tokens")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    q_out = torch.empty(*query.shape, dtype=torch.bfloat16, device=device)
     k_out, k_args = None, (None, 0, 0, 0)
     if key is not None:
-        k = _tokens_view(key)
+        k, k_ts, k_hs = _tokens_view(key)
         if k.shape[0] != tokens or k.shape[2] != d:
             raise ValueError("rope: query and key differ in tokens or head_dim")
-        k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
-        k_args = (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1])
+        k_out = torch.empty(*key.shape, dtype=torch.bfloat16, device=device)
+        k_args = (k.data_ptr(), k_ts, k_hs, k.shape[1])
     check(_lib.load().lr_rope(
-        q.data_ptr(), q.stride(0), q.stride(1), heads, *k_args, positions.data_ptr(), wide, inv_freq.data_ptr(),
+        q.data_ptr(), q_ts, q_hs, heads, *k_args, positions.data_ptr(), wide, inv_freq.data_ptr(),
         float(factor), tokens, d, rotary, bool(interleaved), q_out.data_ptr(), ptr(k_out), stream_of(query)), "rope")
     return q_out, k_out
