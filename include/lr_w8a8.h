@@ -271,7 +271,8 @@ int lr_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_
  *   LR_FP4_MX: blocks of 32 columns, e8m0 scales 2^e, e = floor(log2(max_b |x|)) - 2,
  *     code = e2m1(x * 2^-e); no row scale.
  * Nearest even, saturating. An infinity or NaN turns its row's (NV) or block's
- * (MX) scale into NaN. Widths are multiples of 32.
+ * (MX) scale into NaN. e4m3 scales are not negative (the tensor core takes them
+ * without a sign). Widths are multiples of 32.
  * Scales lie in tiles of 128 rows x 4 blocks: uint8 [ceil(rows/128),
  * ceil(blocks/4), 32, 4, 4], element [R, C, r, j, c] the scale of row
  * 128 R + 32 j + r, block 4 C + c. Blocks past the row hold zeros; bytes of rows

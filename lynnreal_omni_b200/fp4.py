@@ -5,7 +5,7 @@ Two formats of e2m1 codes (two a byte, the even column in the low nibble) under 
   * "mxfp4": blocks of 32 columns, e8m0 scales (powers of two).
 Block scales are kept in the order in which the tensor core reads them, uint8 [ceil(rows / 128), ceil(blocks / 4),
 32, 4, 4]: element [R, C, r, j, c] is the scale of row 128 R + 32 j + r, block 4 C + c; blocks past the row hold zeros
-(``tile_scales`` brings a [rows, blocks] matrix into it). Widths are multiples of 32.
+(``tile_scales`` brings a [rows, blocks] matrix into it). e4m3 scales are not negative. Widths are multiples of 32.
 """
 from __future__ import annotations
 
