@@ -14,6 +14,7 @@ queries than keys (a decoding step, a piece of a prompt).
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -68,6 +69,12 @@ def _head_view(t: torch.Tensor):
     return t, t.shape[1] * d, d
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, seqs: int, tq: int, tk: int, heads: int, kv_heads: int, d: int) -> int:
+    """lr_attention_packed's need for these counts on this device (a function of them alone)."""
+    return _lib.load().lr_attention_packed_workspace_bytes(seqs, tq, tk, heads, kv_heads, d)
+
+
 def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens_q: torch.Tensor,
                      cu_seqlens_k: torch.Tensor | None = None, *, causal: bool = True,
                      scale: float | None = None) -> torch.Tensor:
@@ -108,7 +115,7 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     out = torch.empty(tq, h, d, dtype=torch.bfloat16, device=device)
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
     lib, seqs = _lib.load(), count - 1
-    need = lib.lr_attention_packed_workspace_bytes(seqs, tq, tk, h, hk, d)
+    need = _workspace_bytes(query.get_device(), seqs, tq, tk, h, hk, d)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     check(lib.lr_attention_packed(
         query.data_ptr(), q_ts, q_hs, key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, cu_seqlens_q.data_ptr(),
