@@ -152,8 +152,10 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(desc), "r"(accumulate)
       : "memory");
 }
-// Issue a 32-column load; its registers are valid after tmem_wait32 of them.
+// Issue a 32-column load; its registers are valid after tmem_wait32 of them. The
+// access is .sync.aligned, as the store below: the lanes meet first.
 __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -177,6 +179,7 @@ __device__ __forceinline__ void tmem_wait32(uint32_t* a) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  __syncwarp();
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
