@@ -247,6 +247,7 @@ __device__ __forceinline__ void tc_fence_after() {
 // Load 32 consecutive int32 TMEM columns of this thread's lane and wait for
 // them in the same asm block, so no consumer can be scheduled before the wait.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  __syncwarp();  // .sync.aligned: the lanes meet first
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"

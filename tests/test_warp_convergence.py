@@ -20,9 +20,9 @@ def helpers(text):
             yield name, body
 
 
-@pytest.mark.parametrize("source", ["lr_tc.cuh", "lr_attention_packed.cu"])
+@pytest.mark.parametrize("source", ["lr_tc.cuh", "lr_attention_packed.cu", "lr_gemm_sm100.cu", "lr_attention.cu"])
 def test_tensor_memory_accesses_begin_with_a_converged_warp(source):
     text = (CSRC / source).read_text()
     found = list(helpers(text))
-    assert len(found) == len(re.findall(r"tcgen05\.(?:ld|st)\.sync\.aligned", text)) >= 2
+    assert len(found) == len(re.findall(r"tcgen05\.(?:ld|st)\.sync\.aligned", text)) >= 1
     assert [name for name, body in found if not body.lstrip().startswith("__syncwarp();")] == []
