@@ -194,11 +194,15 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 // 2^x for a pair on the FMA pipe: x = n + f with n = round(x), f in [-1/2, 1/2];
 // 2^f by a cubic fitted to it there (relative error below 7.5e-5, far under the
-// bf16 rounding of the probabilities); 2^n by adding n to the exponent field. x
-// is held above -125, so that the result stays a normal number (2^-125 is
-// nothing against a row sum of at least 2^-8). NaN stays out of the finite range.
+// bf16 rounding of the probabilities), times 2^n. x is held above -125, so that
+// the result stays a normal number, and what the cubic gives there is taken off
+// again (nothing against any result above 2^-100): a score of minus infinity, or
+// one that far below the maximum, weighs exactly 0, however large its value row.
+// 2^n as a factor and not as a sum of exponent fields lets NaN through.
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
   constexpr float kMagic = 12582912.0f;
+  constexpr float kOne = 0.9999280572f;  // the cubic at 0
+  constexpr float kFloor = -kOne * 0x1p-125f;
   x.x = max_nan(x.x, -125.0f);
   x.y = max_nan(x.y, -125.0f);
   const float2 t = __fadd2_rn(x, make_float2(kMagic, kMagic));
@@ -206,9 +210,10 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
   const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);  // exact
   float2 p = __ffma2_rn(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.2426111400f, 0.2426111400f));
   p = __ffma2_rn(p, f, make_float2(0.6932609677f, 0.6932609677f));
-  p = __ffma2_rn(p, f, make_float2(0.9999280572f, 0.9999280572f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  p = __ffma2_rn(p, f, make_float2(kOne, kOne));
+  const float2 power = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return __ffma2_rn(p, power, make_float2(kFloor, kFloor));
 }
 
 // One pair in `kPolyEvery` of a full tile goes through exp2_poly2: the special

@@ -243,3 +243,34 @@ def test_empty_and_refusals():
         attention_packed(q, k, v, cu, offsets([4, 4]))
     with pytest.raises(ValueError, match="cu_seqlens_k is needed"):
         attention_packed(q[:4], k, v, cu)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk,causal", [([300], [300], True), ([200], [515], False), ([1], [3000], False)])
+def test_scores_that_are_not_finite(lq, lk, causal, d):
+    """Rows whose visible scores are all minus infinity have no softmax and give NaN; a NaN key gives NaN to every row
+    that sees it, wherever in a tile it lies; keys of score minus infinity weigh nothing, however large their values."""
+    q, k, v = tensors(lq, lk, 4, 2, d, seed=11)
+    k[..., 0] = -k[..., 0].abs() - 1
+    cu_q, cu_k = offsets(lq), offsets(lk)
+    rows = slice(0, None, 7)
+    lost = q.clone()
+    lost[rows, 1, 0] = math.inf
+    got, clean = attention_packed(lost, k, v, cu_q, cu_k, causal=causal), attention_packed(q, k, v, cu_q, cu_k, causal=causal)
+    assert bool(torch.isnan(got[rows, 1]).all())
+    got[rows, 1] = clean[rows, 1]
+    assert torch.equal(got, clean)
+
+    for at in range(5, 13):
+        bad = k.clone()
+        bad[at, 1, 3] = math.nan
+        got = attention_packed(q, bad, v, cu_q, cu_k, causal=causal)
+        first = at if causal else 0  # heads 2 and 3 read key head 1
+        assert bool(torch.isnan(got[first:, 2:]).all())
+        assert torch.equal(got[:first], clean[:first]) and torch.equal(got[:, :2], clean[:, :2])
+
+    q[..., 0] = 1
+    k[1::2, :, 0], v[1::2] = -math.inf, 2.0 ** 127
+    got = attention_packed(q, k, v, cu_q, cu_k, causal=causal)
+    v[1::2] = 0
+    compare(got, reference(q, k, v, lq, lk, causal, 1 / math.sqrt(d)))
