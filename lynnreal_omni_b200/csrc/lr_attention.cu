@@ -258,24 +258,34 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
 // 2^x for a pair, on the FMA pipe: x = n + f with n = round(x) (add and
 // subtract 1.5 * 2^23) and f in [-1/2, 1/2]; 2^f by a cubic fitted to 2^f on
 // that interval (relative error below 7.5e-5, far under the bf16 rounding of
-// P); 2^n by adding n to the exponent field. x is clamped to >= -125 so the
-// result stays a normal float (2^-125 is negligible against a row sum >= 1).
+// P), times 2^n. x is clamped to >= -125 so the result stays a normal float, and
+// what the cubic gives there is taken off again (nothing against any result
+// above 2^-100): a score that far below the maximum, or minus infinity, weighs
+// exactly 0. 2^n as a factor, not as a sum of exponent fields, lets NaN through.
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
   constexpr float kMagic = 12582912.0f;
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
+  constexpr float kOne = 0.9999280572f;  // the cubic at 0
+  constexpr float kFloor = -kOne * 0x1p-125f;
+  x.x = max_nan(x.x, -125.0f);
+  x.y = max_nan(x.y, -125.0f);
   const float2 t = __fadd2_rn(x, make_float2(kMagic, kMagic));
   const float2 n = __fadd2_rn(t, make_float2(-kMagic, -kMagic));
   const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);  // exact
   float2 p = __ffma2_rn(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.2426111400f, 0.2426111400f));
   p = __ffma2_rn(p, f, make_float2(0.6932609677f, 0.6932609677f));
-  p = __ffma2_rn(p, f, make_float2(0.9999280572f, 0.9999280572f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  p = __ffma2_rn(p, f, make_float2(kOne, kOne));
+  const float2 power = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return __ffma2_rn(p, power, make_float2(kFloor, kFloor));
 }
 
 // P for 64 consecutive scores of a row: p = 2^(s * scale_log2 - m), stored as

@@ -89,3 +89,23 @@ def test_attention_rejects_unsupported():
     y = torch.zeros(1, 8, 2, 128, device=DEV, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         attention_bshd(y, y, y, attn_mask=torch.ones(1, 1, 8, 8, device=DEV, dtype=torch.bool))
+
+
+def test_attention_scores_that_are_not_finite():
+    """A NaN key gives NaN to every row, wherever in a key tile it lies; keys of score minus infinity weigh nothing,
+    however large their values."""
+    g = torch.Generator(device=DEV).manual_seed(17)
+    q, k, v = (torch.randn(1, 300, 2, 128, device=DEV, generator=g).to(torch.bfloat16) for _ in range(3))
+    clean = attention_bshd(q, k, v)
+    for at in range(60, 96):
+        bad = k.clone()
+        bad[0, at, 1, 3] = math.nan
+        got = attention_bshd(q, bad, v)
+        assert bool(torch.isnan(got[:, :, 1]).all()) and torch.equal(got[:, :, 0], clean[:, :, 0])
+    q[..., 0] = 1
+    k[:, 1::2, :, 0], v[:, 1::2] = -math.inf, 2.0 ** 127
+    got = attention_bshd(q, k, v)
+    v[:, 1::2] = 0
+    ref = reference(q, k, v, 1 / math.sqrt(128))
+    err = (got.float() - ref).abs()
+    assert torch.all(err <= 0.02 + 0.02 * ref.abs()), float(err.max())
