@@ -26,7 +26,8 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | N
       * "ntk": the base grown to base * factor^(R / (R - 2)), so that the slowest frequency is divided by the factor
         and the fastest is kept;
       * "yarn": frequencies that make more than ``fast_turns`` turns over the original length are kept, those below
-        ``slow_turns`` divided by the factor, a linear ramp over the index between; outputs times 0.1 ln(factor) + 1.
+        ``slow_turns`` divided by the factor, a linear ramp over the index between (its ends rounded outwards to whole
+        indices and held in [0, rotary_dim - 1]); outputs times 0.1 ln(factor) + 1.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rope_frequencies: rotary_dim must be positive and even, got {rotary_dim}")
@@ -43,7 +44,8 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | N
     elif scaling == "yarn":
         def crossing(turns):  # the (real) index whose frequency makes that many turns over the original length
             return half * math.log(original_length / (2 * math.pi * turns)) / math.log(base)
-        low, high = max(math.floor(crossing(fast_turns)), 0), min(math.ceil(crossing(slow_turns)), half - 1)
+        # the ramp may end beyond the last index, half - 1: no frequency is then divided in full
+        low, high = max(math.floor(crossing(fast_turns)), 0), min(math.ceil(crossing(slow_turns)), rotary_dim - 1)
         divided = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
         inv = inv * (1 - divided) + inv / factor * divided
         output = 0.1 * math.log(factor) + 1.0

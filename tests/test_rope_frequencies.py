@@ -38,3 +38,18 @@ def test_yarn_keeps_fast_and_divides_slow_frequencies():
 def test_refusals(kwargs):
     with pytest.raises(ValueError):
         rope_frequencies(device="cpu", **kwargs)
+
+
+@pytest.mark.parametrize("length,dim,base", [(65536, 128, 10000.0), (131072, 128, 10000.0), (262144, 64, 500.0), (4096, 128, 10000.0),
+                                             (100, 128, 10000.0), (131072, 2, 10000.0)])
+def test_yarn_ramp_may_end_beyond_the_last_index(length, dim, base):
+    """One index at a time: where even the slowest frequency makes more than one turn, it is divided in part only."""
+    inv, _ = rope_frequencies(dim, base=base, scaling="yarn", factor=4.0, original_length=length, device="cpu")
+    start, end = (dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base)) for turns in (32.0, 1.0))
+    start, end = max(math.floor(start), 0), min(math.ceil(end), dim - 1)
+    for i in range(dim // 2):
+        plain = base ** (-2 * i / dim)
+        divided = min(max((i - start) / max(end - start, 1e-3), 0.0), 1.0)
+        assert math.isclose(inv[i], plain * (1 - divided) + plain / 4 * divided, rel_tol=1e-6), i
+    if length == 131072 and dim == 128:
+        assert math.isclose(inv[-1] / 10000.0 ** (-126 / 128), 0.46, rel_tol=1e-6)  # 18 of the ramp's 25 indices
