@@ -274,3 +274,39 @@ def test_scores_that_are_not_finite(lq, lk, causal, d):
     got = attention_packed(q, k, v, cu_q, cu_k, causal=causal)
     v[1::2] = 0
     compare(got, reference(q, k, v, lq, lk, causal, 1 / math.sqrt(d)))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tq,tk,cu_q,cu_k", [
+    (100, 100, [0, 50, 500], None), (100, 100, [0, 80, 40], None), (100, 100, [-5, 20, 100], None), (100, 100, [3, 50, 100], None),
+    (100, 100, [0, -2 ** 31, 2 ** 31 - 1], None), (100, 300, [0, 100], [0, 301]), (100, 300, [0, 100], [-400, 900]),
+    (100, 100, [i * 37 % 131 - 20 for i in range(40)], None), (70, 900, [0, 30, 70], [700, 200, 2000]),
+    (2, 3000, [0, 1, 2], [0, 2500, 1200]), (2, 3000, [0, 1, 2], [-7, 5000, 3000]), (2, 3000, [1, 0, 9], [0, 2 ** 31 - 1, -2 ** 31]),
+    (40, 9000, [i * 29 % 61 - 9 for i in range(40)], [i * 6007 % 14000 - 2000 for i in range(40)])], ids=str)
+def test_wrong_offsets_stay_inside_the_tensors(tq, tk, cu_q, cu_k, d):
+    """Queries, keys and values lie between NaN, output and workspace between marks: none of it is read or written."""
+    h, hk, margin, mark = 4, 2, 256, 7.0
+    lib = _lib.load()
+    cu_q, cu_k = (torch.tensor(c, dtype=torch.int32, device=DEV) for c in (cu_q, cu_k or cu_q))
+    seqs = cu_q.numel() - 1
+
+    def between(tokens, heads, edge):
+        whole = torch.full((tokens + 2 * margin, heads, d), edge, device=DEV, dtype=torch.bfloat16)
+        return whole, whole[margin:-margin]
+
+    q, k, v = (between(n, heads, math.nan)[1] for n, heads in ((tq, h), (tk, hk), (tk, hk)))
+    for t, source in zip((q, k, v), tensors([tq], [tk], h, hk, d, seed=tq + tk)):
+        t.copy_(source)
+    out_all, out = between(tq, h, mark)
+    need = lib.lr_attention_packed_workspace_bytes(seqs, tq, tk, h, hk, d)
+    work_all = torch.full((need + 8192,), 171, dtype=torch.uint8, device=DEV)
+    work = work_all[4096:4096 + need]
+    for causal in (0, 1):
+        status = lib.lr_attention_packed(
+            q.data_ptr(), h * d, d, k.data_ptr(), hk * d, d, v.data_ptr(), hk * d, d, cu_q.data_ptr(), cu_k.data_ptr(), seqs,
+            tq, tk, h, hk, d, causal, d ** -0.5, out.data_ptr(), work.data_ptr() if need else None, need,
+            torch.cuda.current_stream().cuda_stream)
+        assert status == 0 and _lib.device_status() == 8
+        assert bool(torch.isfinite(out).all())
+        assert bool((out_all[:margin] == mark).all()) and bool((out_all[-margin:] == mark).all())
+        assert bool((work_all[:4096] == 171).all()) and bool((work_all[4096 + need:] == 171).all())
