@@ -231,7 +231,8 @@ int lr_attention_bf16(const void* q, int64_t q_token_stride, const void* k, int6
  *   out[i,h,:] = sum_j softmax_j(scale * q[i,h,:] . k[j,h',:]) * v[j,h',:]
  * over the keys of i's sequence; with causal != 0 the queries are the last ones
  * of their sequence: query i of Lq sees the keys j <= i + Lk - Lq of Lk. Rows
- * without a visible key, and rows of q past cu_q[seqs], give zeros. fp32
+ * without a visible key, and rows of q past cu_q[seqs], give zeros; rows whose
+ * visible scores are all minus infinity, or one of them a NaN, give NaN. fp32
  * scores, softmax statistics and accumulation; probabilities rounded to bf16.
  * head_dim 64 or 128; element strides of tokens and heads per operand, columns
  * contiguous; pointers and strides 16-byte aligned; out contiguous

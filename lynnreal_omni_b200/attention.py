@@ -85,7 +85,10 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     [sequences + 1] offsets on the device (never read by the host); the keys' default to the queries'. ``causal``: the
     queries are the last ones of their sequence, each sees the keys up to its own position (one query a sequence is a
     decoding step). Rows without a visible key, and tokens past the last offset, give zeros. Values of other sequences
-    never reach a row; within a sequence, values of masked keys must be finite."""
+    never reach a row; within a sequence, values of masked keys must be finite.
+
+    Kernels are chosen by the average number of queries a sequence: whole prompts and single tokens in one batch are much
+    faster as two calls."""
     device = query.device
     for name, t in (("query", query), ("key", key), ("value", value)):
         if t.dtype != torch.bfloat16 or t.ndim != 3 or not t.is_cuda:

@@ -14,12 +14,12 @@
 //
 //   * prompt_kernel: many queries a sequence; bound by the tensor cores and the
 //     softmax under them. One prompt of 16384 tokens, 32 query and 8 key/value
-//     heads of 128: 1.95 ms, 1127 TFLOP/s, 0.68 of the measured bf16 burst rate
-//     (the GPU is at its power limit then; 0.79 of the sustained rate).
+//     heads of 128: 2.00 ms, 1098 TFLOP/s, 0.66 of the measured bf16 burst rate
+//     (the GPU is at its power limit then; 0.78 of the sustained rate).
 //   * step_kernel (+ join_kernel): up to 64 rows a sequence on average
 //     (decoding); bound by reading keys and values, which are split over the
 //     GPU and joined. 64 requests of one token against 1024 to 5056 keys: 134
-//     us, 5.9 TB/s, 0.91 of the measured copy rate; one against 32768: 30 us.
+//     us, 5.9 TB/s, 0.91 of the measured copy rate; one against 32768: 27 us.
 //     The prompt kernel would leave all but `group` of a tile's 256 rows empty
 //     and one CTA to a sequence's keys.
 #include "lr_common.cuh"

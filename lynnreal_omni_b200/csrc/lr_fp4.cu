@@ -89,7 +89,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   __shared__ float red[kThreads / 32];
   const int t = threadIdx.x % TPR;
   const int row = blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
-  // A product that follows may set itself up: at once beside a grid that leaves room, else when this one ends.
+  // A product that follows may set itself up: at once beside a grid that leaves room (two blocks on each of the 148 SMs),
+  // else when this one ends.
   const bool early = gridDim.x <= 296;
   if (early) tc::allow_dependent();
   const bool live = row < rows;

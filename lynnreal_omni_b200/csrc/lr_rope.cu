@@ -8,8 +8,8 @@
 // The angle of a far position is a large number of radians, of which fp32
 // keeps few digits after the point. It is therefore formed in turns,
 // p f / 2 pi, as an unevaluated sum of two floats: the whole turns fall away
-// exactly and sincospi sees an argument within [-2, 2] that is right to about
-// 1e-7, whatever the position.
+// exactly and what is left, below about 2 turns, is right to about 1e-7 of a turn;
+// sincospi's argument is twice that (below 4, right to 2e-7), whatever the position.
 //
 // Bound by memory: every value is read and written once (4 bytes a value).
 // Angles are computed once a token and kept in shared memory for all heads. 16384
