@@ -51,7 +51,8 @@ const char* lr_last_error(void);
  * modulation); bit 1: a bounded wait inside the GEMM gave up; bit 2: a row
  * index of lr_gather_rows / lr_flash_restore was outside its source (that
  * output row was written from zeros); bit 3: offsets of packed sequences went
- * down or outside their tensor. Bit 1 also covers the bounded waits of the
+ * down or outside their tensor; bit 4: a token's adapter number was past the
+ * last adapter (its row had none). Bit 1 also covers the bounded waits of the
  * attention and 4-bit GEMM kernels. Synchronises the device. */
 int lr_device_status(unsigned int* bits, int clear);
 
@@ -290,6 +291,23 @@ int lr_fp4_quantize_rows(const void* x, int64_t rows, int64_t width, int64_t row
  * rounded once; row_scales may be NULL (1). */
 int lr_fp4_dequantize_rows(const void* codes, const void* scales, const float* row_scales, int64_t rows,
                            int64_t width, int format, void* out, void* stream);
+
+/* D1 — low-rank adapters of many requests beside a shared projection (bf16):
+ *   out[t,:] = base[t,:] + scale[e] * up[e] (down[e] x[t,:]),  e = index[t]
+ * and out[t,:] = base[t,:] where index[t] < 0. x [tokens, width] and base, out
+ * [tokens, outputs] with row strides in elements (out may be base); down
+ * [adapters, rank, width], up [adapters, outputs, rank], contiguous; scale fp32
+ * [adapters] or NULL (1); index int32 [tokens] on the device, in any order (tokens
+ * of one adapter side by side are fastest). The inner values are summed in fp32,
+ * scaled and rounded to bf16; base and update are added in fp32 and rounded once.
+ * rank a multiple of 8 up to 128, width a multiple of 8, x rows and down, up
+ * 16-byte aligned. No counterpart in the reference. */
+int lr_adapters(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* down, const void* up,
+                const float* scale, const int32_t* index, int64_t tokens, int64_t width, int64_t outputs, int64_t rank,
+                int64_t adapters, void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that lr_adapters needs. */
+int64_t lr_adapters_workspace_bytes(int64_t tokens, int64_t width, int64_t outputs, int64_t rank, int64_t adapters);
 
 /* G4 — product of two 4-bit matrices with fp32 accumulation:
  *   out[m,n] = bf16((sum_k A[m,k] B[n,k]) * row_scale[m] * col_scale[n] + bias[n])

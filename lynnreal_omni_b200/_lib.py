@@ -62,6 +62,8 @@ SIGNATURES = {
     "lr_fp4_quantize_rows": ([_p, _i64, _i64, _i64, _i32, _p, _p, _p, _p], _i32),
     "lr_fp4_dequantize_rows": ([_p, _p, _p, _i64, _i64, _i32, _p, _p], _i32),
     "lr_fp4_gemm": ([_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _p], _i32),
+    "lr_adapters": ([_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p], _i32),
+    "lr_adapters_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
     "lr_int8_gemm": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i32, _p, _i64, _p,
                       _i64, _i64, _p, _i64, _i32, _p, _i64, _p], _i32),
     "lr_int8_gemm_workspace_bytes": ([_i64, _i64, _i64], _i64),
@@ -158,7 +160,7 @@ def arithmetic() -> str:
 
 def device_status(clear: bool = True) -> int:
     """Device status bits (1: adaLN index out of range, 2: a bounded wait gave up, 4: row index out of range,
-    8: offsets of packed sequences out of range)."""
+    8: offsets of packed sequences out of range, 16: a token's adapter number past the last adapter)."""
     bits = ctypes.c_uint(0)
     check(load().lr_device_status(ctypes.byref(bits), int(clear)), "device_status")
     return bits.value

@@ -1,0 +1,141 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+``add_adapters`` adds every token's own low-rank update to the output of a projection that all tokens share:
+
+    out[t] = base[t] + scale[e] * up[e] (down[e] x[t]),  e = index[t]        (index[t] < 0: out[t] = base[t])
+
+``AdaptedLinear`` puts it behind an ``Int8Linear``, an ``Fp4Linear`` or any other layer that maps bf16 rows to bf16 rows:
+
+    layer = AdaptedLinear.stack(Fp4Linear(linear), [(down0, up0, 2.0), (down1, up1, 0.5)])
+    index = token_adapters([0, 1, None], [3, 70, 12], "cuda")  # prompts of 3, 70 and 12 tokens, the last without one
+    y = layer(x, index)                                        # x bf16 [85, in_features]
+"""
+from __future__ import annotations
+
+import functools
+
+import torch
+from torch import nn
+
+from . import _lib
+from ._lib import check, ptr, stream_of
+
+__all__ = ["add_adapters", "token_adapters", "AdaptedLinear"]
+
+MOST_RANK = 128
+
+
+def token_adapters(adapters, lengths, device="cuda") -> torch.Tensor:
+    """int32 [tokens]: the adapter of each token of requests of these lengths, one after another (None: no adapter)."""
+    if len(adapters) != len(lengths) or (lengths and min(lengths) < 0):
+        raise ValueError("token_adapters: expected one adapter, or None, for each request's length")
+    if any(a is not None and a < 0 for a in adapters):
+        raise ValueError("token_adapters: adapters are numbered from 0")
+    numbers = torch.tensor([-1 if a is None else a for a in adapters], dtype=torch.int32)
+    return numbers.repeat_interleave(torch.tensor(lengths, dtype=torch.int64)).to(device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, tokens: int, width: int, outputs: int, rank: int, count: int) -> int:
+    """lr_adapters' need for these sizes on this device (a function of them alone)."""
+    return _lib.load().lr_adapters_workspace_bytes(tokens, width, outputs, rank, count)
+
+
+def _check_stack(name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None):
+    """(adapters, rank, width, outputs) of adapters that fit each other."""
+    for what, t in (("down", down), ("up", up)):
+        if t.dtype != torch.bfloat16 or t.ndim != 3:
+            raise ValueError(f"{name}: {what} must be a bf16 tensor of three dimensions, got {t.dtype} {tuple(t.shape)}")
+    count, rank, width = down.shape
+    if up.shape[0] != count or up.shape[2] != rank or up.device != down.device:
+        raise ValueError(f"{name}: down [adapters, rank, in] and up [adapters, out, rank] disagree: {tuple(down.shape)}, {tuple(up.shape)}")
+    if count == 0 or width == 0 or up.shape[1] == 0:
+        raise ValueError(f"{name}: no adapters, or empty ones")
+    if rank == 0 or rank % 8 or rank > MOST_RANK:
+        raise ValueError(f"{name}: the rank must be a multiple of 8 up to {MOST_RANK} (pad with zeros), got {rank}")
+    if width % 8:
+        raise ValueError(f"{name}: the input width must be a multiple of 8, got {width}")
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count or scale.device != down.device):
+        raise ValueError(f"{name}: scale must hold {count} fp32 values on the adapters' device")
+    return count, rank, width, up.shape[1]
+
+
+def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
+                 scale: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [tokens, out]: base plus every token's low-rank update.
+
+    base bf16 [tokens, out] and x bf16 [tokens, in]: rows may be strided; down bf16 [adapters, rank, in], up bf16
+    [adapters, out, rank], rank a multiple of 8 up to 128; scale fp32 [adapters] (None: 1); index int32 [tokens] on the
+    device, negative for no adapter (a number past the last adapter counts as none and raises bit 4 of the device status).
+    Any order will do, tokens of one adapter side by side are fastest. ``out`` may be ``base`` itself; it must not overlap
+    x, nor base in any other way."""
+    count, rank, width, outputs = _check_stack("add_adapters", down, up, scale)
+    device = down.device
+    for what, t, columns in (("base", base, outputs), ("x", x, width)):
+        if t.dtype != torch.bfloat16 or t.ndim != 2 or t.shape[1] != columns or t.device != device:
+            raise ValueError(f"add_adapters: {what} must be a bf16 [tokens, {columns}] tensor on the adapters' device, "
+                             f"got {t.dtype} {tuple(t.shape)}")
+    tokens = x.shape[0]
+    if base.shape[0] != tokens:
+        raise ValueError(f"add_adapters: base and x differ in tokens: {base.shape[0]}, {tokens}")
+    if index.dtype != torch.int32 or index.shape != (tokens,) or index.device != device:
+        raise ValueError("add_adapters: index must be int32 [tokens] on the adapters' device")
+    if out is None:
+        out = torch.empty(tokens, outputs, dtype=torch.bfloat16, device=device)
+    elif (out.dtype != torch.bfloat16 or out.shape != base.shape or out.device != device or out.stride(1) != 1
+          or (tokens > 1 and out.stride(0) < outputs)):
+        raise ValueError("add_adapters: out must be a bf16 tensor of base's shape with contiguous rows that do not overlap")
+    down, up, index = down.contiguous(), up.contiguous(), index.contiguous()
+    if scale is not None:
+        scale = scale.contiguous()
+    if base.stride(1) != 1 or base.stride(0) < 0:
+        base = base.contiguous()
+    x_stride = x.stride(0)
+    if x.stride(1) != 1 or x_stride % 8 or x.data_ptr() % 16:
+        x, x_stride = x.clone(memory_format=torch.contiguous_format), width
+    need = _workspace_bytes(down.get_device(), tokens, width, outputs, rank, count) if down.is_cuda else 0
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(_lib.load().lr_adapters(x.data_ptr(), x_stride, base.data_ptr(), base.stride(0), down.data_ptr(), up.data_ptr(),
+                                  ptr(scale), index.data_ptr(), tokens, width, outputs, rank, count, out.data_ptr(),
+                                  max(out.stride(0), outputs), ptr(workspace), need, stream_of(x)), "add_adapters")
+    return out
+
+
+class AdaptedLinear(nn.Module):
+    """A shared projection and the adapters of its requests. ``base``: a layer from bf16 [..., in] to bf16 [..., out]."""
+
+    def __init__(self, base: nn.Module, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None = None):
+        super().__init__()
+        _, _, width, outputs = _check_stack("AdaptedLinear", down, up, scale)
+        if width != base.in_features or outputs != base.out_features:
+            raise ValueError(f"AdaptedLinear: adapters of {width} to {outputs} beside a projection of {base.in_features} to "
+                             f"{base.out_features}")
+        self.base, self.in_features, self.out_features = base, width, outputs
+        self.register_buffer("down", down.contiguous())
+        self.register_buffer("up", up.contiguous())
+        self.register_buffer("scale", scale)
+
+    @classmethod
+    def stack(cls, base: nn.Module, adapters) -> "AdaptedLinear":
+        """From a list of (down [rank, in], up [out, rank], scale) of any ranks up to 128; ranks are padded with zeros."""
+        if not adapters:
+            raise ValueError("AdaptedLinear: no adapters")
+        ranks = [d.shape[0] for d, _, _ in adapters]
+        if any(d.ndim != 2 or u.ndim != 2 or u.shape[1] != r for (d, u, _), r in zip(adapters, ranks)):
+            raise ValueError("AdaptedLinear: expected (down [rank, in], up [out, rank], scale) for each adapter")
+        rank = max(8, -(-max(ranks) // 8) * 8)
+        device = adapters[0][0].device
+        down = torch.zeros(len(ranks), rank, base.in_features, dtype=torch.bfloat16, device=device)
+        up = torch.zeros(len(ranks), base.out_features, rank, dtype=torch.bfloat16, device=device)
+        for i, (d, u, _) in enumerate(adapters):
+            down[i, :ranks[i]], up[i, :, :ranks[i]] = d, u
+        return cls(base, down, up, torch.tensor([s for _, _, s in adapters], dtype=torch.float32, device=device))
+
+    def forward(self, x: torch.Tensor, index: torch.Tensor | None = None) -> torch.Tensor:
+        """x bf16 [..., in], index int32 with a number for each row (None: the shared projection alone)."""
+        y = self.base(x)
+        if index is None:
+            return y
+        rows = y.view(-1, self.out_features)
+        add_adapters(rows, x.reshape(-1, self.in_features), self.down, self.up, index.reshape(-1), self.scale, out=rows)
+        return y

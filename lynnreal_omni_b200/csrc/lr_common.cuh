@@ -39,6 +39,7 @@ enum : unsigned int {
   kDevErrWaitTimeout = 1u << 1, // a bounded mbarrier wait gave up
   kDevErrRowIndex = 1u << 2,    // a gather/restore row index pointed outside its source
   kDevErrOffsets = 1u << 3,     // sequence offsets went down or outside their tensor
+  kDevErrAdapter = 1u << 4,     // a token's adapter number is past the last adapter
 };
 
 // ------------------------------------------------------- scalar bf16 helpers

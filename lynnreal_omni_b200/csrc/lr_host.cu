@@ -45,6 +45,7 @@ int read_status_flash(unsigned int* bits, int clear);
 int read_status_attention(unsigned int* bits, int clear);
 int read_status_packed(unsigned int* bits, int clear);
 int read_status_fp4(unsigned int* bits, int clear);
+int read_status_adapters(unsigned int* bits, int clear);
 
 }  // namespace lr
 
@@ -66,7 +67,9 @@ extern "C" int lr_device_status(unsigned int* bits, int clear) {
   if (st) return st;
   st = lr::read_status_packed(bits, clear);
   if (st) return st;
-  return lr::read_status_fp4(bits, clear);
+  st = lr::read_status_fp4(bits, clear);
+  if (st) return st;
+  return lr::read_status_adapters(bits, clear);
 }
 
 // ------------------------------------------------------------- CUDA IPC
