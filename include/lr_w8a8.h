@@ -251,6 +251,23 @@ int lr_attention_packed(const void* q, int64_t q_token_stride, int64_t q_head_st
 int64_t lr_attention_packed_workspace_bytes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads,
                                             int64_t kv_heads, int64_t head_dim);
 
+/* A3 — A2 for sequences that all continue one prefix: prefix_k, prefix_v
+ * [prefix, kv_heads, head_dim] (strides as the other operands', prefix > 0) stand
+ * in front of every sequence's keys. Each query sees the whole prefix and, of its
+ * own sequence's keys, those that A2 shows it; rows of q past cu_q[seqs] give
+ * zeros. workspace 32-byte aligned. No counterpart in the reference. */
+int lr_attention_shared(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const void* prefix_k, int64_t pk_token_stride, int64_t pk_head_stride,
+                        const void* prefix_v, int64_t pv_token_stride, int64_t pv_head_stride, const int32_t* cu_q,
+                        const int32_t* cu_k, int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix,
+                        int64_t heads, int64_t kv_heads, int64_t head_dim, int causal, float scale, void* out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that lr_attention_shared needs for these counts. */
+int64_t lr_attention_shared_workspace_bytes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix,
+                                            int64_t heads, int64_t kv_heads, int64_t head_dim);
+
 /* R1 — rotary position embedding of q and k (bf16), no tables: the pair of
  * frequency i of a token at position p is turned by p * inv_freq[i] radians
  * (evaluated in turns to about 1e-7 for |p| < 2^36) and multiplied by `factor`;

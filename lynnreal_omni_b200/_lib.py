@@ -57,6 +57,9 @@ SIGNATURES = {
     "lr_attention_packed": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
                              _i64, _i32, _f32, _p, _p, _i64, _p], _i32),
     "lr_attention_packed_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
+    "lr_attention_shared": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64,
+                             _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f32, _p, _p, _i64, _p], _i32),
+    "lr_attention_shared_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "lr_rope": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _f32, _i64, _i64, _i64, _i32, _p, _p,
                  _p], _i32),
     "lr_fp4_quantize_rows": ([_p, _i64, _i64, _i64, _i32, _p, _p, _p, _p], _i32),

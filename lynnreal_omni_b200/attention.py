@@ -10,7 +10,8 @@ remains available as ``fusion.sdpa_bshd`` for callers that need those.
 
 ``attention_packed`` is the attention of prompts of different lengths, packed
 without padding: causal or full, with grouped key/value heads, and with fewer
-queries than keys (a decoding step, a piece of a prompt).
+queries than keys (a decoding step, a piece of a prompt). ``attention_shared`` is the same for sequences that all
+continue one prefix, whose keys and values are stored and read once.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ import torch
 from . import _lib
 from ._lib import check, ptr, stream_of
 
-__all__ = ["attention_bshd", "attention_packed"]
+__all__ = ["attention_bshd", "attention_packed", "attention_shared"]
 
 
 def _token_view(t: torch.Tensor) -> torch.Tensor:
@@ -124,4 +125,64 @@ def attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         query.data_ptr(), q_ts, q_hs, key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, cu_seqlens_q.data_ptr(),
         cu_seqlens_k.data_ptr(), seqs, tq, tk, h, hk, d, bool(causal), sc, out.data_ptr(), ptr(workspace), need,
         stream_of(query)), "attention_packed")
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace_bytes(device: int, seqs: int, tq: int, tk: int, prefix: int, heads: int, kv_heads: int, d: int) -> int:
+    """lr_attention_shared's need for these counts on this device (a function of them alone)."""
+    return _lib.load().lr_attention_shared_workspace_bytes(seqs, tq, tk, prefix, heads, kv_heads, d)
+
+
+def attention_shared(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, prefix_key: torch.Tensor,
+                     prefix_value: torch.Tensor, cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor | None = None, *,
+                     causal: bool = True, scale: float | None = None) -> torch.Tensor:
+    """Attention of packed sequences that all continue one prefix -> bf16 [tokens, heads, D].
+
+    As ``attention_packed``, with prefix_key and prefix_value bf16 [prefix, kv_heads, D] in front of every sequence's keys:
+    each query sees the whole prefix and, of its own sequence's keys, those that ``attention_packed`` shows it (a query
+    that sees none of those still sees the prefix; tokens past the last offset give zeros). The prefix's
+    keys and values are shared by all sequences, not copied; a single length for it, known to the host. Values of other
+    sequences never reach a row; within a sequence, values of masked keys must be finite.
+
+    Kernels are chosen by the average number of queries a sequence, as there."""
+    device = query.device
+    for name, t in (("query", query), ("key", key), ("value", value), ("prefix_key", prefix_key), ("prefix_value", prefix_value)):
+        if t.dtype != torch.bfloat16 or t.ndim != 3 or not t.is_cuda:
+            raise ValueError(f"attention_shared: {name} must be a CUDA bf16 [tokens, heads, D] tensor")
+        if t.device != device:
+            raise ValueError("attention_shared: query, keys and values are on different devices")
+    tq, h, d = query.shape
+    tk, hk, dk = key.shape
+    prefix = prefix_key.shape[0]
+    if value.shape != key.shape or dk != d or prefix_value.shape != prefix_key.shape or prefix_key.shape[1:] != key.shape[1:]:
+        raise ValueError("attention_shared: query/key/value/prefix shapes disagree")
+    if d not in (64, 128):
+        raise ValueError(f"attention_shared: head_dim {d} (the kernel handles 64 and 128)")
+    if hk == 0 or h == 0 or h % hk:
+        raise ValueError(f"attention_shared: {h} query heads do not share {hk} key/value heads evenly")
+    if cu_seqlens_k is None:
+        if tk != tq:
+            raise ValueError("attention_shared: cu_seqlens_k is needed where queries and keys differ in tokens")
+        cu_seqlens_k = cu_seqlens_q
+    if prefix == 0:
+        return attention_packed(query, key, value, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale)
+    count = cu_seqlens_q.numel()
+    for t in (cu_seqlens_q, cu_seqlens_k):
+        if t.dtype != torch.int32 or t.ndim != 1 or count < 2 or t.device != device:
+            raise ValueError("attention_shared: cu_seqlens must be int32 [sequences + 1] on the query's device")
+    if cu_seqlens_k.numel() != count:
+        raise ValueError("attention_shared: cu_seqlens_q and cu_seqlens_k differ in sequences")
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
+    (query, q_ts, q_hs), (key, k_ts, k_hs), (value, v_ts, v_hs) = _head_view(query), _head_view(key), _head_view(value)
+    (prefix_key, pk_ts, pk_hs), (prefix_value, pv_ts, pv_hs) = _head_view(prefix_key), _head_view(prefix_value)
+    out = torch.empty(tq, h, d, dtype=torch.bfloat16, device=device)
+    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    lib, seqs = _lib.load(), count - 1
+    need = _shared_workspace_bytes(query.get_device(), seqs, tq, tk, prefix, h, hk, d)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(lib.lr_attention_shared(
+        query.data_ptr(), q_ts, q_hs, key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, prefix_key.data_ptr(), pk_ts,
+        pk_hs, prefix_value.data_ptr(), pv_ts, pv_hs, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), seqs, tq, tk, prefix, h,
+        hk, d, bool(causal), sc, out.data_ptr(), ptr(workspace), need, stream_of(query)), "attention_shared")
     return out

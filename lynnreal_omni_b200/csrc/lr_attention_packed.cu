@@ -233,6 +233,19 @@ struct PromptShape {
   int wide_out;     // out is 32-byte aligned
 };
 
+// What a prefix in front of every sequence adds to the prompt kernel.
+enum PrefixMode {
+  kNoPrefix,
+  kWithPrefix,  // a block takes the prefix's keys, then its sequence's
+  kPrefixPart,  // a block takes a run of the prefix's keys for rows of any sequences and leaves a part
+};
+struct Prefix {
+  int keys, tiles;
+  int chunk, chunks;  // kPrefixPart: keys of a run, runs
+  float* part_o;      // [chunks][total_q][heads][D] unnormalised
+  float2* part_ml;    // [chunks][total_q][heads] maximum (base 2, scaled) and sum
+};
+
 // A block of work: two query tiles of one key/value head (or a part of its group).
 struct PromptItem {
   int q_row;       // first query token
@@ -250,7 +263,9 @@ constexpr int kItemSlots = 4;
 // (16 sequences of up to 2048 tokens, 24 heads of 64: 51 -> 41 us; 24 of up to
 // 1500, 32 heads of 128: 229 -> 196 us), else each sequence's in turn (40 such
 // sequences are as fast either way: there are blocks enough to even out).
-__device__ __forceinline__ bool prompt_item(const Args& a, const PromptShape& ps, int index, int lane, PromptItem& w) {
+template <int MODE>
+__device__ __forceinline__ bool prompt_item(const Args& a, const PromptShape& ps, const Prefix& px, int index, int lane,
+                                            PromptItem& w) {
   const int parts = a.kv_heads * ps.head_parts;
   const int part = index % parts, rank = index / parts;
   w.kv_head = part / ps.head_parts;
@@ -258,6 +273,16 @@ __device__ __forceinline__ bool prompt_item(const Args& a, const PromptShape& ps
   w.heads_here = min(ps.tile_heads, a.group - in_group);
   w.head0 = w.kv_head * a.group + in_group;
   const int block = 2 * ps.tokens_tile;
+  if constexpr (MODE == kPrefixPart) {  // rank: run of keys, then block of tokens
+    w.tok0 = rank / px.chunks * block;
+    w.q_row = w.tok0;
+    w.lq = a.total_q;
+    w.k_row = rank % px.chunks * px.chunk;
+    w.lk = min(px.chunk, px.keys - w.k_row);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) w.tiles[t] = w.tok0 + t * ps.tokens_tile < w.lq ? (w.lk + kKeys - 1) / kKeys : 0;
+    return true;
+  }
   // "Sequence" a.seqs is what lies past the last offset: queries without keys.
   int b, qs, qe, ke;
   if (a.seqs < 32) {  // every offset in one lane: one round of loads
@@ -305,6 +330,7 @@ __device__ __forceinline__ bool prompt_item(const Args& a, const PromptShape& ps
     const int first = w.tok0 + t * ps.tokens_tile, last = min(first + ps.tokens_tile, w.lq) - 1;
     const int seen = first >= w.lq ? 0 : a.causal ? min(max(last + w.lk - w.lq + 1, 0), w.lk) : w.lk;
     w.tiles[t] = (seen + kKeys - 1) / kKeys;
+    if (MODE == kWithPrefix && first < w.lq && b < a.seqs) w.tiles[t] += px.tiles;
   }
   return true;
 }
@@ -351,10 +377,14 @@ __device__ __forceinline__ void store_16(bf16* dst, const uint32_t* y, int wide)
 // probabilities, half a column a key, overwrite its own scores. The softmax
 // therefore reads a tile's first half twice instead of holding 128 scores a
 // thread, and hands the second half over first.
-template <int D>
+//
+// With a prefix (kWithPrefix) its key tiles come first, from maps of their own;
+// as parts (kPrefixPart) map_k and map_v are the prefix's.
+template <int D, int MODE>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const Args a, const PromptShape ps) {
+                  const __grid_constant__ CUtensorMap map_v, const Args a, const PromptShape ps,
+                  const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv, const Prefix px) {
   using C = Prompt<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -379,9 +409,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_map(&map_q);
-    if (a.total_k > 0) {  // else there is no map
+    if (MODE == kPrefixPart || a.total_k > 0) {  // else there is no map
       prefetch_map(&map_k);
       prefetch_map(&map_v);
+    }
+    if (MODE == kWithPrefix) {
+      prefetch_map(&map_pk);
+      prefetch_map(&map_pv);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&q_full[t]), 1);
@@ -411,7 +445,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   };
   PromptItem first{};
   bool first_there = false;
-  if (warp == 3) first_there = prompt_item(a, ps, item_index(0), lane, first);
+  if (MODE == kPrefixPart) allow_dependent();  // the step kernel, which waits for this one before it reads the parts
+  if (warp == 3) first_there = prompt_item<MODE>(a, ps, px, item_index(0), lane, first);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -436,7 +471,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (warp < 4) {
     if (warp == 3) {
       // ------------------------------------------------------- items
-      if (blockIdx.x == 0) check_offsets(a, lane, 32);
+      if (MODE != kPrefixPart && blockIdx.x == 0) check_offsets(a, lane, 32);
       uint32_t number = 0;
       for (int round = 0;; ++round) {
         PromptItem w{};
@@ -444,7 +479,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (round == 0) {
           if (!first_there) continue;
           w = first;
-        } else if (!end && (item_index(round) >= ps.items || !prompt_item(a, ps, item_index(round), lane, w))) {
+        } else if (!end && (item_index(round) >= ps.items || !prompt_item<MODE>(a, ps, px, item_index(round), lane, w))) {
           continue;
         }
         const uint32_t s = number % kItemSlots;
@@ -484,9 +519,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (el && ok) {
             const uint32_t bar = entry_bar(full, e), dst = entry_addr(e);
             mbar_expect_tx(bar, C::kTile);
+            const int tile = i >> 1;
+            if (MODE == kWithPrefix && tile < px.tiles) {
 #pragma unroll
-            for (int x = 0; x < D / 64; ++x)
-              tma_load_3d(dst + x * kAtom, i & 1 ? &map_v : &map_k, bar, x * 64, w.kv_head, w.k_row + (i >> 1) * kKeys);
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_3d(dst + x * kAtom, i & 1 ? &map_pv : &map_pk, bar, x * 64, w.kv_head, tile * kKeys);
+            } else {
+              const int row = w.k_row + (MODE == kWithPrefix ? tile - px.tiles : tile) * kKeys;
+#pragma unroll
+              for (int x = 0; x < D / 64; ++x) tma_load_3d(dst + x * kAtom, i & 1 ? &map_v : &map_k, bar, x * 64, w.kv_head, row);
+            }
           }
           __syncwarp();
         }
@@ -509,13 +551,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int j = -1; j < most && ok; ++j) {
           const uint32_t ev = e0 + 2 * j + 1, ek = ev + 1;  // V_j, K_{j+1}
           if (j >= 0 && !(ok = warp_wait(entry_bar(full, ev), entry_phase(ev), watch, lane))) break;
-          if (j >= 0 && j == most - 1 && most * kKeys > w.lk) {
+          const int before = MODE == kWithPrefix ? px.tiles : 0;  // tiles of the prefix: past its end there are zeros
+          if (j >= before && j == most - 1 && (most - before) * kKeys > w.lk) {
             // The last V tile ends past the sequence: its rows there, another sequence's, become zeros (their
             // probabilities are 0, but 0 times an infinity is not).
             uint8_t* tile = smem + C::kRing + (ev % C::kSlots) * C::kTile;
 #pragma unroll
             for (int x = 0; x < D / 64; ++x)
-              for (int i = (w.lk - j * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
+              for (int i = (w.lk - (j - before) * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
                 *reinterpret_cast<uint4*>(tile + x * kAtom + i * 16) = make_uint4(0u, 0u, 0u, 0u);
             fence_async_smem();
             __syncwarp();
@@ -591,14 +634,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     PromptItem w;
     for (uint32_t number = 0; ok && next_item(number, w); ++number) {
       // keys that this row sees, -1 for a row that stands for nothing
-      int seen = -1;
+      int seen = -1, prefix_seen = -1;
       bf16* dst = a.out;
+      int64_t part = 0;
       {
         const int offset = t * ps.tokens_tile + in_tile;  // of this row's token in the block
         const int token = w.tok0 + offset;
         if (in_tile < ps.tokens_tile && head < w.heads_here && token < w.lq) {
-          seen = a.causal ? min(max(token + w.lk - w.lq + 1, 0), w.lk) : w.lk;
-          dst += ((int64_t)(w.q_row + offset) * a.heads + w.head0 + head) * D;
+          seen = MODE != kPrefixPart && a.causal ? min(max(token + w.lk - w.lq + 1, 0), w.lk) : w.lk;
+          if (MODE == kWithPrefix) prefix_seen = px.keys;
+          const int64_t at = (int64_t)(w.q_row + offset) * a.heads + w.head0 + head;
+          dst += at * D;
+          if (MODE == kPrefixPart) part = (int64_t)(w.k_row / px.chunk) * a.total_q * a.heads + at;
         }
       }
       const int n = w.tiles[t];
@@ -607,7 +654,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!(ok = warp_wait(smem_u32(&s_full[t]), done & 1u, watch, lane))) break;
         tc_fence_after();
         // Both halves for the maximum; the second stays in registers, the first is read again for its probabilities.
-        const int valid = seen - j * kKeys;
+        const int valid = MODE == kWithPrefix ? (j < px.tiles ? prefix_seen - j * kKeys : seen - (j - px.tiles) * kKeys)
+                                              : seen - j * kKeys;
         const bool full_tile = __all_sync(0xffffffffu, valid >= kKeys);
         uint32_t s[kHalf];
         float mx = -INFINITY;
@@ -678,12 +726,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
         }
         if (seen < 0) continue;
-        uint32_t y[16];
+        if constexpr (MODE == kPrefixPart) {
+          float* to = px.part_o + part * D + c;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          y[e] = seen == 0 ? 0u : cvt2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          for (int x = 0; x < 4; ++x)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 8 * x), "r"(o[8 * x]),
+                         "r"(o[8 * x + 1]), "r"(o[8 * x + 2]), "r"(o[8 * x + 3]), "r"(o[8 * x + 4]), "r"(o[8 * x + 5]),
+                         "r"(o[8 * x + 6]), "r"(o[8 * x + 7])
+                         : "memory");
+          if (c == 0) px.part_ml[part] = make_float2(m_run, l_run);
+        } else {
+          uint32_t y[16];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) store_16(dst + c + 16 * x, y + 8 * x, ps.wide_out);
+          for (int e = 0; e < 16; ++e)
+            y[e] = (MODE == kWithPrefix ? n == 0 : seen == 0)
+                       ? 0u
+                       : cvt2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) store_16(dst + c + 16 * x, y + 8 * x, ps.wide_out);
+        }
       }
     }
   }
@@ -732,16 +793,56 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// What a prefix in front of every sequence adds to the step kernel.
+struct StepPrefix {
+  const bf16 *k, *v;
+  int64_t k_ts, k_hs, v_ts, v_hs;
+  int keys;
+  int chunk, chunks;  // keys of a part of the prefix, parts
+  int slots;          // chunks where this kernel makes the prefix's parts itself, 0 where prompt_kernel has
+  float *part_o, *own_o;      // [chunks][total_q][heads][D], [total_q][heads][D] (the sequences that are not split)
+  float2 *part_ml, *own_ml;
+};
+
+// One row's parts, added in order, to y (columns lane, lane + 32, ...) and sum, which belong to the maximum `top`: a warp.
+template <int D>
+__device__ __forceinline__ void add_prefix(const StepPrefix& sp, int64_t rows, int64_t row, int lane, float& top, float& sum,
+                                           float (&y)[D / 32]) {
+  float most = top;
+  for (int p = lane; p < sp.chunks; p += 32) most = fmaxf(most, __ldcg(&sp.part_ml[p * rows + row]).x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  const float sub = most == -INFINITY ? 0.0f : most, f = ex2(top - sub);
+  sum *= f;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) y[c] *= f;
+#pragma unroll 4
+  for (int p = 0; p < sp.chunks; ++p) {
+    const float2 ml = __ldcg(&sp.part_ml[p * rows + row]);
+    const float g = ex2(ml.x - sub);
+    sum = fmaf(ml.y, g, sum);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) y[c] = fmaf(__ldcg(&sp.part_o[(p * rows + row) * D + c * 32 + lane]), g, y[c]);
+  }
+  top = most;
+}
+
 // NT tiles of 8 rows. A CTA takes one slot's keys for one key/value head and
 // every gridDim.z-th group of 8 NT rows.
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, const StepShape ss) {
+//
+// SHARED: behind a prefix. Its parts either come from this kernel's first slots,
+// for the rows of all sequences (then join_shared_kernel joins every row's), or
+// from prompt_kernel, which runs meanwhile: rows of a sequence that is not split
+// take them up here.
+template <int D, int NT, bool SHARED>
+__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   constexpr int R = 8 * NT;
   __shared__ float sh_m[kStepWarps][R], sh_l[kStepWarps][R];
   __shared__ float sh_o[kStepWarps][R][D + 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int slot = blockIdx.x, kv_head = blockIdx.y;
+  const bool of_prefix = SHARED && (int)blockIdx.x < sp.slots;
+  const int slot = SHARED ? (int)blockIdx.x - sp.slots : (int)blockIdx.x, kv_head = blockIdx.y;
   if (slot == 0 && kv_head == 0 && blockIdx.z == 0 && warp == 0) check_offsets(a, lane, 32);
   if (slot == 0 && blockIdx.z == 0) {  // tokens past the last offset
     const int from = clamped(a.cu_q, a.seqs, a.total_q);
@@ -752,16 +853,32 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
       *reinterpret_cast<uint4*>(a.out + at) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  const int b = find_sequence(a.cu_k, a.seqs - 1, a.total_k, ss.chunk, slot, lane);
-  const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
-  const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
+  int ks = 0, lk = sp.keys, qs = 0, lq = a.total_q, index = blockIdx.x, k0, k1;
+  bool split = false, causal = false;
+  const bf16 *keys = a.k, *values = a.v;
+  int64_t k_ts = a.k_ts, k_hs = a.k_hs, v_ts = a.v_ts, v_hs = a.v_hs;
+  if (SHARED && of_prefix) {
+    keys = sp.k, values = sp.v;
+    k_ts = sp.k_ts, k_hs = sp.k_hs, v_ts = sp.v_ts, v_hs = sp.v_hs;
+    k0 = index * sp.chunk;
+    k1 = min(k0 + sp.chunk, lk);
+  } else {
+    const int b = find_sequence(a.cu_k, a.seqs - 1, a.total_k, ss.chunk, slot, lane);
+    ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
+    qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
+    index = slot - (int)((uint32_t)ks / (uint32_t)ss.chunk) - b;
+    const int pieces = max((int)((lk + (int64_t)ss.chunk - 1) / ss.chunk), 1);
+    // a sequence with more rows than the parts have room for is not split
+    split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
+    if (index < 0 || index >= pieces || (index > 0 && !split)) {
+      if (SHARED && sp.slots == 0) wait_for_predecessor();
+      return;
+    }
+    k0 = split ? index * ss.chunk : 0, k1 = split ? min(k0 + ss.chunk, lk) : lk;
+    causal = a.causal;
+  }
   const int rows = lq * a.group;
-  const int index = slot - (int)((uint32_t)ks / (uint32_t)ss.chunk) - b;
-  const int pieces = max((int)((lk + (int64_t)ss.chunk - 1) / ss.chunk), 1);
-  // a sequence with more rows than the parts have room for is not split
-  const bool split = pieces > 1 && rows <= ss.max_rows;
-  if (index < 0 || index >= pieces || (index > 0 && !split)) return;
-  const int k0 = split ? index * ss.chunk : 0, k1 = split ? min(k0 + ss.chunk, lk) : lk;
+  bool waited = false;
 
   for (int r0 = blockIdx.z * R; r0 < rows; r0 += gridDim.z * R) {
     // Q^T: row g of each row tile, the columns that this thread loads of K.
@@ -785,7 +902,7 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = r0 + n * 8 + 2 * t + e;
-        see[n][e] = r >= rows ? k1 : a.causal ? min(max(r / a.group + lk - lq + 1, 0), lk) : lk;
+        see[n][e] = r >= rows ? k1 : causal ? min(max(r / a.group + lk - lq + 1, 0), lk) : lk;
         least = min(least, see[n][e]);
         m[n][e] = -INFINITY;
         l[n][e] = 0.0f;
@@ -803,14 +920,14 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
       uint4 kr[2][D / 32], vr[4][D / 64];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bf16* src = a.k + (int64_t)(ks + min(k + g + 8 * h, k1 - 1)) * a.k_ts + (int64_t)kv_head * a.k_hs + t * 8;
+        const bf16* src = keys + (int64_t)(ks + min(k + g + 8 * h, k1 - 1)) * k_ts + (int64_t)kv_head * k_hs + t * 8;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) kr[h][c] = ld_stream(src + c * 32);
       }
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const int key = k + 2 * t + (h & 1) + (h >> 1) * 8;
-        const bf16* src = a.v + (int64_t)(ks + min(key, k1 - 1)) * a.v_ts + (int64_t)kv_head * a.v_hs + g * 8;
+        const bf16* src = values + (int64_t)(ks + min(key, k1 - 1)) * v_ts + (int64_t)kv_head * v_hs + g * 8;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           vr[h][c] = ld_stream(src + c * 64);
@@ -883,6 +1000,10 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
     allow_dependent();  // join_kernel looks its row up meanwhile
     // The warps' parts to shared memory, added in order.
     __syncthreads();
+    if (SHARED && sp.slots == 0 && !waited) {
+      wait_for_predecessor();
+      waited = true;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -921,6 +1042,19 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
         for (int w = 0; w < kStepWarps; ++w) y[c] = fmaf(sh_o[w][r][c * 32 + lane], f[w], y[c]);
       }
       const int row = r0 + r;
+      if constexpr (SHARED) {
+        const int64_t all = (int64_t)a.total_q * a.heads;
+        const int64_t at = (int64_t)(qs + row / a.group) * a.heads + kv_head * a.group + row % a.group;
+        if (of_prefix || (!split && sp.slots > 0)) {
+          float* to = of_prefix ? sp.part_o + index * all * D : sp.own_o;
+          float2* to_ml = of_prefix ? sp.part_ml + index * all : sp.own_ml;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) to[at * D + c * 32 + lane] = y[c];
+          if (lane == 0) to_ml[at] = make_float2(top, sum);
+          continue;
+        }
+        if (!split) add_prefix<D>(sp, all, at, lane, top, sum, y);
+      }
       if (split) {
         const int64_t at = ((first_part(ks, ss.chunk) + index) * a.kv_heads + kv_head) * ss.max_rows + row;
 #pragma unroll
@@ -928,7 +1062,7 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
         if (lane == 0) ss.part_ml[at] = make_float2(top, sum);
       } else {
         const int token = row / a.group;
-        const int seen = a.causal ? min(token + lk - lq + 1, lk) : lk;
+        const int seen = SHARED ? 1 : causal ? min(token + lk - lq + 1, lk) : lk;
         const float inv = 1.0f / sum;
         bf16* dst = a.out + ((int64_t)(qs + token) * a.heads + kv_head * a.group + row % a.group) * D;
 #pragma unroll
@@ -936,12 +1070,16 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, con
       }
     }
   }
+  if (SHARED && sp.slots == 0 && !waited) wait_for_predecessor();  // a sequence without queries
 }
 
 // The parts of the sequences whose keys were split: a block a row, a thread a
 // column and every THREADS / D-th part; the groups' sums are added in order.
-template <int D, int THREADS>
-__global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepShape ss) {
+//
+// SHARED: behind a prefix, whose parts are joined as well: for every row where
+// the step kernel made them, else for the sequences that were split.
+template <int D, int THREADS, bool SHARED>
+__global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   constexpr int kGroups = THREADS / D;
   __shared__ float sh_y[kGroups][D], sh_l[kGroups];
   const int lane = threadIdx.x & 31;
@@ -959,27 +1097,41 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
   const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
   const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
   const int pieces = (int)((lk + (int64_t)ss.chunk - 1) / ss.chunk);
-  if (pieces <= 1 || (int64_t)lq * a.group > ss.max_rows || tok < qs || tok >= qs + lq) {
+  const bool split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
+  if (!(split || (SHARED && sp.slots > 0)) || tok < qs || tok >= qs + lq) {
     wait_for_predecessor();
     return;
   }
   const int row = (tok - qs) * a.group + head % a.group;
-  const int seen = a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
+  const int seen = SHARED ? 1 : a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
   const int64_t stride = (int64_t)a.kv_heads * ss.max_rows;
   const int64_t at = (first_part(ks, ss.chunk) * a.kv_heads + head / a.group) * ss.max_rows + row;
+  const int64_t all = (int64_t)a.total_q * a.heads;
+  // part p: the sequence's own, then the prefix's
+  const int own = split ? pieces : 1, parts = SHARED ? own + sp.chunks : own;
+  const auto part_ml = [&](int p) -> float2 {
+    if (SHARED && p >= own) return sp.part_ml[(p - own) * all + item];
+    if (SHARED && !split) return sp.own_ml[item];
+    return ss.part_ml[at + p * stride];
+  };
+  const auto part_o = [&](int p) -> float {
+    if (SHARED && p >= own) return sp.part_o[((p - own) * all + item) * D + col];
+    if (SHARED && !split) return sp.own_o[item * D + col];
+    return ss.part_o[(at + p * stride) * D + col];
+  };
   wait_for_predecessor();
   float top = -INFINITY;
-  for (int p = lane; p < pieces; p += 32) top = fmaxf(top, ss.part_ml[at + p * stride].x);
+  for (int p = lane; p < parts; p += 32) top = fmaxf(top, part_ml(p).x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float sub = top == -INFINITY ? 0.0f : top;
   float y = 0.0f, sum = 0.0f;
 #pragma unroll 8
-  for (int p = group; p < pieces; p += kGroups) {
-    const float2 ml = ss.part_ml[at + p * stride];
+  for (int p = group; p < parts; p += kGroups) {
+    const float2 ml = part_ml(p);
     const float f = ex2(ml.x - sub);
     sum = fmaf(ml.y, f, sum);
-    y = fmaf(ss.part_o[(at + p * stride) * D + col], f, y);
+    y = fmaf(part_o(p), f, y);
   }
   sh_y[group][col] = y;
   if (col == 0) sh_l[group] = sum;
@@ -1032,53 +1184,114 @@ int head_map(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, 
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int D>
-int launch_prompt(const Args& a, cudaStream_t stream) {
+template <int D, int MODE>
+int launch_prompt(const Args& a, const StepPrefix& sp, int64_t most_blocks, cudaStream_t stream) {
   using C = Prompt<D>;
   PromptShape ps;
   ps.head_parts = (a.group + kRows - 1) / kRows;
   ps.tile_heads = (a.group + ps.head_parts - 1) / ps.head_parts;
   ps.tokens_tile = kRows / ps.tile_heads;
   ps.slots = a.total_q / (2 * ps.tokens_tile) + a.seqs + 1;
+  if (MODE == kPrefixPart) ps.slots = (a.total_q + 2 * ps.tokens_tile - 1) / (2 * ps.tokens_tile) * sp.chunks;
   const int64_t items = (int64_t)ps.slots * a.kv_heads * ps.head_parts;
   LR_REQUIRE(items <= INT32_MAX - 65536, "attention_packed: too many blocks");
   ps.items = (int)items;
   ps.wide_out = aligned(a.out, 32);
-  CUtensorMap mq, mk{}, mv{};
+  const Prefix px{sp.keys, (sp.keys + kKeys - 1) / kKeys, sp.chunk, sp.chunks, sp.part_o, sp.part_ml};
+  CUtensorMap mq, mk{}, mv{}, mpk{}, mpv{};
   int st = head_map<D>(&mq, a.q, a.heads, a.total_q, a.q_ts, a.q_hs, (uint32_t)ps.tile_heads, (uint32_t)ps.tokens_tile);
   if (st) return st;
-  if (a.total_k > 0 && ((st = head_map<D>(&mk, a.k, a.kv_heads, a.total_k, a.k_ts, a.k_hs, 1, kKeys)) ||
+  if (MODE != kNoPrefix && ((st = head_map<D>(&mpk, sp.k, a.kv_heads, sp.keys, sp.k_ts, sp.k_hs, 1, kKeys)) ||
+                            (st = head_map<D>(&mpv, sp.v, a.kv_heads, sp.keys, sp.v_ts, sp.v_hs, 1, kKeys))))
+    return st;
+  if (MODE == kPrefixPart) mk = mpk, mv = mpv;
+  if (MODE != kPrefixPart && a.total_k > 0 && ((st = head_map<D>(&mk, a.k, a.kv_heads, a.total_k, a.k_ts, a.k_hs, 1, kKeys)) ||
                         (st = head_map<D>(&mv, a.v, a.kv_heads, a.total_k, a.v_ts, a.v_hs, 1, kKeys))))
     return st;
   static bool done[64] = {};
-  if ((st = configure_smem(prompt_kernel<D>, C::kSmem, done))) return st;
-  prompt_kernel<D><<<(unsigned)(items < sm_count() ? items : sm_count()), kPromptThreads, C::kSmem, stream>>>(mq, mk, mv, a, ps);
-  return launch_status("attention_packed (prompts)");
+  if ((st = configure_smem(prompt_kernel<D, MODE>, C::kSmem, done))) return st;
+  prompt_kernel<D, MODE><<<(unsigned)(items < most_blocks ? items : most_blocks), kPromptThreads, C::kSmem, stream>>>(
+      mq, mk, mv, a, ps, mpk, mpv, px);
+  return launch_status(MODE == kNoPrefix ? "attention_packed (prompts)" : "attention_shared (prompts)");
 }
 
-template <int D>
-int launch_step(const Args& a, const Plan& p, void* workspace, cudaStream_t stream) {
+template <int D, bool SHARED>
+int launch_step(const Args& a, const Plan& p, const StepPrefix& sp, void* workspace, cudaStream_t stream) {
   StepShape ss{p.chunk, p.slots, p.max_rows, nullptr, nullptr};
   if (p.bytes > 0) {
     ss.part_o = static_cast<float*>(workspace);
     ss.part_ml = reinterpret_cast<float2*>(ss.part_o + p.parts * a.kv_heads * p.max_rows * D);
   }
-  const int nt = p.max_rows <= 8 ? 1 : 2;
-  const dim3 grid((unsigned)p.slots, (unsigned)a.kv_heads, (unsigned)((p.max_rows + 8 * nt - 1) / (8 * nt)));
-  if (nt == 1)
-    step_kernel<D, 1><<<grid, 32 * kStepWarps, 0, stream>>>(a, ss);
-  else
-    step_kernel<D, 2><<<grid, 32 * kStepWarps, 0, stream>>>(a, ss);
-  int st = launch_status("attention_packed (steps)");
-  if (st || p.bytes == 0) return st;
+  const int most_rows = sp.slots > 0 && a.total_q * a.group > p.max_rows ? a.total_q * a.group : p.max_rows;
+  const int nt = most_rows <= 8 ? 1 : 2;
+  const dim3 grid((unsigned)(p.slots + sp.slots), (unsigned)a.kv_heads, (unsigned)((most_rows + 8 * nt - 1) / (8 * nt)));
+  const int st = launch(SHARED ? "attention_shared (steps)" : "attention_packed (steps)",
+                        nt == 1 ? step_kernel<D, 1, SHARED> : step_kernel<D, 2, SHARED>, grid, 32 * kStepWarps, 0, stream, 1,
+                        SHARED && sp.slots == 0, a, ss, sp);
+  if (st || (p.bytes == 0 && sp.slots == 0)) return st;
   const int64_t rows = (int64_t)a.total_q * a.heads;
   LR_REQUIRE(rows <= INT32_MAX, "attention_packed: too many rows");
   // a thread takes about eight parts at most: one token against 32768 keys 33.8 us with 256 threads, 30.2 us with 512
   // (64 requests of a few parts each, 139 us, lose 5 us to the larger blocks)
-  const int parts_each = p.slots / a.seqs;
-  const auto join = parts_each > 32 ? join_kernel<D, 1024> : parts_each > 8 ? join_kernel<D, 512> : join_kernel<D, 128>;
+  const int parts_each = p.slots / a.seqs + sp.chunks;
+  const auto join =
+      parts_each > 32 ? join_kernel<D, 1024, SHARED> : parts_each > 8 ? join_kernel<D, 512, SHARED> : join_kernel<D, 128, SHARED>;
   const unsigned threads = parts_each > 32 ? 1024 : parts_each > 8 ? 512 : 128;
-  return launch("attention_packed (join)", join, dim3((unsigned)rows), threads, 0, stream, 1, true, a, ss);
+  return launch(SHARED ? "attention_shared (join)" : "attention_packed (join)", join, dim3((unsigned)rows), threads, 0, stream, 1,
+                true, a, ss, sp);
+}
+
+// How a call behind a prefix is laid out.
+struct SharedPlan {
+  bool parts;       // the prefix in parts, else key tiles in front of every block's own
+  bool step;        // parts by step_kernel, else by prompt_kernel
+  int chunk, chunks;
+  Plan own;         // parts: of the sequences' own keys
+  int64_t prefix_at, own_at, bytes;  // of workspace: the prefix's parts, the parts of sequences that are not split
+};
+SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix, int64_t group, int64_t kv_heads,
+                       int64_t head_dim) {
+  SharedPlan p{};
+  p.own = plan(seqs, total_q, total_k, group, kv_heads, head_dim);
+  p.parts = p.own.step;
+  if (!p.parts) return p;
+  const int64_t rows = total_q * group;
+  p.step = rows <= 16;
+  int64_t want;  // parts
+  if (p.step) {
+    want = (int64_t)sm_count() * 4 / kv_heads;
+    p.chunk = 64;
+  } else {
+    const int64_t head_parts = (group + kRows - 1) / kRows, tile_heads = (group + head_parts - 1) / head_parts;
+    const int64_t tokens = 2 * (kRows / tile_heads);
+    want = sm_count() / ((total_q + tokens - 1) / tokens * kv_heads * head_parts);
+    p.chunk = kKeys;
+  }
+  if (want < 1) want = 1;
+  p.chunk = (int)(((prefix + want - 1) / want + p.chunk - 1) / p.chunk * p.chunk);
+  p.chunks = (int)((prefix + p.chunk - 1) / p.chunk);
+  p.prefix_at = (p.own.bytes + 31) / 32 * 32;
+  const int64_t row_bytes = (head_dim + 2) * 4, all = total_q * group * kv_heads;
+  p.own_at = p.prefix_at + p.chunks * all * row_bytes;
+  p.own_at = (p.own_at + 31) / 32 * 32;
+  p.bytes = p.own_at + (p.step ? all * row_bytes : 0);
+  return p;
+}
+
+template <int D>
+int launch_shared(const Args& a, const SharedPlan& p, StepPrefix sp, void* workspace, cudaStream_t stream) {
+  if (!p.parts) return launch_prompt<D, kWithPrefix>(a, sp, sm_count(), stream);
+  const int64_t all = (int64_t)a.total_q * a.heads;
+  sp.chunk = p.chunk, sp.chunks = p.chunks, sp.slots = p.step ? p.chunks : 0;
+  sp.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.prefix_at);
+  sp.part_ml = reinterpret_cast<float2*>(sp.part_o + p.chunks * all * D);
+  sp.own_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.own_at);
+  sp.own_ml = reinterpret_cast<float2*>(sp.own_o + all * D);
+  if (!p.step) {
+    const int st = launch_prompt<D, kPrefixPart>(a, sp, sm_count(), stream);
+    if (st) return st;
+  }
+  return launch_step<D, true>(a, p.own, sp, workspace, stream);
 }
 
 }  // namespace
@@ -1142,7 +1355,62 @@ extern "C" int lr_attention_packed(const void* q, int64_t q_token_stride, int64_
                        (int)seqs, (int)total_q, (int)total_k, (int)heads, (int)kv_heads, (int)group, causal,
                        (float)((double)scale * 1.4426950408889634)};
   auto* s = static_cast<cudaStream_t>(stream);
+  const packed::StepPrefix none{};
   if (p.step)
-    return head_dim == 64 ? packed::launch_step<64>(a, p, workspace, s) : packed::launch_step<128>(a, p, workspace, s);
-  return head_dim == 64 ? packed::launch_prompt<64>(a, s) : packed::launch_prompt<128>(a, s);
+    return head_dim == 64 ? packed::launch_step<64, false>(a, p, none, workspace, s)
+                          : packed::launch_step<128, false>(a, p, none, workspace, s);
+  return head_dim == 64 ? packed::launch_prompt<64, packed::kNoPrefix>(a, none, sm_count(), s)
+                        : packed::launch_prompt<128, packed::kNoPrefix>(a, none, sm_count(), s);
+}
+
+static int check_shared(int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix, int64_t heads, int64_t kv_heads,
+                        int64_t head_dim) {
+  const int st = check_packed(seqs, total_q, total_k, heads, kv_heads, head_dim);
+  if (st) return st;
+  LR_REQUIRE(prefix > 0 && prefix < (1 << 30), "attention_shared: prefix of %lld keys", (long long)prefix);
+  return LR_OK;
+}
+
+extern "C" int64_t lr_attention_shared_workspace_bytes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix,
+                                                       int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  if (check_shared(seqs, total_q, total_k, prefix, heads, kv_heads, head_dim) || total_q == 0) return 0;
+  return lr::packed::shared_plan(seqs, total_q, total_k, prefix, heads / kv_heads, kv_heads, head_dim).bytes;
+}
+
+extern "C" int lr_attention_shared(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                   int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                   int64_t v_head_stride, const void* prefix_k, int64_t pk_token_stride, int64_t pk_head_stride,
+                                   const void* prefix_v, int64_t pv_token_stride, int64_t pv_head_stride, const int32_t* cu_q,
+                                   const int32_t* cu_k, int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix,
+                                   int64_t heads, int64_t kv_heads, int64_t head_dim, int causal, float scale, void* out,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace lr;
+  const int st = check_shared(seqs, total_q, total_k, prefix, heads, kv_heads, head_dim);
+  if (st) return st;
+  if (total_q == 0) return LR_OK;
+  LR_REQUIRE(q && out && cu_q && cu_k && prefix_k && prefix_v && (total_k == 0 || (k && v)), "attention_shared: null pointer");
+  const int64_t strides[] = {q_token_stride,  q_head_stride,   k_token_stride,  k_head_stride,   v_token_stride,
+                             v_head_stride,   pk_token_stride, pk_head_stride,  pv_token_stride, pv_head_stride};
+  for (const int64_t s : strides) {
+    LR_REQUIRE(s >= 0, "attention_shared: negative strides");
+    if (s % 8) return set_error(LR_ERR_UNSUPPORTED, "attention_shared: strides must be multiples of 16 bytes");
+  }
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(prefix_k, 16) || !aligned(prefix_v, 16) ||
+      !aligned(out, 16))
+    return set_error(LR_ERR_UNSUPPORTED, "attention_shared: pointers must be 16-byte aligned");
+  const int64_t group = heads / kv_heads;
+  const packed::SharedPlan p = packed::shared_plan(seqs, total_q, total_k, prefix, group, kv_heads, head_dim);
+  LR_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 32)),
+             "attention_shared: a workspace of %lld bytes is needed", (long long)p.bytes);
+  const packed::Args a{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
+                       static_cast<const __nv_bfloat16*>(v), static_cast<__nv_bfloat16*>(out), q_token_stride,
+                       q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_q, cu_k,
+                       (int)seqs, (int)total_q, (int)total_k, (int)heads, (int)kv_heads, (int)group, causal,
+                       (float)((double)scale * 1.4426950408889634)};
+  packed::StepPrefix sp{};
+  sp.k = static_cast<const __nv_bfloat16*>(prefix_k), sp.v = static_cast<const __nv_bfloat16*>(prefix_v);
+  sp.k_ts = pk_token_stride, sp.k_hs = pk_head_stride, sp.v_ts = pv_token_stride, sp.v_hs = pv_head_stride;
+  sp.keys = (int)prefix;
+  auto* s = static_cast<cudaStream_t>(stream);
+  return head_dim == 64 ? packed::launch_shared<64>(a, p, sp, workspace, s) : packed::launch_shared<128>(a, p, sp, workspace, s);
 }
