@@ -91,7 +91,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     if base.stride(1) != 1 or base.stride(0) < 0:
         base = base.contiguous()
     x_stride = x.stride(0)
-    if x.stride(1) != 1 or x_stride % 8 or x.data_ptr() % 16:
+    if x.stride(1) != 1 or x_stride % 8 or x_stride < width or x.data_ptr() % 16:
         x, x_stride = x.clone(memory_format=torch.contiguous_format), width
     need = _workspace_bytes(down.get_device(), tokens, width, outputs, rank, count) if down.is_cuda else 0
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None

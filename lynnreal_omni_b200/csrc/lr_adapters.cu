@@ -2,18 +2,20 @@
 //   out[t, :] = base[t, :] + scale[e] * up[e] (down[e] x[t, :]),  e = index[t]
 // (e < 0: out[t, :] = base[t, :]), where base is the shared projection's output.
 //
-// Two kernels: shrink_kernel makes the few values down[e] x[t] of every token
-// (fp32, in parts over the columns), expand_kernel adds up[e] times them to the
-// base row. Both are bound by memory: per byte of x or base a rank of 16 to 128
-// gives the tensor core 8 to 64 products, so mma.sync is fast enough, and its
-// operands come straight from global memory, 16 bytes a load: a sum over columns
-// does not mind their order, and neither do the outputs of a tile, so what a
-// thread loads at once are the columns that it stands for. Nothing but the small
-// inner rows passes through shared memory.
+// Two kernels: shrink_kernel makes the few values scale[e] down[e] x[t] of every
+// token, the expand kernels add up[e] times them to the base row. Both are bound
+// by memory: per byte of x or base a rank of 16 to 128 gives the tensor core 8 to
+// 64 products, so mma.sync is fast enough, and its operands come straight from
+// global memory, 16 bytes a load: a sum over columns does not mind their order,
+// and neither do the outputs of a tile, so what a thread loads at once are the
+// columns that it stands for.
 //
-// Tokens are taken in tiles, whatever their adapters: for each adapter that
-// occurs in a tile the rows of the others are zeros, and their sums are put back
-// afterwards (an infinity in one request's row or adapter reaches no other).
+// Up to kFew tokens, where one token a request is usual, a block stands for one
+// adapter and lists its tokens first, so that every adapter in use is read about
+// once whatever the order. More tokens are taken in tiles of neighbours: for each
+// adapter that occurs in a tile the rows of the others are zeros, and their sums
+// are put back afterwards. Either way an infinity in one request's row or adapter
+// reaches no other.
 #include "lr_common.cuh"
 #include "lr_host.h"
 #include "lr_tc.cuh"
@@ -31,43 +33,94 @@ struct Args {
   const bf16 *x, *base, *down, *up;
   const float* scale;
   const int32_t* index;
-  bf16* out;
+  bf16 *out, *inner;  // inner: [tokens][padded]
   int64_t x_stride, base_stride, out_stride;
   int tokens, width, outputs, rank, count;
-  int splits;    // parts of the columns
-  int padded;    // columns of an inner row
-  float* inner;  // [splits][tokens][padded]
+  int padded;  // columns of an inner row
+  int groups;  // up to kFew tokens: blocks that stand for adapters
 };
 
 constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kFew = 2 * kThreads;
 
-// The adapters of a tile of up to 64 tokens, one after another, in every warp alike.
-struct Groups {
-  int id[2];  // of tokens lane and lane + 32; -1: none, or had already
-  uint64_t none;
+__device__ __forceinline__ bool adapter_of(const Args& a, int id) { return id >= 0 && id < a.count; }
 
-  __device__ __forceinline__ Groups(const Args& a, int first, int tile, int lane) {
-    bool bad = false;
+// The tokens of one block's adapter, in order (up to kFew tokens). With no more
+// adapters than tokens group z is adapter z, else the one of token z if that is
+// its first token. Group a.groups is the tokens without one. Whole block; the
+// count, and the adapter (-1: none).
+struct List {
+  uint16_t token[kFew];
+  int counts[kFew / 32];
+};
+__device__ __forceinline__ int list_tokens(const Args& a, List& list, int group, int& adapter) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  adapter = group == a.groups ? -1 : a.count <= a.tokens ? group : a.index[group];
+  if (group < a.groups && !adapter_of(a, adapter)) return 0;
+  unsigned mine[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = lane + 32 * i;
-      id[i] = at < tile && first + at < a.tokens ? a.index[first + at] : -1;
-      bad |= id[i] >= a.count;
-      if (id[i] >= a.count) id[i] = -1;
+  for (int i = 0; i < 2; ++i) {
+    const int at = i * kThreads + threadIdx.x;
+    const int id = at < a.tokens ? a.index[at] : -1;
+    const bool there = adapter_of(a, id);
+    if (group == a.groups && id >= a.count) atomicOr(&g_adapters_status, (unsigned)kDevErrAdapter);
+    mine[i] = __ballot_sync(0xffffffffu, at < a.tokens && (adapter < 0 ? !there : id == adapter));
+    if (lane == 0) list.counts[i * kWarps + warp] = __popc(mine[i]);
+  }
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int before = total;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = list.counts[i * kWarps + w];
+      before += w < warp ? n : 0;
+      total += n;
     }
-    if (bad) atomicOr(&g_adapters_status, (unsigned)kDevErrAdapter);
-    none = ~((uint64_t)__ballot_sync(0xffffffffu, id[0] >= 0) | (uint64_t)__ballot_sync(0xffffffffu, id[1] >= 0) << 32);
+    if (mine[i] >> lane & 1) list.token[before + __popc(mine[i] & ((1u << lane) - 1))] = (uint16_t)(i * kThreads + threadIdx.x);
+  }
+  __syncthreads();
+  if (group < a.groups && a.count > a.tokens && list.token[0] != group) total = 0;
+  return total;
+}
+
+// The adapters of a tile of 32 W neighbours, one after another, in every warp alike.
+template <int W>
+struct Groups {
+  int id[W];  // of tokens lane + 32 i; -1: none, or had already
+
+  __device__ __forceinline__ void load(const Args& a, int first, int lane) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) id[i] = first + lane + 32 * i < a.tokens ? a.index[first + lane + 32 * i] : -1;
+  }
+  // Numbers past the last adapter become none.
+  __device__ __forceinline__ void check(const Args& a) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (id[i] >= a.count) {
+        atomicOr(&g_adapters_status, (unsigned)kDevErrAdapter);
+        id[i] = -1;
+      }
   }
   // The next adapter and the tokens that have it; false at the end.
-  __device__ __forceinline__ bool next(int& adapter, uint64_t& members) {
-    const unsigned b0 = __ballot_sync(0xffffffffu, id[0] >= 0), b1 = __ballot_sync(0xffffffffu, id[1] >= 0);
-    if ((b0 | b1) == 0u) return false;
-    adapter = b0 ? __shfl_sync(0xffffffffu, id[0], __ffs(b0) - 1) : __shfl_sync(0xffffffffu, id[1], __ffs(b1) - 1);
-    members = (uint64_t)__ballot_sync(0xffffffffu, id[0] == adapter) |
-              (uint64_t)__ballot_sync(0xffffffffu, id[1] == adapter) << 32;
+  __device__ __forceinline__ bool next(int& adapter, uint32_t (&members)[W]) {
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = W - 1; i >= 0; --i) {
+      const unsigned left = __ballot_sync(0xffffffffu, id[i] >= 0);
+      if (left) {
+        any = true;
+        adapter = __shfl_sync(0xffffffffu, id[i], __ffs(left) - 1);
+      }
+    }
+    if (!any) return false;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      members[i] = __ballot_sync(0xffffffffu, id[i] == adapter);
       if (id[i] == adapter) id[i] = -1;
+    }
     return true;
   }
 };
@@ -82,297 +135,632 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ uint4 load16(const bf16* p, bool there) {
   return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
 }
+__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::map_to_rank(tc::smem_u32(p), rank)) : "memory");
+  return v;
+}
 
 // ------------------------------------------------------------------ shrink
-// MT tiles of 16 tokens, NR tiles of 8 rank rows. The warps of a block, and the
-// blocks of a tile (blockIdx.y), each take a run of columns; the warps' sums are
-// added in a fixed order, the blocks' by expand_kernel. Blocks of blockIdx.z take
-// every gridDim.z-th adapter of the tile.
-template <int MT, int NR>
-__global__ void __launch_bounds__(32 * kWarps) shrink_kernel(const Args a) {
-  constexpr int kRegs = MT * NR * 4;
-  extern __shared__ float sums[];  // [kWarps / 2][kRegs][32]
+// Few tokens. NR tiles of 8 rank rows. The warps of the blocks of a cluster
+// (gridDim.x blocks) take every gridDim.x * kWarps-th 32 columns; their sums are
+// added in a fixed order through shared memory, scaled and rounded to bf16 for the
+// second product (2^-9 of the update, as every factor of it is rounded already).
+template <int NR>
+__global__ void __launch_bounds__(kThreads, 2) shrink_few_kernel(const Args a) {
+  constexpr int kTile = 16 * 8 * NR;
+  constexpr int kAhead = NR <= 2 ? 4 : NR <= 4 ? 2 : 1;  // steps whose loads are under way together
+  extern __shared__ float sums[];                         // [kWarps][kTile], then the block's [kTile]
+  __shared__ List list;
+  float* block_sums = sums + kWarps * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int first = blockIdx.x * (16 * MT);
+  const int part = blockIdx.x, parts = gridDim.x;
   tc::allow_dependent();
-  Groups groups(a, first, 16 * MT, lane);
-  const int steps = (a.width + 31) / 32;
-  const int each = (steps + kWarps * a.splits - 1) / (kWarps * a.splits);
-  const int k0 = min((int)(blockIdx.y * kWarps + warp) * each, steps) * 32, k1 = min(k0 + each * 32, a.width);
-
   int adapter;
-  uint64_t members;
-  for (int number = 0; groups.next(adapter, members); ++number) {
-    if (number % gridDim.z != blockIdx.z) continue;
-    float acc[MT][NR][4];
+  const int count = list_tokens(a, list, blockIdx.y, adapter);
+  for (int first = blockIdx.z * 16; first < count; first += gridDim.z * 16) {
+    float acc[NR][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < NR * 4; ++i) acc[i / 4][i % 4] = 0.0f;
+    const bf16* down = a.down + ((int64_t)adapter * a.rank + g) * a.width;
+    const bool lo = first + g < count, hi = first + 8 + g < count;
+    const bf16* r0 = a.x + (int64_t)list.token[lo ? first + g : first] * a.x_stride;
+    const bf16* r1 = a.x + (int64_t)list.token[hi ? first + 8 + g : first] * a.x_stride;
+#pragma unroll kAhead
+    for (int k0 = (part * kWarps + warp) * 32; k0 < a.width; k0 += parts * kWarps * 32) {
+      const int k = k0 + 8 * t;
+      const bool there = k < a.width;
+      uint4 w[NR];
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
+      for (int n = 0; n < NR; ++n) w[n] = load16(down + (int64_t)(8 * n) * a.width + k, there && 8 * n + g < a.rank);
+      const uint4 x0 = load16(r0 + k, there && lo), x1 = load16(r1 + k, there && hi);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
-    const bf16* down = a.down + (int64_t)adapter * a.rank * a.width;
-#pragma unroll 2
-    for (int k = k0 + 8 * t; k < k1 + 8 * t; k += 32) {
-      const bool there = k < k1;
-      uint4 w[NR], x[MT][2];
-#pragma unroll
-      for (int n = 0; n < NR; ++n) w[n] = load16(down + (int64_t)(8 * n + g) * a.width + k, there && 8 * n + g < a.rank);
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = 16 * m + 8 * h + g;
-          x[m][h] = load16(a.x + (int64_t)(first + row) * a.x_stride + k, there && (members >> row & 1));
-        }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          mma_16816(acc[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, w[n].x, w[n].y);
-          mma_16816(acc[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, w[n].z, w[n].w);
-        }
-    }
-#pragma unroll
-    for (int half = kWarps / 2; half >= 1; half /= 2) {
-      __syncthreads();
-      if (warp >= half && warp < 2 * half) {
-        float* dst = sums + (warp - half) * kRegs * 32 + lane;
-#pragma unroll
-        for (int i = 0; i < kRegs; ++i) dst[i * 32] = acc[i / (NR * 4)][i / 4 % NR][i % 4];
-      }
-      __syncthreads();
-      if (warp < half) {
-        const float* src = sums + warp * kRegs * 32 + lane;
-#pragma unroll
-        for (int i = 0; i < kRegs; ++i) acc[i / (NR * 4)][i / 4 % NR][i % 4] += src[i * 32];
+      for (int n = 0; n < NR; ++n) {
+        mma_16816(acc[n], x0.x, x1.x, x0.y, x1.y, w[n].x, w[n].y);
+        mma_16816(acc[n], x0.z, x1.z, x0.w, x1.w, w[n].z, w[n].w);
       }
     }
+    // [register][lane] of each warp: no two lanes in one bank
+#pragma unroll
+    for (int i = 0; i < NR * 4; ++i) sums[warp * kTile + i * 32 + lane] = acc[i / 4][i % 4];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTile; i += kThreads) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) v += sums[w * kTile + i];
+      block_sums[i] = v;
+    }
+    if (parts > 1) tc::cluster_sync_all(); else __syncthreads();
+    const float scale = a.scale ? a.scale[adapter] : 1.0f;
+    for (int i = part * kThreads + threadIdx.x; i < kTile / 2; i += parts * kThreads) {
+      // two columns side by side: registers 2 e, 2 e + 1 of a lane
+      const int l = i % 32, e = i / 32 % 2, n = i / 64;
+      const int at = (n * 4 + 2 * e) * 32 + l, r = first + 8 * e + l / 4;
+      if (r >= count) continue;
+      float v0 = 0.0f, v1 = 0.0f;
+      if (parts > 1) {
+        for (int p = 0; p < parts; ++p) {
+          v0 += cluster_load(block_sums + at, p);
+          v1 += cluster_load(block_sums + at + 32, p);
+        }
+      } else {
+        v0 = block_sums[at], v1 = block_sums[at + 32];
+      }
+      *reinterpret_cast<uint32_t*>(a.inner + (int64_t)list.token[r] * a.padded + 8 * n + 2 * (l % 4)) = cvt2(v0 * scale, v1 * scale);
+    }
+    if (parts > 1) tc::cluster_sync_all(); else __syncthreads();
+  }
+}
+
+// Many tokens: 128 neighbours against an adapter's N rank rows (padded with zeros)
+// on the tensor core, 64 columns of both a stage. The cluster's blocks take every
+// gridDim.x-th 64 columns and add their sums in order through shared memory. For
+// each adapter that occurs among the tokens the rows pass through again.
+constexpr int kShrinkRows = 128;
+template <int N>
+struct Shrink {
+  static constexpr int kX = kShrinkRows * 128, kStage = kX + N * 128;
+  static constexpr int kStages = N <= 32 ? 4 : 3;
+  static constexpr int kSums = kStages * kStage;             // fp32 [N][kShrinkRows]
+  static constexpr int kBars = kSums + N * kShrinkRows * 4;  // full, empty, done; TMEM address, abort flag
+  static constexpr size_t kSmem = 1024 + kBars + (2 * kStages + 1) * 8 + 8;
+  static constexpr uint32_t kColumns = N < 32 ? 32 : N;
+  // kind::f16: fp32 accumulator, bf16 operands, N / 8 at 17, M / 16 at 24
+  static constexpr uint32_t kDesc =
+      (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N / 8) << 17) | ((uint32_t)(kShrinkRows / 16) << 24);
+};
+constexpr int kShrinkThreads = 192;
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+      : "memory");
+}
+
+// Warp 0 copies, warp 1 issues the products, warps 2-5 take the sums.
+template <int N>
+__global__ void __launch_bounds__(kShrinkThreads)
+    shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_down, const Args a) {
+  using C = Shrink<N>;
+  using namespace tc;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* sums = reinterpret_cast<float*>(smem + C::kSums);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint64_t *empty = full + C::kStages, *done = empty + C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const Watch watch{tmem_slot + 1, &g_adapters_status};
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int part = blockIdx.x, parts = gridDim.x, first = blockIdx.y * kShrinkRows;
+  allow_dependent();
+  if (threadIdx.x == 0) {
+    prefetch_map(&map_x);
+    prefetch_map(&map_down);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(done), 1);
+    *watch.abort_flag = 0u;
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc<1>(smem_u32(tmem_slot), C::kColumns);
+  Groups<4> groups;
+  groups.load(a, first, lane);
+  groups.check(a);
+  const int row = ((warp & 3) * 32) + lane;  // of the sums' warps
+  const int mine = warp >= 2 && first + row < a.tokens ? a.index[first + row] : -1;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(*tmem_slot);
+
+  const int steps = (a.width + 63) / 64;
+  const bool el = elect_one();
+  bool ok = true;
+  uint32_t stage = 0;  // of the ring, over all adapters
+  int adapter;
+  uint32_t members[4];
+  for (uint32_t number = 0; groups.next(adapter, members); ++number) {
+    adapter = uniform(adapter);
     if (warp == 0) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = 16 * m + 8 * h + g;
-          if (!(members >> row & 1)) continue;
-          float* dst = a.inner + ((int64_t)blockIdx.y * a.tokens + first + row) * a.padded + 2 * t;
-#pragma unroll
-          for (int n = 0; n < NR; ++n)
-            if (8 * n < a.padded) *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+      for (int step = part; step < steps && ok; step += parts, ++stage) {
+        const uint32_t s = stage % C::kStages;
+        ok = warp_wait(smem_u32(&empty[s]), ((stage / C::kStages) & 1u) ^ 1u, watch, lane);
+        if (el && ok) {
+          const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + s * C::kStage);
+          mbar_expect_tx(bar, C::kStage);
+          tma_load_2d(dst, &map_x, bar, step * 64, first);
+          tma_load_3d(dst + C::kX, &map_down, bar, step * 64, 0, adapter);
         }
+        __syncwarp();
+      }
+    } else if (warp == 1) {
+      for (int step = part; step < steps && ok; step += parts, ++stage) {
+        const uint32_t s = stage % C::kStages;
+        ok = warp_wait(smem_u32(&full[s]), (stage / C::kStages) & 1u, watch, lane);
+        tc_fence_after();
+        if (el && ok) {
+          const uint32_t x = smem_u32(smem + s * C::kStage), w = x + C::kX;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(tmem, desc_kmajor(x + kk * 32), desc_kmajor(w + kk * 32), C::kDesc, step != part || kk != 0 ? 1u : 0u);
+          mma_commit(smem_u32(&empty[s]));
+        }
+        __syncwarp();
+      }
+      if (el) mma_commit(smem_u32(done));
+      __syncwarp();
+    } else {
+      ok = ok && warp_wait(smem_u32(done), number & 1u, watch, lane);
+      tc_fence_after();
+      const float scale = a.scale ? a.scale[adapter] : 1.0f;
+      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      bf16* dst = a.inner + (int64_t)(first + row) * a.padded;
+#pragma unroll
+      for (int c = 0; c < N; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(lanes + c, v);
+        if (parts > 1) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sums[(c + i) * kShrinkRows + row] = __uint_as_float(v[i]);
+        } else if (ok && mine == adapter) {
+          uint32_t y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = cvt2(__uint_as_float(v[2 * i]) * scale, __uint_as_float(v[2 * i + 1]) * scale);
+          *reinterpret_cast<uint4*>(dst + c) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+      }
+      tc_fence_before();
     }
+    if (parts > 1) {
+      __syncwarp();
+      cluster_sync_all();
+      // this block's share of the columns, eight at a time
+      if (warp >= 2 && mine == adapter) {
+        const float scale = a.scale ? a.scale[adapter] : 1.0f;
+        for (int c = part * 8; c < N; c += parts * 8) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+          for (int p = 0; p < parts; ++p)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += cluster_load(sums + (c + i) * kShrinkRows + row, p);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= scale;
+          *reinterpret_cast<uint4*>(a.inner + (int64_t)(first + row) * a.padded + c) = pack8(v);
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();
+    } else {
+      __syncwarp();
+      __syncthreads();
+    }
+    tc_fence_after();
+  }
+  if (!ok) {  // giving up: time for the copies in flight to land before the block can exit
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 100000ull) {
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, C::kColumns);
   }
 }
 
 // ------------------------------------------------------------------ expand
-// MT tiles of 16 tokens, 32 columns a warp, rank up to 16 KS. The base values
-// are the products' accumulators. A thread's eight columns lie side by side:
-// column n of the tile's i-th product stands for column 8 (n / 2) + 2 i + n % 2.
-// The inner values, scaled, are rounded to bf16 for the product (2^-9 of the
-// update, as every factor of it is rounded already); sums and base stay in fp32
-// and are rounded once.
-template <int MT, int KS, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps) expand_kernel(const Args a) {
-  constexpr int kPad = KS > 1 ? 16 * KS : 16;
-  constexpr int kLine = kPad >= 64 ? kPad + 32 : kPad;  // rows side by side in different banks
-  __shared__ __align__(16) bf16 inner[16 * MT * kLine];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int column_blocks = (a.outputs + 32 * kWarps - 1) / (32 * kWarps);
-  const int first = (int)(blockIdx.x / column_blocks) * (16 * MT);
-  const int column = (int)(blockIdx.x % column_blocks) * (32 * kWarps) + warp * 32;
-  Groups groups(a, first, 16 * MT, lane);
-
-  // The rows of this block: those of its adapters, and, in the first one, those of none.
-  uint64_t owned = blockIdx.z == 0 ? groups.none : 0;
-  {
-    Groups all = groups;
-    int adapter;
-    uint64_t members;
-    for (int number = 0; all.next(adapter, members); ++number)
-      if (number % gridDim.z == blockIdx.z) owned |= members;
-  }
-  const int rows = min(16 * MT, a.tokens - first);
-  if (rows < 64) owned &= (1ull << rows) - 1;
-  if (owned == 0) {  // the same in every thread
-    tc::wait_for_predecessor();
-    return;
-  }
-  const int mine = column + 8 * t;
-  float acc[MT][4][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = 16 * m + 8 * h + g;
-      const bf16* src = a.base + (int64_t)(first + row) * a.base_stride + mine;
-      uint32_t y[4] = {0u, 0u, 0u, 0u};
-      if (owned >> row & 1) {
-        if (VEC) {
-          if (mine < a.outputs) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-          }
-        } else {
-          const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (mine + i < a.outputs) y[i / 2] |= (uint32_t)s[i] << (16 * (i % 2));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[m][i][2 * h] = bf_lo(y[i]);
-        acc[m][i][2 * h + 1] = bf_hi(y[i]);
-      }
-    }
-  bool waited = false;
-  int adapter;
-  uint64_t members;
-  for (int number = 0; groups.next(adapter, members); ++number) {
-    if (number % gridDim.z != blockIdx.z) continue;
-    uint32_t up[4][KS][2];
-    const bf16* weight = a.up + (int64_t)adapter * a.outputs * a.rank;
+// 32 columns a warp, rank up to 16 KS. The base values are the products'
+// accumulators: sums stay in fp32 and are rounded once. A thread's eight columns
+// lie side by side: column n of the i-th product stands for column
+// 8 (n / 2) + 2 i + n % 2 of the 32.
+template <int KS>
+struct Up {
+  uint32_t w[4][KS][2];
+  __device__ __forceinline__ void load(const Args& a, int adapter, int column, int g, int t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = column + 8 * (g >> 1) + 2 * i + (g & 1);
-      const bf16* src = weight + (int64_t)n * a.rank;
-      if (KS == 1) {
-        const uint2 w = n < a.outputs && 4 * t < a.rank ? *reinterpret_cast<const uint2*>(src + 4 * t) : make_uint2(0u, 0u);
-        up[i][0][0] = w.x, up[i][0][1] = w.y;
+      const bf16* src = a.up + ((int64_t)adapter * a.outputs + n) * a.rank;
+      if constexpr (KS == 1) {
+        const uint2 v = n < a.outputs && 4 * t < a.rank ? *reinterpret_cast<const uint2*>(src + 4 * t) : make_uint2(0u, 0u);
+        w[i][0][0] = v.x, w[i][0][1] = v.y;
       } else {
 #pragma unroll
-        for (int s = 0; s < KS / 2; ++s) {
-          const uint4 w = load16(src + 32 * s + 8 * t, n < a.outputs && 32 * s + 8 * t < a.rank);
-          up[i][2 * s][0] = w.x, up[i][2 * s][1] = w.y;
-          up[i][(2 * s + 1) % KS][0] = w.z, up[i][(2 * s + 1) % KS][1] = w.w;
+        for (int s = 0; s < KS; s += 2) {
+          const uint4 v = load16(src + 16 * s + 8 * t, n < a.outputs && 16 * s + 8 * t < a.rank);
+          w[i][s][0] = v.x, w[i][s][1] = v.y;
+          w[i][s + 1][0] = v.z, w[i][s + 1][1] = v.w;
         }
       }
     }
-    if (!waited) {
-      waited = true;
-      tc::wait_for_predecessor();
-      // The inner rows: parts added in order, scaled.
-      for (int at = threadIdx.x; at < 16 * MT * (kPad / 4); at += 32 * kWarps) {
-        const int row = at / (kPad / 4), c = at % (kPad / 4) * 4;
-        const int token = first + row;
-        uint2 packed = make_uint2(0u, 0u);
-        int e = token < a.tokens ? a.index[token] : -1;
-        if (e >= 0 && e < a.count && (owned >> row & 1) && c < a.rank) {
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const float* src = a.inner + (int64_t)token * a.padded + c;
-          for (int s = 0; s < a.splits; ++s, src += (int64_t)a.tokens * a.padded) {
-            const float4 part = __ldcg(reinterpret_cast<const float4*>(src));
-            v[0] += part.x, v[1] += part.y, v[2] += part.z, v[3] += part.w;
-          }
-          const float scale = a.scale ? a.scale[e] : 1.0f;
-          packed = make_uint2(cvt2(v[0] * scale, v[1] * scale), cvt2(v[2] * scale, v[3] * scale));
-        }
-        *reinterpret_cast<uint2*>(inner + row * kLine + c) = packed;
+  }
+};
+// acc += inner rows r0 (rows g) and r1 (rows g + 8), where they are to be read, times the weights.
+template <int KS>
+__device__ __forceinline__ void add_update(float (&acc)[4][4], const Up<KS>& up, const bf16* r0, bool lo, const bf16* r1, bool hi,
+                                           int t) {
+  if constexpr (KS == 1) {
+    const uint2 h0 = lo ? *reinterpret_cast<const uint2*>(r0 + 4 * t) : make_uint2(0u, 0u);
+    const uint2 h1 = hi ? *reinterpret_cast<const uint2*>(r1 + 4 * t) : make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mma_16816(acc[i], h0.x, h1.x, h0.y, h1.y, up.w[i][0][0], up.w[i][0][1]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < KS; s += 2) {
+      const uint4 h0 = load16(r0 + 16 * s + 8 * t, lo), h1 = load16(r1 + 16 * s + 8 * t, hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mma_16816(acc[i], h0.x, h1.x, h0.y, h1.y, up.w[i][s][0], up.w[i][s][1]);
+        mma_16816(acc[i], h0.z, h1.z, h0.w, h1.w, up.w[i][s + 1][0], up.w[i][s + 1][1]);
       }
-      __syncthreads();
+    }
+  }
+}
+// Eight neighbouring columns of a row, as far as there are any.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_row(const bf16* p, int columns, bool there) {
+  if (VEC) return load16(p, there && columns > 0);
+  uint32_t y[4] = {0u, 0u, 0u, 0u};
+  if (there) {
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < columns) y[i / 2] |= (uint32_t)s[i] << (16 * (i % 2));
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void store_row(bf16* p, const float (&acc)[4][4], int h, int columns) {
+  if (VEC) {
+    if (columns > 0)
+      *reinterpret_cast<uint4*>(p) = make_uint4(cvt2(acc[0][2 * h], acc[0][2 * h + 1]), cvt2(acc[1][2 * h], acc[1][2 * h + 1]),
+                                                cvt2(acc[2][2 * h], acc[2][2 * h + 1]), cvt2(acc[3][2 * h], acc[3][2 * h + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < columns) p[i] = __float2bfloat16_rn(acc[i / 2][2 * h + i % 2]);
+  }
+}
+__device__ __forceinline__ void unpack_row(float (&acc)[4][4], int h, const uint4& y) {
+  const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc[i][2 * h] = bf_lo(w[i]);
+    acc[i][2 * h + 1] = bf_hi(w[i]);
+  }
+}
+
+// Few tokens: a block stands for one adapter and STRIPS times 256 columns. The
+// weights and the base rows are under way before the inner rows are there.
+template <int KS, int STRIPS, bool VEC>
+__global__ void __launch_bounds__(kThreads) expand_few_kernel(const Args a) {
+  __shared__ List list;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int column = blockIdx.x * (STRIPS * kThreads) + warp * 32;
+  int adapter;
+  const int n = list_tokens(a, list, blockIdx.y, adapter);
+  if ((int)blockIdx.z * 16 >= n || (adapter < 0 && a.out == a.base && a.out_stride == a.base_stride)) {
+    tc::wait_for_predecessor();
+    return;
+  }
+  Up<KS> up[STRIPS];
+  if (adapter >= 0) {
+#pragma unroll
+    for (int s = 0; s < STRIPS; ++s) up[s].load(a, adapter, column + s * kThreads, g, t);
+  }
+  for (int first = blockIdx.z * 16; first < n; first += gridDim.z * 16) {
+    const bool lo = first + g < n, hi = first + 8 + g < n;
+    const int64_t t0 = list.token[lo ? first + g : first], t1 = list.token[hi ? first + 8 + g : first];
+    float acc[STRIPS][4][4];
+#pragma unroll
+    for (int s = 0; s < STRIPS; ++s) {
+      const int mine = column + s * kThreads + 8 * t;
+      unpack_row(acc[s], 0, load_row<VEC>(a.base + t0 * a.base_stride + mine, a.outputs - mine, lo));
+      unpack_row(acc[s], 1, load_row<VEC>(a.base + t1 * a.base_stride + mine, a.outputs - mine, hi));
+    }
+    if (first == (int)blockIdx.z * 16) tc::wait_for_predecessor();
+    if (adapter >= 0) {
+#pragma unroll
+      for (int s = 0; s < STRIPS; ++s)
+        add_update<KS>(acc[s], up[s], a.inner + t0 * a.padded, lo, a.inner + t1 * a.padded, hi, t);
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (!(members >> (16 * m) & 0xffff)) continue;
-      float before[4][4];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) before[i / 4][i % 4] = acc[m][i / 4][i % 4];
-      const bool lo = members >> (16 * m + g) & 1, hi = members >> (16 * m + 8 + g) & 1;
-      const bf16 *r0 = inner + (16 * m + g) * kLine, *r1 = r0 + 8 * kLine;
-      if (KS == 1) {
-        uint2 h0 = *reinterpret_cast<const uint2*>(r0 + 4 * t), h1 = *reinterpret_cast<const uint2*>(r1 + 4 * t);
-        if (!lo) h0 = make_uint2(0u, 0u);
-        if (!hi) h1 = make_uint2(0u, 0u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mma_16816(acc[m][i], h0.x, h1.x, h0.y, h1.y, up[i][0][0], up[i][0][1]);
-      } else {
-#pragma unroll
-        for (int s = 0; s < KS / 2; ++s) {
-          const uint4 h0 = load16(r0 + 32 * s + 8 * t, lo), h1 = load16(r1 + 32 * s + 8 * t, hi);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mma_16816(acc[m][i], h0.x, h1.x, h0.y, h1.y, up[i][2 * s][0], up[i][2 * s][1]);
-            mma_16816(acc[m][i], h0.z, h1.z, h0.w, h1.w, up[i][(2 * s + 1) % KS][0], up[i][(2 * s + 1) % KS][1]);
-          }
+    for (int s = 0; s < STRIPS; ++s) {
+      const int mine = column + s * kThreads + 8 * t;
+      if (lo) store_row<VEC>(a.out + t0 * a.out_stride + mine, acc[s], 0, a.outputs - mine);
+      if (hi) store_row<VEC>(a.out + t1 * a.out_stride + mine, acc[s], 1, a.outputs - mine);
+    }
+  }
+}
+
+// Many tokens: tiles of 64 neighbours by 32 columns a warp, dealt out in runs down
+// the columns, so that a warp keeps its weights while the adapter stays the same.
+// A warp has a ring of tiles of its own in shared memory, which bulk copies fill
+// and empty: nothing but bytes in flight makes this kernel fast. (Base rows through
+// registers, the next tile's on their way meanwhile: 12240 tokens to 24576, rank
+// 32, 400 us, a third of the memory's rate.) Rows in shared memory are 64 bytes
+// long and two of them fill the banks.
+constexpr int kExpandRows = 64;
+constexpr int kExpandSlots = 3;
+constexpr int kSlotBytes = kExpandRows * 64;
+constexpr size_t kExpandSmem = 128 + kWarps * kExpandSlots * (kSlotBytes + 8) + 8;
+
+// One row's eight columns in a tile.
+__device__ __forceinline__ uint4* tile_at(uint8_t* tile, int row, int t) { return reinterpret_cast<uint4*>(tile + row * 64 + t * 16); }
+
+template <int KS>
+__global__ void __launch_bounds__(kThreads, 2)
+    expand_kernel(const __grid_constant__ CUtensorMap map_base, const __grid_constant__ CUtensorMap map_out, const Args a) {
+  using namespace tc;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * (kExpandSlots * kSlotBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kExpandSlots * kSlotBytes) + warp * kExpandSlots;
+  uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + kWarps * kExpandSlots * (kSlotBytes + 8));
+  const Watch watch{abort_flag, &g_adapters_status};
+  if (lane == 0) {
+    for (int s = 0; s < kExpandSlots; ++s) mbar_init(smem_u32(&full[s]), 1);
+    if (warp == 0) {
+      *abort_flag = 0u;
+      prefetch_map(&map_base);
+      prefetch_map(&map_out);
+    }
+    mbar_init_fence();
+  }
+  __syncthreads();
+  const bool el = elect_one();
+  const int tiles = (a.tokens + kExpandRows - 1) / kExpandRows;
+  const int64_t items = (int64_t)tiles * ((a.outputs + kThreads - 1) / kThreads);
+  const int64_t begin = items * blockIdx.x / gridDim.x;
+  const int count = (int)(items * (blockIdx.x + 1) / gridDim.x - begin);
+  // the next tile to be fetched, and the one in hand
+  int fetch_tile = (int)(begin % tiles), fetch_column = (int)(begin / tiles) * kThreads + warp * 32, fetched = 0;
+  int tile = fetch_tile, column = fetch_column;
+  const auto fetch = [&] {
+    if (fetched < count && fetch_column < a.outputs && el) {
+      const uint32_t s = (uint32_t)fetched % kExpandSlots, bar = smem_u32(&full[s]);
+      mbar_expect_tx(bar, kSlotBytes);
+      tma_load_2d(smem_u32(ring + s * kSlotBytes), &map_base, bar, fetch_column, fetch_tile * kExpandRows);
+    }
+    ++fetched;
+    if (++fetch_tile == tiles) fetch_tile = 0, fetch_column += kThreads;
+  };
+  for (int s = 0; s < kExpandSlots; ++s) fetch();
+  Groups<2> groups;
+  groups.load(a, tile * kExpandRows, lane);
+  wait_for_predecessor();
+  Up<KS> up;
+  int kept = -1, kept_column = -1;  // whose weights `up` holds
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    const int first = tile * kExpandRows, this_column = column;
+    Groups<2> now = groups;
+    now.check(a);
+    if (++tile == tiles) tile = 0, column += kThreads;
+    if (i + 1 < count) groups.load(a, tile * kExpandRows, lane);
+    const uint32_t s = (uint32_t)i % kExpandSlots;
+    uint8_t* rows = ring + s * kSlotBytes;
+    const bool there = this_column < a.outputs;  // the last columns' warps may have none
+    if (there) {
+      if (!(ok = warp_wait(smem_u32(&full[s]), ((uint32_t)i / kExpandSlots) & 1u, watch, lane))) break;
+      __syncwarp();
+      int adapter;
+      uint32_t members[2];
+      while (now.next(adapter, members)) {
+        if (adapter != kept || this_column != kept_column) {
+          kept = adapter, kept_column = this_column;
+          up.load(a, adapter, this_column, g, t);
         }
+#pragma unroll
+        for (int m = 0; m < kExpandRows / 16; ++m) {
+          const uint32_t here = members[m / 2] >> (16 * (m % 2)) & 0xffffu;
+          if (here == 0u) continue;
+          // rows of other adapters are neither changed nor used
+          const bool lo = here >> g & 1, hi = here >> (8 + g) & 1;
+          const bf16* r = a.inner + (int64_t)(first + 16 * m + g) * a.padded;
+          uint4 *r0 = tile_at(rows, 16 * m + g, t), *r1 = tile_at(rows, 16 * m + 8 + g, t);
+          float acc[4][4];
+          unpack_row(acc, 0, *r0);
+          unpack_row(acc, 1, *r1);
+          add_update<KS>(acc, up, r, lo, r + 8 * a.padded, hi, t);
+          if (lo) *r0 = make_uint4(cvt2(acc[0][0], acc[0][1]), cvt2(acc[1][0], acc[1][1]), cvt2(acc[2][0], acc[2][1]), cvt2(acc[3][0], acc[3][1]));
+          if (hi) *r1 = make_uint4(cvt2(acc[0][2], acc[0][3]), cvt2(acc[1][2], acc[1][3]), cvt2(acc[2][2], acc[2][3]), cvt2(acc[3][2], acc[3][3]));
+        }
+        __syncwarp();
       }
-      // rows of other adapters stay as they were, whatever this one's values
+      fence_async_smem();
+      __syncwarp();
+      if (el) {
+        tma_store_2d(&map_out, smem_u32(rows), this_column, first);
+        bulk_commit();
+      }
+    }
+    // The tile before this one has been stored: its slot takes the next.
+    if (i > 0) {
+      if (el) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      fetch();
+    }
+    __syncwarp();
+  }
+  if (el) bulk_wait_all();
+  if (!ok) {  // giving up: time for the copies in flight to land before the block can exit
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 100000ull) {
+    }
+  }
+}
+
+// The same for rows that bulk copies cannot address (an odd number of columns, other strides): 32 tokens at a time.
+template <int KS>
+__global__ void __launch_bounds__(kThreads) expand_odd_kernel(const Args a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int blocks = (a.outputs + kThreads - 1) / kThreads;
+  const int first = (int)(blockIdx.x / blocks) * 32, column = (int)(blockIdx.x % blocks) * kThreads + warp * 32;
+  const int mine = column + 8 * t;
+  Groups<1> groups;
+  groups.load(a, first, lane);
+  groups.check(a);
+  float acc[2][4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!(e < 2 ? lo : hi)) acc[m][i][e] = before[i][e];
+    for (int h = 0; h < 2; ++h) {
+      const int token = first + 16 * m + 8 * h + g;
+      unpack_row(acc[m], h, load_row<false>(a.base + (int64_t)token * a.base_stride + mine, a.outputs - mine, token < a.tokens));
+    }
+  int adapter;
+  uint32_t members[1];
+  bool waited = false;
+  while (groups.next(adapter, members)) {
+    Up<KS> up;
+    up.load(a, adapter, column, g, t);
+    if (!waited) tc::wait_for_predecessor();
+    waited = true;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const bool lo = members[0] >> (16 * m + g) & 1, hi = members[0] >> (16 * m + 8 + g) & 1;
+      const bf16* r = a.inner + (int64_t)(first + 16 * m + g) * a.padded;
+      float sum[4][4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[i / 4][i % 4] = acc[m][i / 4][i % 4];
+      add_update<KS>(sum, up, r, lo, r + 8 * a.padded, hi, t);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)  // rows of other adapters stay as they were
+        if (i % 4 < 2 ? lo : hi) acc[m][i / 4][i % 4] = sum[i / 4][i % 4];
     }
   }
   if (!waited) tc::wait_for_predecessor();
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = 16 * m + 8 * h + g;
-      if (!(owned >> row & 1)) continue;
-      bf16* dst = a.out + (int64_t)(first + row) * a.out_stride + mine;
-      if (VEC) {
-        if (mine < a.outputs)
-          *reinterpret_cast<uint4*>(dst) =
-              make_uint4(cvt2(acc[m][0][2 * h], acc[m][0][2 * h + 1]), cvt2(acc[m][1][2 * h], acc[m][1][2 * h + 1]),
-                         cvt2(acc[m][2][2 * h], acc[m][2][2 * h + 1]), cvt2(acc[m][3][2 * h], acc[m][3][2 * h + 1]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (mine + i < a.outputs) dst[i] = __float2bfloat16_rn(acc[m][i / 2][2 * h + i % 2]);
-      }
+      const int token = first + 16 * m + 8 * h + g;
+      if (token < a.tokens) store_row<false>(a.out + (int64_t)token * a.out_stride + mine, acc[m], h, a.outputs - mine);
     }
 }
 
 // ------------------------------------------------------------------ host
-struct Plan {
-  bool few;  // tiles of 16 tokens, a block for each adapter of a tile
-  int splits, padded;
-  int64_t bytes;
-};
-Plan plan(int64_t tokens, int64_t width, int64_t rank) {
-  Plan p{};
-  p.few = tokens <= 512;
-  p.padded = (int)((rank + 15) / 16 * 16);
-  const int64_t tiles = p.few ? (tokens + 15) / 16 : (tokens + 63) / 64;
-  int64_t splits = (2 * sm_count() + tiles - 1) / tiles;
-  const int64_t most = (width + 64 * kWarps - 1) / (64 * kWarps);  // two steps a warp at least
-  if (splits > most) splits = most;
-  if (splits > 16) splits = 16;
-  p.splits = (int)splits;
-  p.bytes = splits * tokens * p.padded * 4;
-  return p;
+int padded_rank(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+int64_t workspace_bytes(int64_t tokens, int64_t rank) { return tokens * padded_rank(rank) * 2; }
+
+// Blocks of a cluster that share the columns of `tiles` tiles: as many as give the GPU `blocks`, each at least `columns` wide.
+int column_parts(const Args& a, int64_t tiles, int64_t blocks, int columns) {
+  int parts = 1;
+  while (parts < 8 && 2 * tiles * parts <= blocks && (int64_t)parts * columns < a.width) parts *= 2;
+  return parts;
 }
 
-template <int MT, int NR>
-int launch_shrink(const Args& a, unsigned groups, cudaStream_t stream) {
-  constexpr size_t smem = kWarps / 2 * MT * NR * 4 * 32 * 4;
+template <int NR>
+int launch_shrink_few(const Args& a, int chunks, cudaStream_t stream) {
+  constexpr size_t smem = (kWarps + 1) * 16 * 8 * NR * 4;
   static bool done[64] = {};
-  if (smem > 48 * 1024) {
-    const int st = tc::configure_smem(shrink_kernel<MT, NR>, smem, done);
+  if (smem > 40 * 1024) {
+    const int st = tc::configure_smem(shrink_few_kernel<NR>, smem, done);
     if (st) return st;
   }
-  const dim3 grid((unsigned)((a.tokens + 16 * MT - 1) / (16 * MT)), (unsigned)a.splits, groups);
-  shrink_kernel<MT, NR><<<grid, 32 * kWarps, smem, stream>>>(a);
-  return launch_status("adapters (inner rows)");
+  const int parts = column_parts(a, (int64_t)a.groups * chunks, 2 * sm_count(), 64 * kWarps);
+  const dim3 grid((unsigned)parts, (unsigned)a.groups, (unsigned)chunks);
+  return tc::launch("adapters (inner rows)", shrink_few_kernel<NR>, grid, kThreads, smem, stream, (unsigned)parts, false, a);
 }
 
-template <int MT, int KS>
-int launch_expand(const Args& a, unsigned groups, bool vec, cudaStream_t stream) {
-  const int64_t blocks = (int64_t)((a.tokens + 16 * MT - 1) / (16 * MT)) * ((a.outputs + 32 * kWarps - 1) / (32 * kWarps));
-  LR_REQUIRE(blocks <= INT32_MAX, "adapters: too many blocks");
-  const dim3 grid((unsigned)blocks, 1, groups);
-  return tc::launch("adapters (outputs)", vec ? expand_kernel<MT, KS, true> : expand_kernel<MT, KS, false>, grid, 32 * kWarps, 0,
-                    stream, 1, true, a);
+template <int KS, int STRIPS>
+int launch_expand_few(const Args& a, int chunks, bool vec, cudaStream_t stream) {
+  const dim3 grid((unsigned)((a.outputs + STRIPS * kThreads - 1) / (STRIPS * kThreads)), (unsigned)(a.groups + 1), (unsigned)chunks);
+  return tc::launch("adapters (outputs)", vec ? expand_few_kernel<KS, STRIPS, true> : expand_few_kernel<KS, STRIPS, false>, grid,
+                    kThreads, 0, stream, 1, true, a);
 }
 
-template <int MT_SHRINK, int NR, int MT_EXPAND>
-int launch_both(const Args& a, unsigned groups, bool vec, cudaStream_t stream) {
-  const int st = launch_shrink<MT_SHRINK, NR>(a, groups, stream);
-  return st ? st : launch_expand<MT_EXPAND, (NR + 1) / 2>(a, groups, vec, stream);
+template <int N>
+int launch_shrink(const Args& a, cudaStream_t stream) {
+  using C = Shrink<N>;
+  static bool done[64] = {};
+  int st = tc::configure_smem(shrink_kernel<N>, C::kSmem, done);
+  if (st) return st;
+  CUtensorMap mx, md;
+  const cuuint64_t x_dims[2] = {(cuuint64_t)a.width, (cuuint64_t)a.tokens}, x_strides[1] = {(cuuint64_t)a.x_stride * 2};
+  const cuuint32_t x_box[2] = {64, kShrinkRows};
+  const cuuint64_t d_dims[3] = {(cuuint64_t)a.width, (cuuint64_t)a.rank, (cuuint64_t)a.count};
+  const cuuint64_t d_strides[2] = {(cuuint64_t)a.width * 2, (cuuint64_t)a.width * (cuuint64_t)a.rank * 2};
+  const cuuint32_t d_box[3] = {64, N, 1};
+  if ((st = tc::make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, x_dims, x_strides, x_box, CU_TENSOR_MAP_SWIZZLE_128B)) ||
+      (st = tc::make_map(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.down, d_dims, d_strides, d_box, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return st;
+  const int64_t tiles = (a.tokens + kShrinkRows - 1) / kShrinkRows;
+  LR_REQUIRE(tiles <= 65535, "adapters: too many tokens");
+  const int parts = column_parts(a, tiles, 2 * sm_count(), 256);
+  return tc::launch("adapters (inner rows)", shrink_kernel<N>, dim3((unsigned)parts, (unsigned)tiles), kShrinkThreads, C::kSmem, stream,
+                    (unsigned)parts, false, mx, md, a);
+}
+
+template <int KS>
+int launch_expand(const Args& a, bool vec, cudaStream_t stream) {
+  const int64_t blocks = (a.outputs + kThreads - 1) / kThreads;
+  if (!vec) {
+    const int64_t all = (int64_t)((a.tokens + 31) / 32) * blocks;
+    LR_REQUIRE(all <= INT32_MAX, "adapters: too many blocks");
+    return tc::launch("adapters (outputs)", expand_odd_kernel<KS>, dim3((unsigned)all), kThreads, 0, stream, 1, true, a);
+  }
+  static bool done[64] = {};
+  int st = tc::configure_smem(expand_kernel<KS>, kExpandSmem, done);
+  if (st) return st;
+  CUtensorMap mb, mo;
+  const cuuint64_t dims[2] = {(cuuint64_t)a.outputs, (cuuint64_t)a.tokens};
+  const cuuint64_t base_strides[1] = {(cuuint64_t)a.base_stride * 2}, out_strides[1] = {(cuuint64_t)a.out_stride * 2};
+  const cuuint32_t box[2] = {32, kExpandRows};
+  if ((st = tc::make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.base, dims, base_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) ||
+      (st = tc::make_map(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.out, dims, out_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return st;
+  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks, most = 2 * sm_count();
+  return tc::launch("adapters (outputs)", expand_kernel<KS>, dim3((unsigned)(items < most ? items : most)), kThreads, kExpandSmem, stream,
+                    1, true, mb, mo, a);
+}
+
+// NR: tiles of 8 rank rows. Neighbours are tiled where an adapter has 64 tokens or more on average.
+template <int NR, int STRIPS>
+int run(const Args& a, bool vec, cudaStream_t stream) {
+  if (a.tokens <= kFew && a.tokens < 64 * (int64_t)a.count) {
+    const int tiles = (a.tokens + 15) / 16, chunks = (tiles + a.groups - 1) / a.groups;
+    const int st = launch_shrink_few<NR>(a, chunks, stream);
+    if (st) return st;
+    if (STRIPS > 1 && (int64_t)(a.outputs / kThreads) * a.groups * chunks > 4 * sm_count())
+      return launch_expand_few<NR / 2, STRIPS>(a, chunks, vec, stream);
+    return launch_expand_few<NR / 2, 1>(a, chunks, vec, stream);
+  }
+  const int st = launch_shrink<8 * NR>(a, stream);
+  return st ? st : launch_expand<NR / 2>(a, vec, stream);
 }
 
 }  // namespace
@@ -403,7 +791,7 @@ static int check_adapters(int64_t tokens, int64_t width, int64_t outputs, int64_
 
 extern "C" int64_t lr_adapters_workspace_bytes(int64_t tokens, int64_t width, int64_t outputs, int64_t rank, int64_t adapters) {
   if (check_adapters(tokens, width, outputs, rank, adapters) || tokens == 0) return 0;
-  return lr::adapters::plan(tokens, width, rank).bytes;
+  return lr::adapters::workspace_bytes(tokens, rank);
 }
 
 extern "C" int lr_adapters(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* down, const void* up,
@@ -414,27 +802,21 @@ extern "C" int lr_adapters(const void* x, int64_t x_stride, const void* base, in
   if (st) return st;
   if (tokens == 0) return LR_OK;
   LR_REQUIRE(x && base && down && up && index && out, "adapters: null pointer");
-  LR_REQUIRE(x_stride >= 0 && base_stride >= 0 && out_stride >= outputs, "adapters: strides");
+  LR_REQUIRE((x_stride >= width || tokens == 1) && x_stride >= 0 && base_stride >= 0 && out_stride >= outputs, "adapters: strides");
   if (x_stride % 8 || !aligned(x, 16) || !aligned(down, 16) || !aligned(up, 16))
     return set_error(LR_ERR_UNSUPPORTED, "adapters: x, down and up must be 16-byte aligned");
-  const adapters::Plan p = adapters::plan(tokens, width, rank);
-  LR_REQUIRE(workspace && workspace_bytes >= p.bytes && aligned(workspace, 16), "adapters: a workspace of %lld bytes is needed",
-             (long long)p.bytes);
+  const int64_t need = adapters::workspace_bytes(tokens, rank);
+  LR_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), "adapters: a workspace of %lld bytes is needed",
+             (long long)need);
   const adapters::Args a{static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(base),
                          static_cast<const __nv_bfloat16*>(down), static_cast<const __nv_bfloat16*>(up), scale, index,
-                         static_cast<__nv_bfloat16*>(out), x_stride, base_stride, out_stride, (int)tokens, (int)width,
-                         (int)outputs, (int)rank, (int)adapters, p.splits, p.padded, static_cast<float*>(workspace)};
-  const bool vec = outputs % 8 == 0 && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
+                         static_cast<__nv_bfloat16*>(out), static_cast<__nv_bfloat16*>(workspace), x_stride, base_stride,
+                         out_stride, (int)tokens, (int)width, (int)outputs, (int)rank, (int)adapters,
+                         adapters::padded_rank(rank), (int)(adapters < tokens ? adapters : tokens)};
+  const bool vec = outputs % 8 == 0 && base_stride >= outputs && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
   auto* s = static_cast<cudaStream_t>(stream);
-  if (p.few) {
-    const unsigned groups = (unsigned)(adapters < 16 ? adapters : 16);
-    if (rank <= 16) return adapters::launch_both<1, 2, 1>(a, groups, vec, s);
-    if (rank <= 32) return adapters::launch_both<1, 4, 1>(a, groups, vec, s);
-    if (rank <= 64) return adapters::launch_both<1, 8, 1>(a, groups, vec, s);
-    return adapters::launch_both<1, 16, 1>(a, groups, vec, s);
-  }
-  if (rank <= 16) return adapters::launch_both<4, 2, 4>(a, 1, vec, s);
-  if (rank <= 32) return adapters::launch_both<4, 4, 4>(a, 1, vec, s);
-  if (rank <= 64) return adapters::launch_both<2, 8, 4>(a, 1, vec, s);
-  return adapters::launch_both<2, 16, 4>(a, 1, vec, s);
+  if (rank <= 16) return adapters::run<2, 4>(a, vec, s);
+  if (rank <= 32) return adapters::run<4, 2>(a, vec, s);
+  if (rank <= 64) return adapters::run<8, 1>(a, vec, s);
+  return adapters::run<16, 1>(a, vec, s);
 }
