@@ -215,17 +215,19 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_few_kernel(const Args a) {
 
 // Many tokens: 128 neighbours against an adapter's N rank rows (padded with zeros)
 // on the tensor core, 64 columns of both a stage. The cluster's blocks take every
-// gridDim.x-th 64 columns and add their sums in order through shared memory. For
-// each adapter that occurs among the tokens the rows pass through again.
+// gridDim.x-th 64 columns and add their sums in order through shared memory. Up to
+// kTogether adapters that occur among the tokens are taken in one pass over the
+// rows, each in columns of its own of tensor memory.
 constexpr int kShrinkRows = 128;
 template <int N>
 struct Shrink {
-  static constexpr int kX = kShrinkRows * 128, kStage = kX + N * 128;
-  static constexpr int kStages = N <= 32 ? 4 : 3;
-  static constexpr int kSums = kStages * kStage;             // fp32 [N][kShrinkRows]
-  static constexpr int kBars = kSums + N * kShrinkRows * 4;  // full, empty, done; TMEM address, abort flag
+  static constexpr int kTogether = N <= 32 ? 4 : N == 64 ? 2 : 1;
+  static constexpr int kX = kShrinkRows * 128, kStage = kX + kTogether * N * 128;
+  static constexpr int kStages = 3;
+  static constexpr int kBars = kStages * kStage;  // full, empty, done; TMEM address, abort flag
+  static_assert(kBars >= N * kShrinkRows * 4, "the sums fit the ring");
   static constexpr size_t kSmem = 1024 + kBars + (2 * kStages + 1) * 8 + 8;
-  static constexpr uint32_t kColumns = N < 32 ? 32 : N;
+  static constexpr uint32_t kColumns = kTogether * N;
   // kind::f16: fp32 accumulator, bf16 operands, N / 8 at 17, M / 16 at 24
   static constexpr uint32_t kDesc =
       (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N / 8) << 17) | ((uint32_t)(kShrinkRows / 16) << 24);
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kShrinkThreads)
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* sums = reinterpret_cast<float*>(smem + C::kSums);
+  float* sums = reinterpret_cast<float*>(smem);  // [N][kShrinkRows], where the ring is between passes
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
   uint64_t *empty = full + C::kStages, *done = empty + C::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -281,20 +283,35 @@ __global__ void __launch_bounds__(kShrinkThreads)
   const int steps = (a.width + 63) / 64;
   const bool el = elect_one();
   bool ok = true;
-  uint32_t stage = 0;  // of the ring, over all adapters
+  uint32_t stage = 0;  // of the ring, over all passes
   int adapter;
   uint32_t members[4];
-  for (uint32_t number = 0; groups.next(adapter, members); ++number) {
-    adapter = uniform(adapter);
+  bool more = groups.next(adapter, members);
+  for (uint32_t pass = 0; more; ++pass) {
+    int taken[C::kTogether], together = 0;  // this pass's adapters
+#pragma unroll
+    for (int i = 0; i < C::kTogether; ++i) {
+      taken[i] = -1;
+      if (!more) continue;
+      taken[i] = uniform(adapter);
+      ++together;
+      more = groups.next(adapter, members);
+    }
+    int slot = -1;  // of this row's adapter among them
+#pragma unroll
+    for (int i = 0; i < C::kTogether; ++i)
+      if (mine >= 0 && mine == taken[i]) slot = i;
     if (warp == 0) {
       for (int step = part; step < steps && ok; step += parts, ++stage) {
         const uint32_t s = stage % C::kStages;
         ok = warp_wait(smem_u32(&empty[s]), ((stage / C::kStages) & 1u) ^ 1u, watch, lane);
         if (el && ok) {
           const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + s * C::kStage);
-          mbar_expect_tx(bar, C::kStage);
+          mbar_expect_tx(bar, C::kX + together * (N * 128));
           tma_load_2d(dst, &map_x, bar, step * 64, first);
-          tma_load_3d(dst + C::kX, &map_down, bar, step * 64, 0, adapter);
+#pragma unroll
+          for (int i = 0; i < C::kTogether; ++i)
+            if (i < together) tma_load_3d(dst + C::kX + i * (N * 128), &map_down, bar, step * 64, 0, taken[i]);
         }
         __syncwarp();
       }
@@ -306,8 +323,13 @@ __global__ void __launch_bounds__(kShrinkThreads)
         if (el && ok) {
           const uint32_t x = smem_u32(smem + s * C::kStage), w = x + C::kX;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem, desc_kmajor(x + kk * 32), desc_kmajor(w + kk * 32), C::kDesc, step != part || kk != 0 ? 1u : 0u);
+          for (int i = 0; i < C::kTogether; ++i) {
+            if (i >= together) break;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tmem + i * N, desc_kmajor(x + kk * 32), desc_kmajor(w + i * (N * 128) + kk * 32), C::kDesc,
+                     step != part || kk != 0 ? 1u : 0u);
+          }
           mma_commit(smem_u32(&empty[s]));
         }
         __syncwarp();
@@ -315,24 +337,27 @@ __global__ void __launch_bounds__(kShrinkThreads)
       if (el) mma_commit(smem_u32(done));
       __syncwarp();
     } else {
-      ok = ok && warp_wait(smem_u32(done), number & 1u, watch, lane);
+      ok = ok && warp_wait(smem_u32(done), pass & 1u, watch, lane);
       tc_fence_after();
-      const float scale = a.scale ? a.scale[adapter] : 1.0f;
+      const float scale = a.scale && slot >= 0 ? a.scale[mine] : 1.0f;
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       bf16* dst = a.inner + (int64_t)(first + row) * a.padded;
+      for (int i = 0; i < together; ++i) {
 #pragma unroll
-      for (int c = 0; c < N; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(lanes + c, v);
-        if (parts > 1) {
+        for (int c = 0; c < N; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(lanes + i * N + c, v);
+          if (slot != i || !ok) continue;
+          if (parts > 1) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sums[(c + i) * kShrinkRows + row] = __uint_as_float(v[i]);
-        } else if (ok && mine == adapter) {
-          uint32_t y[8];
+            for (int j = 0; j < 16; ++j) sums[(c + j) * kShrinkRows + row] = __uint_as_float(v[j]);
+          } else {
+            uint32_t y[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = cvt2(__uint_as_float(v[2 * i]) * scale, __uint_as_float(v[2 * i + 1]) * scale);
-          *reinterpret_cast<uint4*>(dst + c) = make_uint4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+            for (int j = 0; j < 8; ++j) y[j] = cvt2(__uint_as_float(v[2 * j]) * scale, __uint_as_float(v[2 * j + 1]) * scale);
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
         }
       }
       tc_fence_before();
@@ -341,8 +366,8 @@ __global__ void __launch_bounds__(kShrinkThreads)
       __syncwarp();
       cluster_sync_all();
       // this block's share of the columns, eight at a time
-      if (warp >= 2 && mine == adapter) {
-        const float scale = a.scale ? a.scale[adapter] : 1.0f;
+      if (slot >= 0) {
+        const float scale = a.scale ? a.scale[mine] : 1.0f;
         for (int c = part * 8; c < N; c += parts * 8) {
           float v[8];
 #pragma unroll
@@ -355,6 +380,7 @@ __global__ void __launch_bounds__(kShrinkThreads)
           *reinterpret_cast<uint4*>(a.inner + (int64_t)(first + row) * a.padded + c) = pack8(v);
         }
       }
+      fence_async_smem();  // the next pass's copies write where the sums were
       __syncwarp();
       cluster_sync_all();
     } else {
@@ -404,25 +430,35 @@ struct Up {
     }
   }
 };
-// acc += inner rows r0 (rows g) and r1 (rows g + 8), where they are to be read, times the weights.
+// The inner values of rows g and g + 8 of 16 that a thread multiplies.
 template <int KS>
-__device__ __forceinline__ void add_update(float (&acc)[4][4], const Up<KS>& up, const bf16* r0, bool lo, const bf16* r1, bool hi,
-                                           int t) {
-  if constexpr (KS == 1) {
-    const uint2 h0 = lo ? *reinterpret_cast<const uint2*>(r0 + 4 * t) : make_uint2(0u, 0u);
-    const uint2 h1 = hi ? *reinterpret_cast<const uint2*>(r1 + 4 * t) : make_uint2(0u, 0u);
+struct Inner {
+  uint32_t lo[2 * KS], hi[2 * KS];
+  // From rows r0 and r1 (zeros where they are not to be read).
+  __device__ __forceinline__ void load(const bf16* r0, bool there0, const bf16* r1, bool there1, int t) {
+    if constexpr (KS == 1) {
+      const uint2 h0 = there0 ? *reinterpret_cast<const uint2*>(r0 + 4 * t) : make_uint2(0u, 0u);
+      const uint2 h1 = there1 ? *reinterpret_cast<const uint2*>(r1 + 4 * t) : make_uint2(0u, 0u);
+      lo[0] = h0.x, lo[1] = h0.y, hi[0] = h1.x, hi[1] = h1.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mma_16816(acc[i], h0.x, h1.x, h0.y, h1.y, up.w[i][0][0], up.w[i][0][1]);
-  } else {
-#pragma unroll
-    for (int s = 0; s < KS; s += 2) {
-      const uint4 h0 = load16(r0 + 16 * s + 8 * t, lo), h1 = load16(r1 + 16 * s + 8 * t, hi);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mma_16816(acc[i], h0.x, h1.x, h0.y, h1.y, up.w[i][s][0], up.w[i][s][1]);
-        mma_16816(acc[i], h0.z, h1.z, h0.w, h1.w, up.w[i][s + 1][0], up.w[i][s + 1][1]);
+      for (int s = 0; s < KS; s += 2) {
+        const uint4 h0 = load16(r0 + 16 * s + 8 * t, there0), h1 = load16(r1 + 16 * s + 8 * t, there1);
+        lo[2 * s] = h0.x, lo[2 * s + 1] = h0.y, lo[2 * s + 2] = h0.z, lo[2 * s + 3] = h0.w;
+        hi[2 * s] = h1.x, hi[2 * s + 1] = h1.y, hi[2 * s + 2] = h1.z, hi[2 * s + 3] = h1.w;
       }
     }
+  }
+};
+// acc += inner values times the weights; rows that are not `lo`, `hi` count as zeros.
+template <int KS>
+__device__ __forceinline__ void add_update(float (&acc)[4][4], const Up<KS>& up, const Inner<KS>& h, bool lo, bool hi) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const uint32_t a0 = lo ? h.lo[2 * s] : 0u, a1 = hi ? h.hi[2 * s] : 0u;
+    const uint32_t a2 = lo ? h.lo[2 * s + 1] : 0u, a3 = hi ? h.hi[2 * s + 1] : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mma_16816(acc[i], a0, a1, a2, a3, up.w[i][s][0], up.w[i][s][1]);
   }
 }
 // Eight neighbouring columns of a row, as far as there are any.
@@ -490,9 +526,10 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const Args a) {
     }
     if (first == (int)blockIdx.z * 16) tc::wait_for_predecessor();
     if (adapter >= 0) {
+      Inner<KS> inner;
+      inner.load(a.inner + t0 * a.padded, lo, a.inner + t1 * a.padded, hi, t);
 #pragma unroll
-      for (int s = 0; s < STRIPS; ++s)
-        add_update<KS>(acc[s], up[s], a.inner + t0 * a.padded, lo, a.inner + t1 * a.padded, hi, t);
+      for (int s = 0; s < STRIPS; ++s) add_update<KS>(acc[s], up[s], inner, true, true);
     }
 #pragma unroll
     for (int s = 0; s < STRIPS; ++s) {
@@ -511,27 +548,33 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const Args a) {
 // 32, 400 us, a third of the memory's rate.) Rows in shared memory are 64 bytes
 // long and two of them fill the banks.
 constexpr int kExpandRows = 64;
-constexpr int kExpandSlots = 3;
 constexpr int kSlotBytes = kExpandRows * 64;
-constexpr size_t kExpandSmem = 128 + kWarps * kExpandSlots * (kSlotBytes + 8) + 8;
+template <int KS>
+struct Expand {
+  static constexpr int kBlocks = KS <= 4 ? 2 : 1;  // an SM: at rank 128 the weights alone are 64 registers
+  static constexpr int kSlots = KS <= 4 ? 3 : 6;
+  static constexpr int kHeld = KS <= 2 ? 4 : 2;  // 16-row tiles whose inner values are loaded together
+  static constexpr size_t kSmem = 128 + kWarps * kSlots * (kSlotBytes + 8) + 8;
+};
 
 // One row's eight columns in a tile.
 __device__ __forceinline__ uint4* tile_at(uint8_t* tile, int row, int t) { return reinterpret_cast<uint4*>(tile + row * 64 + t * 16); }
 
 template <int KS>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, Expand<KS>::kBlocks)
     expand_kernel(const __grid_constant__ CUtensorMap map_base, const __grid_constant__ CUtensorMap map_out, const Args a) {
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * (kExpandSlots * kSlotBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kExpandSlots * kSlotBytes) + warp * kExpandSlots;
-  uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + kWarps * kExpandSlots * (kSlotBytes + 8));
+  constexpr int kSlots = Expand<KS>::kSlots, kHeld = Expand<KS>::kHeld;
+  uint8_t* ring = smem + warp * (kSlots * kSlotBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kSlots * kSlotBytes) + warp * kSlots;
+  uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + kWarps * kSlots * (kSlotBytes + 8));
   const Watch watch{abort_flag, &g_adapters_status};
   if (lane == 0) {
-    for (int s = 0; s < kExpandSlots; ++s) mbar_init(smem_u32(&full[s]), 1);
+    for (int s = 0; s < kSlots; ++s) mbar_init(smem_u32(&full[s]), 1);
     if (warp == 0) {
       *abort_flag = 0u;
       prefetch_map(&map_base);
@@ -550,14 +593,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   int tile = fetch_tile, column = fetch_column;
   const auto fetch = [&] {
     if (fetched < count && fetch_column < a.outputs && el) {
-      const uint32_t s = (uint32_t)fetched % kExpandSlots, bar = smem_u32(&full[s]);
+      const uint32_t s = (uint32_t)fetched % kSlots, bar = smem_u32(&full[s]);
       mbar_expect_tx(bar, kSlotBytes);
       tma_load_2d(smem_u32(ring + s * kSlotBytes), &map_base, bar, fetch_column, fetch_tile * kExpandRows);
     }
     ++fetched;
     if (++fetch_tile == tiles) fetch_tile = 0, fetch_column += kThreads;
   };
-  for (int s = 0; s < kExpandSlots; ++s) fetch();
+  for (int s = 0; s < kSlots; ++s) fetch();
   Groups<2> groups;
   groups.load(a, tile * kExpandRows, lane);
   wait_for_predecessor();
@@ -570,35 +613,54 @@ __global__ void __launch_bounds__(kThreads, 2)
     now.check(a);
     if (++tile == tiles) tile = 0, column += kThreads;
     if (i + 1 < count) groups.load(a, tile * kExpandRows, lane);
-    const uint32_t s = (uint32_t)i % kExpandSlots;
+    const uint32_t s = (uint32_t)i % kSlots;
     uint8_t* rows = ring + s * kSlotBytes;
     const bool there = this_column < a.outputs;  // the last columns' warps may have none
     if (there) {
-      if (!(ok = warp_wait(smem_u32(&full[s]), ((uint32_t)i / kExpandSlots) & 1u, watch, lane))) break;
-      __syncwarp();
+      // Inner values do not depend on whose they are; they load before the base rows are there.
+      Inner<KS> inner[kHeld];
+      const auto load_inner = [&](int from) {
+#pragma unroll
+        for (int m = 0; m < kHeld; ++m) {
+          const int token = first + 16 * (from + m) + g;
+          const bf16* r = a.inner + (int64_t)token * a.padded;
+          inner[m].load(r, token < a.tokens, r + 8 * a.padded, token + 8 < a.tokens, t);
+        }
+      };
+      load_inner(0);
       int adapter;
       uint32_t members[2];
-      while (now.next(adapter, members)) {
+      bool all = this_column == kept_column && __all_sync(0xffffffffu, now.id[0] == kept && now.id[1] == kept);
+      bool any = all || now.next(adapter, members);
+      if (all) members[0] = members[1] = 0xffffffffu, adapter = kept;
+      bool held = true;  // the first kHeld tiles' inner values
+      if (!(ok = warp_wait(smem_u32(&full[s]), ((uint32_t)i / kSlots) & 1u, watch, lane))) break;
+      __syncwarp();
+      while (any) {
         if (adapter != kept || this_column != kept_column) {
           kept = adapter, kept_column = this_column;
           up.load(a, adapter, this_column, g, t);
         }
 #pragma unroll
-        for (int m = 0; m < kExpandRows / 16; ++m) {
-          const uint32_t here = members[m / 2] >> (16 * (m % 2)) & 0xffffu;
-          if (here == 0u) continue;
-          // rows of other adapters are neither changed nor used
-          const bool lo = here >> g & 1, hi = here >> (8 + g) & 1;
-          const bf16* r = a.inner + (int64_t)(first + 16 * m + g) * a.padded;
-          uint4 *r0 = tile_at(rows, 16 * m + g, t), *r1 = tile_at(rows, 16 * m + 8 + g, t);
-          float acc[4][4];
-          unpack_row(acc, 0, *r0);
-          unpack_row(acc, 1, *r1);
-          add_update<KS>(acc, up, r, lo, r + 8 * a.padded, hi, t);
-          if (lo) *r0 = make_uint4(cvt2(acc[0][0], acc[0][1]), cvt2(acc[1][0], acc[1][1]), cvt2(acc[2][0], acc[2][1]), cvt2(acc[3][0], acc[3][1]));
-          if (hi) *r1 = make_uint4(cvt2(acc[0][2], acc[0][3]), cvt2(acc[1][2], acc[1][3]), cvt2(acc[2][2], acc[2][3]), cvt2(acc[3][2], acc[3][3]));
+        for (int from = 0; from < kExpandRows / 16; from += kHeld) {
+          if (kHeld < kExpandRows / 16 && !(from == 0 && held)) load_inner(from);
+#pragma unroll
+          for (int m = from; m < from + kHeld; ++m) {
+            const uint32_t here = members[m / 2] >> (16 * (m % 2)) & 0xffffu;
+            if (here == 0u) continue;
+            // rows of other adapters are neither changed nor used
+            const bool lo = here >> g & 1, hi = here >> (8 + g) & 1;
+            uint4 *r0 = tile_at(rows, 16 * m + g, t), *r1 = tile_at(rows, 16 * m + 8 + g, t);
+            float acc[4][4];
+            unpack_row(acc, 0, *r0);
+            unpack_row(acc, 1, *r1);
+            add_update<KS>(acc, up, inner[m - from], lo, hi);
+            if (lo) *r0 = make_uint4(cvt2(acc[0][0], acc[0][1]), cvt2(acc[1][0], acc[1][1]), cvt2(acc[2][0], acc[2][1]), cvt2(acc[3][0], acc[3][1]));
+            if (hi) *r1 = make_uint4(cvt2(acc[0][2], acc[0][3]), cvt2(acc[1][2], acc[1][3]), cvt2(acc[2][2], acc[2][3]), cvt2(acc[3][2], acc[3][3]));
+          }
         }
-        __syncwarp();
+        held = false;
+        any = !all && now.next(adapter, members);
       }
       fence_async_smem();
       __syncwarp();
@@ -656,7 +718,9 @@ __global__ void __launch_bounds__(kThreads) expand_odd_kernel(const Args a) {
       float sum[4][4];
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum[i / 4][i % 4] = acc[m][i / 4][i % 4];
-      add_update<KS>(sum, up, r, lo, r + 8 * a.padded, hi, t);
+      Inner<KS> inner;
+      inner.load(r, lo, r + 8 * a.padded, hi, t);
+      add_update<KS>(sum, up, inner, true, true);
 #pragma unroll
       for (int i = 0; i < 16; ++i)  // rows of other adapters stay as they were
         if (i % 4 < 2 ? lo : hi) acc[m][i / 4][i % 4] = sum[i / 4][i % 4];
@@ -734,7 +798,7 @@ int launch_expand(const Args& a, bool vec, cudaStream_t stream) {
     return tc::launch("adapters (outputs)", expand_odd_kernel<KS>, dim3((unsigned)all), kThreads, 0, stream, 1, true, a);
   }
   static bool done[64] = {};
-  int st = tc::configure_smem(expand_kernel<KS>, kExpandSmem, done);
+  int st = tc::configure_smem(expand_kernel<KS>, Expand<KS>::kSmem, done);
   if (st) return st;
   CUtensorMap mb, mo;
   const cuuint64_t dims[2] = {(cuuint64_t)a.outputs, (cuuint64_t)a.tokens};
@@ -743,9 +807,9 @@ int launch_expand(const Args& a, bool vec, cudaStream_t stream) {
   if ((st = tc::make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.base, dims, base_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) ||
       (st = tc::make_map(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.out, dims, out_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return st;
-  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks, most = 2 * sm_count();
-  return tc::launch("adapters (outputs)", expand_kernel<KS>, dim3((unsigned)(items < most ? items : most)), kThreads, kExpandSmem, stream,
-                    1, true, mb, mo, a);
+  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks, most = Expand<KS>::kBlocks * sm_count();
+  return tc::launch("adapters (outputs)", expand_kernel<KS>, dim3((unsigned)(items < most ? items : most)), kThreads, Expand<KS>::kSmem,
+                    stream, 1, true, mb, mo, a);
 }
 
 // NR: tiles of 8 rank rows. Neighbours are tiled where an adapter has 64 tokens or more on average.
