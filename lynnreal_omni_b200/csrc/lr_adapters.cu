@@ -2,9 +2,8 @@
 //   out[t, :] = base[t, :] + scale[e] * up[e] (down[e] x[t, :]),  e = index[t]
 // (e < 0: out[t, :] = base[t, :]), where base is the shared projection's output.
 //
-// Two kernels: shrink_kernel makes the few values scale[e] down[e] x[t] of every
-// token, the expand kernels add up[e] times them to the base row. Both are bound
-// by memory: per byte of x or base a rank of 16 to 128 gives the tensor core 8 to
+// The first product makes the few inner values scale[e] down[e] x[t] of every
+// token, the second adds up[e] times them to the base row. Both are bound by memory: per byte of x or base a rank of 16 to 128 gives the tensor core 8 to
 // 64 products, so mma.sync is fast enough, and its operands come straight from
 // global memory, 16 bytes a load: a sum over columns does not mind their order,
 // and neither do the outputs of a tile, so what a thread loads at once are the
@@ -12,7 +11,8 @@
 //
 // Up to kFew tokens, where one token a request is usual, a block stands for one
 // adapter and lists its tokens first, so that every adapter in use is read about
-// once whatever the order. More tokens are taken in tiles of neighbours: for each
+// once whatever the order: few_kernel, both products. More tokens are taken in
+// tiles of neighbours, by shrink_kernel and an expand kernel: for each
 // adapter that occurs in a tile the rows of the others are zeros, and their sums
 // are put back afterwards. Either way an infinity in one request's row or adapter
 // reaches no other.
@@ -142,77 +142,6 @@ __device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
 }
 
 // ------------------------------------------------------------------ shrink
-// Few tokens. NR tiles of 8 rank rows. The warps of the blocks of a cluster
-// (gridDim.x blocks) take every gridDim.x * kWarps-th 32 columns; their sums are
-// added in a fixed order through shared memory, scaled and rounded to bf16 for the
-// second product (2^-9 of the update, as every factor of it is rounded already).
-template <int NR>
-__global__ void __launch_bounds__(kThreads, 2) shrink_few_kernel(const Args a) {
-  constexpr int kTile = 16 * 8 * NR;
-  constexpr int kAhead = NR <= 2 ? 4 : NR <= 4 ? 2 : 1;  // steps whose loads are under way together
-  extern __shared__ float sums[];                         // [kWarps][kTile], then the block's [kTile]
-  __shared__ List list;
-  float* block_sums = sums + kWarps * kTile;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int part = blockIdx.x, parts = gridDim.x;
-  tc::allow_dependent();
-  int adapter;
-  const int count = list_tokens(a, list, blockIdx.y, adapter);
-  for (int first = blockIdx.z * 16; first < count; first += gridDim.z * 16) {
-    float acc[NR][4];
-#pragma unroll
-    for (int i = 0; i < NR * 4; ++i) acc[i / 4][i % 4] = 0.0f;
-    const bf16* down = a.down + ((int64_t)adapter * a.rank + g) * a.width;
-    const bool lo = first + g < count, hi = first + 8 + g < count;
-    const bf16* r0 = a.x + (int64_t)list.token[lo ? first + g : first] * a.x_stride;
-    const bf16* r1 = a.x + (int64_t)list.token[hi ? first + 8 + g : first] * a.x_stride;
-#pragma unroll kAhead
-    for (int k0 = (part * kWarps + warp) * 32; k0 < a.width; k0 += parts * kWarps * 32) {
-      const int k = k0 + 8 * t;
-      const bool there = k < a.width;
-      uint4 w[NR];
-#pragma unroll
-      for (int n = 0; n < NR; ++n) w[n] = load16(down + (int64_t)(8 * n) * a.width + k, there && 8 * n + g < a.rank);
-      const uint4 x0 = load16(r0 + k, there && lo), x1 = load16(r1 + k, there && hi);
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        mma_16816(acc[n], x0.x, x1.x, x0.y, x1.y, w[n].x, w[n].y);
-        mma_16816(acc[n], x0.z, x1.z, x0.w, x1.w, w[n].z, w[n].w);
-      }
-    }
-    // [register][lane] of each warp: no two lanes in one bank
-#pragma unroll
-    for (int i = 0; i < NR * 4; ++i) sums[warp * kTile + i * 32 + lane] = acc[i / 4][i % 4];
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile; i += kThreads) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += sums[w * kTile + i];
-      block_sums[i] = v;
-    }
-    if (parts > 1) tc::cluster_sync_all(); else __syncthreads();
-    const float scale = a.scale ? a.scale[adapter] : 1.0f;
-    for (int i = part * kThreads + threadIdx.x; i < kTile / 2; i += parts * kThreads) {
-      // two columns side by side: registers 2 e, 2 e + 1 of a lane
-      const int l = i % 32, e = i / 32 % 2, n = i / 64;
-      const int at = (n * 4 + 2 * e) * 32 + l, r = first + 8 * e + l / 4;
-      if (r >= count) continue;
-      float v0 = 0.0f, v1 = 0.0f;
-      if (parts > 1) {
-        for (int p = 0; p < parts; ++p) {
-          v0 += cluster_load(block_sums + at, p);
-          v1 += cluster_load(block_sums + at + 32, p);
-        }
-      } else {
-        v0 = block_sums[at], v1 = block_sums[at + 32];
-      }
-      *reinterpret_cast<uint32_t*>(a.inner + (int64_t)list.token[r] * a.padded + 8 * n + 2 * (l % 4)) = cvt2(v0 * scale, v1 * scale);
-    }
-    if (parts > 1) tc::cluster_sync_all(); else __syncthreads();
-  }
-}
-
 // Many tokens: 128 neighbours against an adapter's N rank rows (padded with zeros)
 // on the tensor core, 64 columns of both a stage. The cluster's blocks take every
 // gridDim.x-th 64 columns and add their sums in order through shared memory. Up to
@@ -411,18 +340,19 @@ __global__ void __launch_bounds__(kShrinkThreads)
 template <int KS>
 struct Up {
   uint32_t w[4][KS][2];
-  __device__ __forceinline__ void load(const Args& a, int adapter, int column, int g, int t) {
+  // From `weight`, the adapter's. Columns past the last are the last one's again: they are not stored.
+  __device__ __forceinline__ void load(const bf16* weight, int column, int outputs, int rank, int g, int t) {
+    const int n = column + 8 * (g >> 1) + (g & 1), last = outputs - 1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int n = column + 8 * (g >> 1) + 2 * i + (g & 1);
-      const bf16* src = a.up + ((int64_t)adapter * a.outputs + n) * a.rank;
+      const bf16* src = weight + (int64_t)min(n + 2 * i, last) * rank;
       if constexpr (KS == 1) {
-        const uint2 v = n < a.outputs && 4 * t < a.rank ? *reinterpret_cast<const uint2*>(src + 4 * t) : make_uint2(0u, 0u);
+        const uint2 v = 4 * t < rank ? *reinterpret_cast<const uint2*>(src + 4 * t) : make_uint2(0u, 0u);
         w[i][0][0] = v.x, w[i][0][1] = v.y;
       } else {
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
-          const uint4 v = load16(src + 16 * s + 8 * t, n < a.outputs && 16 * s + 8 * t < a.rank);
+          const uint4 v = load16(src + 16 * s + 8 * t, 16 * s + 8 * t < rank);
           w[i][s][0] = v.x, w[i][s][1] = v.y;
           w[i][s + 1][0] = v.z, w[i][s + 1][1] = v.w;
         }
@@ -430,6 +360,7 @@ struct Up {
     }
   }
 };
+__device__ __forceinline__ const bf16* up_of(const Args& a, int adapter) { return a.up + (int64_t)adapter * a.outputs * a.rank; }
 // The inner values of rows g and g + 8 of 16 that a thread multiplies.
 template <int KS>
 struct Inner {
@@ -495,47 +426,132 @@ __device__ __forceinline__ void unpack_row(float (&acc)[4][4], int h, const uint
   }
 }
 
-// Few tokens: a block stands for one adapter and STRIPS times 256 columns. The
-// weights and the base rows are under way before the inner rows are there.
-template <int KS, int STRIPS, bool VEC>
-__global__ void __launch_bounds__(kThreads) expand_few_kernel(const Args a) {
+// ------------------------------------------------------------------ few tokens
+// Both products in one kernel: clusters stand for one adapter and their blocks for
+// every gridDim.x-th 256 columns. A cluster's blocks share the first product, every
+// warp 32 columns of x at a time, add their sums in a fixed order through shared
+// memory and have the inner rows in it at once. (A launch of its own for the inner
+// rows: one token 6144 to 18432 5.2 us and 18.4 us with the host, now 5.0 and 13.6.)
+// Weights and base rows of the second product load meanwhile, and then kAhead
+// strips ahead. An adapter's second cluster reads `down` again, from L2; grids are
+// one wave.
+template <int KS>
+struct Few {
+  static constexpr int kTile = 16 * 16 * KS;                      // inner values of 16 tokens
+  static constexpr int kSteps = KS == 1 ? 4 : KS <= 4 ? 2 : 1;    // of the first product whose loads are under way together
+  static constexpr int kAhead = KS == 1 ? 4 : KS == 2 ? 2 : 1;
+  static constexpr int kLine = KS >= 4 ? 16 * KS + 32 : 16 * KS;  // inner rows side by side in different banks
+  static constexpr int kBlocks = KS <= 2 ? 2 : 1;                 // an SM
+  static constexpr size_t kSmem = (kWarps + 1) * kTile * 4 + 16 * kLine * 2;
+};
+
+template <int KS, bool VEC>
+__global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const Args a) {
+  using C = Few<KS>;
+  constexpr int NR = 2 * KS;
+  extern __shared__ float sums[];  // [kWarps][kTile], the block's [kTile], then the inner rows
   __shared__ List list;
+  float* block_sums = sums + kWarps * C::kTile;
+  bf16* inner_rows = reinterpret_cast<bf16*>(block_sums + C::kTile);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int column = blockIdx.x * (STRIPS * kThreads) + warp * 32;
+  const int parts = tc::cluster_size(), part = parts > 1 ? (int)tc::cluster_rank() : 0;
+  const int stride = gridDim.x * kThreads;
+  const int start = blockIdx.x * kThreads + warp * 32;
   int adapter;
-  const int n = list_tokens(a, list, blockIdx.y, adapter);
-  if ((int)blockIdx.z * 16 >= n || (adapter < 0 && a.out == a.base && a.out_stride == a.base_stride)) {
-    tc::wait_for_predecessor();
-    return;
-  }
-  Up<KS> up[STRIPS];
-  if (adapter >= 0) {
-#pragma unroll
-    for (int s = 0; s < STRIPS; ++s) up[s].load(a, adapter, column + s * kThreads, g, t);
-  }
-  for (int first = blockIdx.z * 16; first < n; first += gridDim.z * 16) {
-    const bool lo = first + g < n, hi = first + 8 + g < n;
+  const int count = list_tokens(a, list, blockIdx.y, adapter);
+  // the same in all blocks of the cluster
+  if ((int)blockIdx.z * 16 >= count || (adapter < 0 && a.out == a.base && a.out_stride == a.base_stride)) return;
+  for (int first = blockIdx.z * 16; first < count; first += gridDim.z * 16) {
+    const bool lo = first + g < count, hi = first + 8 + g < count;
     const int64_t t0 = list.token[lo ? first + g : first], t1 = list.token[hi ? first + 8 + g : first];
-    float acc[STRIPS][4][4];
+    // strips of columns under way, a ring
+    Up<KS> up[C::kAhead];
+    uint4 base[C::kAhead][2];
+    const bf16 *weight = up_of(a, max(adapter, 0)), *b0 = a.base + t0 * a.base_stride, *b1 = a.base + t1 * a.base_stride;
+    bf16 *o0 = a.out + t0 * a.out_stride, *o1 = a.out + t1 * a.out_stride;
+    const auto load_strip = [&](int s, int column) {
+      if (column >= a.outputs) return;
+      const int mine = column + 8 * t;
+      base[s][0] = load_row<VEC>(b0 + mine, a.outputs - mine, lo);
+      base[s][1] = load_row<VEC>(b1 + mine, a.outputs - mine, hi);
+      if (adapter >= 0) up[s].load(weight, column, a.outputs, a.rank, g, t);
+    };
+    if (KS <= 4) {  // else the registers are not there yet
 #pragma unroll
-    for (int s = 0; s < STRIPS; ++s) {
-      const int mine = column + s * kThreads + 8 * t;
-      unpack_row(acc[s], 0, load_row<VEC>(a.base + t0 * a.base_stride + mine, a.outputs - mine, lo));
-      unpack_row(acc[s], 1, load_row<VEC>(a.base + t1 * a.base_stride + mine, a.outputs - mine, hi));
+      for (int s = 0; s < C::kAhead; ++s) load_strip(s, start + s * stride);
     }
-    if (first == (int)blockIdx.z * 16) tc::wait_for_predecessor();
     if (adapter >= 0) {
-      Inner<KS> inner;
-      inner.load(a.inner + t0 * a.padded, lo, a.inner + t1 * a.padded, hi, t);
+      float acc[NR][4];
 #pragma unroll
-      for (int s = 0; s < STRIPS; ++s) add_update<KS>(acc[s], up[s], inner, true, true);
+      for (int i = 0; i < NR * 4; ++i) acc[i / 4][i % 4] = 0.0f;
+      const bf16* down = a.down + ((int64_t)adapter * a.rank + g) * a.width;
+      const bf16 *x0 = a.x + t0 * a.x_stride, *x1 = a.x + t1 * a.x_stride;
+#pragma unroll C::kSteps
+      for (int k0 = (part * kWarps + warp) * 32; k0 < a.width; k0 += parts * kWarps * 32) {
+        const int k = k0 + 8 * t;
+        const bool there = k < a.width;
+        uint4 w[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) w[n] = load16(down + (int64_t)(8 * n) * a.width + k, there && 8 * n + g < a.rank);
+        const uint4 v0 = load16(x0 + k, there && lo), v1 = load16(x1 + k, there && hi);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          mma_16816(acc[n], v0.x, v1.x, v0.y, v1.y, w[n].x, w[n].y);
+          mma_16816(acc[n], v0.z, v1.z, v0.w, v1.w, w[n].z, w[n].w);
+        }
+      }
+      // [register][lane] of each warp: no two lanes in one bank
+#pragma unroll
+      for (int i = 0; i < NR * 4; ++i) sums[warp * C::kTile + i * 32 + lane] = acc[i / 4][i % 4];
+      __syncthreads();
+      for (int i = threadIdx.x; i < C::kTile; i += kThreads) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += sums[w * C::kTile + i];
+        block_sums[i] = v;
+      }
+      if (parts > 1) tc::cluster_sync_all(); else __syncthreads();
+      const float scale = a.scale ? a.scale[adapter] : 1.0f;
+      for (int i = threadIdx.x; i < C::kTile / 2; i += kThreads) {
+        // two columns side by side: registers 2 e, 2 e + 1 of a lane
+        const int l = i % 32, e = i / 32 % 2, n = i / 64;
+        const int at = (n * 4 + 2 * e) * 32 + l;
+        float h0 = 0.0f, h1 = 0.0f;
+        if (parts > 1) {
+#pragma unroll 8
+          for (int p = 0; p < parts; ++p) {
+            h0 += cluster_load(block_sums + at, p);
+            h1 += cluster_load(block_sums + at + 32, p);
+          }
+        } else {
+          h0 = block_sums[at], h1 = block_sums[at + 32];
+        }
+        *reinterpret_cast<uint32_t*>(inner_rows + (8 * e + l / 4) * C::kLine + 8 * n + 2 * (l % 4)) = cvt2(h0 * scale, h1 * scale);
+      }
+      __syncthreads();
+      if (parts > 1) tc::cluster_arrive();  // done with the other blocks' sums
     }
+    Inner<KS> inner;
+    if (adapter >= 0) inner.load(inner_rows + g * C::kLine, lo, inner_rows + (8 + g) * C::kLine, hi, t);
+    if (KS > 4) load_strip(0, start);
+    for (int next = start; next < a.outputs;) {
 #pragma unroll
-    for (int s = 0; s < STRIPS; ++s) {
-      const int mine = column + s * kThreads + 8 * t;
-      if (lo) store_row<VEC>(a.out + t0 * a.out_stride + mine, acc[s], 0, a.outputs - mine);
-      if (hi) store_row<VEC>(a.out + t1 * a.out_stride + mine, acc[s], 1, a.outputs - mine);
+      for (int s = 0; s < C::kAhead; ++s, next += stride) {
+        if (next >= a.outputs) break;
+        const int mine = next + 8 * t;
+        float acc[4][4];
+        unpack_row(acc, 0, base[s][0]);
+        unpack_row(acc, 1, base[s][1]);
+        if (adapter >= 0) add_update<KS>(acc, up[s], inner, true, true);
+        load_strip(s, next + C::kAhead * stride);
+        if (lo) store_row<VEC>(o0 + mine, acc, 0, a.outputs - mine);
+        if (hi) store_row<VEC>(o1 + mine, acc, 1, a.outputs - mine);
+      }
+    }
+    if (adapter >= 0) {
+      __syncthreads();  // the inner rows have been read
+      if (parts > 1) tc::cluster_wait();
     }
   }
 }
@@ -639,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, Expand<KS>::kBlocks)
       while (any) {
         if (adapter != kept || this_column != kept_column) {
           kept = adapter, kept_column = this_column;
-          up.load(a, adapter, this_column, g, t);
+          up.load(up_of(a, adapter), this_column, a.outputs, a.rank, g, t);
         }
 #pragma unroll
         for (int from = 0; from < kExpandRows / 16; from += kHeld) {
@@ -708,7 +724,7 @@ __global__ void __launch_bounds__(kThreads) expand_odd_kernel(const Args a) {
   bool waited = false;
   while (groups.next(adapter, members)) {
     Up<KS> up;
-    up.load(a, adapter, column, g, t);
+    up.load(up_of(a, adapter), column, a.outputs, a.rank, g, t);
     if (!waited) tc::wait_for_predecessor();
     waited = true;
 #pragma unroll
@@ -738,7 +754,6 @@ __global__ void __launch_bounds__(kThreads) expand_odd_kernel(const Args a) {
 
 // ------------------------------------------------------------------ host
 int padded_rank(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-int64_t workspace_bytes(int64_t tokens, int64_t rank) { return tokens * padded_rank(rank) * 2; }
 
 // Blocks of a cluster that share the columns of `tiles` tiles: as many as give the GPU `blocks`, each at least `columns` wide.
 int column_parts(const Args& a, int64_t tiles, int64_t blocks, int columns) {
@@ -747,24 +762,26 @@ int column_parts(const Args& a, int64_t tiles, int64_t blocks, int columns) {
   return parts;
 }
 
-template <int NR>
-int launch_shrink_few(const Args& a, int chunks, cudaStream_t stream) {
-  constexpr size_t smem = (kWarps + 1) * 16 * 8 * NR * 4;
-  static bool done[64] = {};
-  if (smem > 40 * 1024) {
-    const int st = tc::configure_smem(shrink_few_kernel<NR>, smem, done);
-    if (st) return st;
-  }
-  const int parts = column_parts(a, (int64_t)a.groups * chunks, 2 * sm_count(), 64 * kWarps);
-  const dim3 grid((unsigned)parts, (unsigned)a.groups, (unsigned)chunks);
-  return tc::launch("adapters (inner rows)", shrink_few_kernel<NR>, grid, kThreads, smem, stream, (unsigned)parts, false, a);
+// Tokens by their adapters, in one kernel? Neighbours are tiled where an adapter has 64 of them or more on average.
+bool few(int64_t tokens, int64_t adapters) { return tokens <= kFew && tokens < 64 * adapters; }
+int64_t workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank) {
+  return few(tokens, adapters) ? 0 : tokens * padded_rank(rank) * 2;
 }
 
-template <int KS, int STRIPS>
-int launch_expand_few(const Args& a, int chunks, bool vec, cudaStream_t stream) {
-  const dim3 grid((unsigned)((a.outputs + STRIPS * kThreads - 1) / (STRIPS * kThreads)), (unsigned)(a.groups + 1), (unsigned)chunks);
-  return tc::launch("adapters (outputs)", vec ? expand_few_kernel<KS, STRIPS, true> : expand_few_kernel<KS, STRIPS, false>, grid,
-                    kThreads, 0, stream, 1, true, a);
+template <int KS>
+int launch_few(const Args& a, bool vec, cudaStream_t stream) {
+  const auto kernel = vec ? few_kernel<KS, true> : few_kernel<KS, false>;
+  static bool done[2][64] = {};
+  const int st = tc::configure_smem(kernel, Few<KS>::kSmem, done[vec]);
+  if (st) return st;
+  const int tiles = (a.tokens + 15) / 16, chunks = (tiles + a.groups - 1) / a.groups;
+  int blocks = Few<KS>::kBlocks * sm_count() / (a.groups * chunks);  // for one adapter's tile
+  if (blocks > (a.outputs + kThreads - 1) / kThreads) blocks = (a.outputs + kThreads - 1) / kThreads;
+  int parts = 1;
+  while (parts < 8 && 2 * parts <= blocks && (int64_t)parts * kWarps * 32 < a.width) parts *= 2;
+  blocks = blocks < 1 ? 1 : blocks / parts * parts;
+  const dim3 grid((unsigned)blocks, (unsigned)(a.groups + 1), (unsigned)chunks);
+  return tc::launch("adapters (few tokens)", kernel, grid, kThreads, Few<KS>::kSmem, stream, (unsigned)parts, false, a);
 }
 
 template <int N>
@@ -812,19 +829,11 @@ int launch_expand(const Args& a, bool vec, cudaStream_t stream) {
                     stream, 1, true, mb, mo, a);
 }
 
-// NR: tiles of 8 rank rows. Neighbours are tiled where an adapter has 64 tokens or more on average.
-template <int NR, int STRIPS>
+template <int KS>
 int run(const Args& a, bool vec, cudaStream_t stream) {
-  if (a.tokens <= kFew && a.tokens < 64 * (int64_t)a.count) {
-    const int tiles = (a.tokens + 15) / 16, chunks = (tiles + a.groups - 1) / a.groups;
-    const int st = launch_shrink_few<NR>(a, chunks, stream);
-    if (st) return st;
-    if (STRIPS > 1 && (int64_t)(a.outputs / kThreads) * a.groups * chunks > 4 * sm_count())
-      return launch_expand_few<NR / 2, STRIPS>(a, chunks, vec, stream);
-    return launch_expand_few<NR / 2, 1>(a, chunks, vec, stream);
-  }
-  const int st = launch_shrink<8 * NR>(a, stream);
-  return st ? st : launch_expand<NR / 2>(a, vec, stream);
+  if (few(a.tokens, a.count)) return launch_few<KS>(a, vec, stream);
+  const int st = launch_shrink<16 * KS>(a, stream);
+  return st ? st : launch_expand<KS>(a, vec, stream);
 }
 
 }  // namespace
@@ -855,7 +864,7 @@ static int check_adapters(int64_t tokens, int64_t width, int64_t outputs, int64_
 
 extern "C" int64_t lr_adapters_workspace_bytes(int64_t tokens, int64_t width, int64_t outputs, int64_t rank, int64_t adapters) {
   if (check_adapters(tokens, width, outputs, rank, adapters) || tokens == 0) return 0;
-  return lr::adapters::workspace_bytes(tokens, rank);
+  return lr::adapters::workspace_bytes(tokens, adapters, rank);
 }
 
 extern "C" int lr_adapters(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* down, const void* up,
@@ -869,8 +878,8 @@ extern "C" int lr_adapters(const void* x, int64_t x_stride, const void* base, in
   LR_REQUIRE((x_stride >= width || tokens == 1) && x_stride >= 0 && base_stride >= 0 && out_stride >= outputs, "adapters: strides");
   if (x_stride % 8 || !aligned(x, 16) || !aligned(down, 16) || !aligned(up, 16))
     return set_error(LR_ERR_UNSUPPORTED, "adapters: x, down and up must be 16-byte aligned");
-  const int64_t need = adapters::workspace_bytes(tokens, rank);
-  LR_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), "adapters: a workspace of %lld bytes is needed",
+  const int64_t need = adapters::workspace_bytes(tokens, adapters, rank);
+  LR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "adapters: a workspace of %lld bytes is needed",
              (long long)need);
   const adapters::Args a{static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(base),
                          static_cast<const __nv_bfloat16*>(down), static_cast<const __nv_bfloat16*>(up), scale, index,
@@ -879,8 +888,8 @@ extern "C" int lr_adapters(const void* x, int64_t x_stride, const void* base, in
                          adapters::padded_rank(rank), (int)(adapters < tokens ? adapters : tokens)};
   const bool vec = outputs % 8 == 0 && base_stride >= outputs && base_stride % 8 == 0 && out_stride % 8 == 0 && aligned(base, 16) && aligned(out, 16);
   auto* s = static_cast<cudaStream_t>(stream);
-  if (rank <= 16) return adapters::run<2, 4>(a, vec, s);
-  if (rank <= 32) return adapters::run<4, 2>(a, vec, s);
-  if (rank <= 64) return adapters::run<8, 1>(a, vec, s);
-  return adapters::run<16, 1>(a, vec, s);
+  if (rank <= 16) return adapters::run<1>(a, vec, s);
+  if (rank <= 32) return adapters::run<2>(a, vec, s);
+  if (rank <= 64) return adapters::run<4>(a, vec, s);
+  return adapters::run<8>(a, vec, s);
 }
