@@ -22,6 +22,8 @@
 //     us, 5.9 TB/s, 0.91 of the measured copy rate; one against 32768: 27 us.
 //     The prompt kernel would leave all but `group` of a tile's 256 rows empty
 //     and one CTA to a sequence's keys.
+#include <type_traits>
+
 #include "lr_common.cuh"
 #include "lr_host.h"
 #include "lr_tc.cuh"
@@ -634,18 +636,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     PromptItem w;
     for (uint32_t number = 0; ok && next_item(number, w); ++number) {
       // keys that this row sees, -1 for a row that stands for nothing
-      int seen = -1, prefix_seen = -1;
+      int seen = -1;
+      bool there = false;
       bf16* dst = a.out;
       int64_t part = 0;
       {
         const int offset = t * ps.tokens_tile + in_tile;  // of this row's token in the block
         const int token = w.tok0 + offset;
         if (in_tile < ps.tokens_tile && head < w.heads_here && token < w.lq) {
+          there = true;
           seen = MODE != kPrefixPart && a.causal ? min(max(token + w.lk - w.lq + 1, 0), w.lk) : w.lk;
-          if (MODE == kWithPrefix) prefix_seen = px.keys;
           const int64_t at = (int64_t)(w.q_row + offset) * a.heads + w.head0 + head;
           dst += at * D;
           if (MODE == kPrefixPart) part = (int64_t)(w.k_row / px.chunk) * a.total_q * a.heads + at;
+        } else if (MODE != kNoPrefix) {
+          // A row that stands for nothing sees every key, so that its warp has no mask to test: 48 prompts of 1 to 512 tokens
+          // behind 1000 keys 183 us with no key, PENDING us with all.
+          seen = w.lk;
         }
       }
       const int n = w.tiles[t];
@@ -654,7 +661,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!(ok = warp_wait(smem_u32(&s_full[t]), done & 1u, watch, lane))) break;
         tc_fence_after();
         // Both halves for the maximum; the second stays in registers, the first is read again for its probabilities.
-        const int valid = MODE == kWithPrefix ? (j < px.tiles ? prefix_seen - j * kKeys : seen - (j - px.tiles) * kKeys)
+        const int valid = MODE == kWithPrefix ? (j < px.tiles ? px.keys - j * kKeys : seen - (j - px.tiles) * kKeys)
                                               : seen - j * kKeys;
         const bool full_tile = __all_sync(0xffffffffu, valid >= kKeys);
         uint32_t s[kHalf];
@@ -725,7 +732,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(&o_empty[t]));
           }
         }
-        if (seen < 0) continue;
+        if (!there) continue;
         if constexpr (MODE == kPrefixPart) {
           float* to = px.part_o + part * D + c;
 #pragma unroll
@@ -799,55 +806,44 @@ struct StepPrefix {
   int64_t k_ts, k_hs, v_ts, v_hs;
   int keys;
   int chunk, chunks;  // keys of a part of the prefix, parts
-  int slots;          // chunks where this kernel makes the prefix's parts itself, 0 where prompt_kernel has
+  int slots;          // chunks where this kernel makes the prefix's parts itself, 0 where prompt_kernel does
   float *part_o, *own_o;      // [chunks][total_q][heads][D], [total_q][heads][D] (the sequences that are not split)
   float2 *part_ml, *own_ml;
 };
 
-// One row's parts, added in order, to y (columns lane, lane + 32, ...) and sum, which belong to the maximum `top`: a warp.
-template <int D>
-__device__ __forceinline__ void add_prefix(const StepPrefix& sp, int64_t rows, int64_t row, int lane, float& top, float& sum,
-                                           float (&y)[D / 32]) {
-  float most = top;
-  for (int p = lane; p < sp.chunks; p += 32) most = fmaxf(most, __ldcg(&sp.part_ml[p * rows + row]).x);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-  const float sub = most == -INFINITY ? 0.0f : most, f = ex2(top - sub);
-  sum *= f;
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) y[c] *= f;
-#pragma unroll 4
-  for (int p = 0; p < sp.chunks; ++p) {
-    const float2 ml = __ldcg(&sp.part_ml[p * rows + row]);
-    const float g = ex2(ml.x - sub);
-    sum = fmaf(ml.y, g, sum);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) y[c] = fmaf(__ldcg(&sp.part_o[(p * rows + row) * D + c * 32 + lane]), g, y[c]);
-  }
-  top = most;
-}
-
 // NT tiles of 8 rows. A CTA takes one slot's keys for one key/value head and
 // every gridDim.z-th group of 8 NT rows.
 //
-// SHARED: behind a prefix. Its parts either come from this kernel's first slots,
-// for the rows of all sequences (then join_shared_kernel joins every row's), or
-// from prompt_kernel, which runs meanwhile: rows of a sequence that is not split
-// take them up here.
-template <int D, int NT, bool SHARED>
+// SHARED: behind a prefix; every row leaves a part, which join_prefix_kernel joins
+// with the prefix's. Those either come from this kernel's first slots, for the
+// rows of all sequences, or from prompt_kernel, which runs meanwhile: one block
+// waits for it, so that this kernel does not end before it.
+//
+// WARPS: of a slot and head. One where there are enough slots and heads to fill
+// the GPU: a block is then that many heads side by side, and no warp waits for
+// another.
+template <int D, int NT, int WARPS, bool SHARED>
 __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   constexpr int R = 8 * NT;
+  constexpr int kHeads = kStepWarps / WARPS;
   __shared__ float sh_m[kStepWarps][R], sh_l[kStepWarps][R];
   __shared__ float sh_o[kStepWarps][R][D + 4];
+  if (SHARED && blockIdx.x == gridDim.x - 1) {
+    if ((blockIdx.y | blockIdx.z) == 0) wait_for_predecessor();
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const bool of_prefix = SHARED && (int)blockIdx.x < sp.slots;
-  const int slot = SHARED ? (int)blockIdx.x - sp.slots : (int)blockIdx.x, kv_head = blockIdx.y;
+  const int slot = SHARED ? (int)blockIdx.x - sp.slots : (int)blockIdx.x;
+  const int kv_head = kHeads == 1 ? (int)blockIdx.y : (int)blockIdx.y * kHeads + warp;
+  const int first_warp = kHeads == 1 ? 0 : warp;  // of this head's
+  if (kHeads > 1 && kv_head >= a.kv_heads) return;
   if (slot == 0 && kv_head == 0 && blockIdx.z == 0 && warp == 0) check_offsets(a, lane, 32);
   if (slot == 0 && blockIdx.z == 0) {  // tokens past the last offset
     const int from = clamped(a.cu_q, a.seqs, a.total_q);
     const int64_t count = (int64_t)(a.total_q - from) * a.group * (D / 8);
-    for (int64_t i = threadIdx.x; i < count; i += 32 * kStepWarps) {
+    for (int64_t i = threadIdx.x - 32 * first_warp; i < count; i += 32 * WARPS) {
       const int64_t row = i / (D / 8);
       const int64_t at = ((from + row / a.group) * a.heads + kv_head * a.group + row % a.group) * D + i % (D / 8) * 8;
       *reinterpret_cast<uint4*>(a.out + at) = make_uint4(0u, 0u, 0u, 0u);
@@ -870,15 +866,11 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
     const int pieces = max((int)((lk + (int64_t)ss.chunk - 1) / ss.chunk), 1);
     // a sequence with more rows than the parts have room for is not split
     split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
-    if (index < 0 || index >= pieces || (index > 0 && !split)) {
-      if (SHARED && sp.slots == 0) wait_for_predecessor();
-      return;
-    }
+    if (index < 0 || index >= pieces || (index > 0 && !split)) return;
     k0 = split ? index * ss.chunk : 0, k1 = split ? min(k0 + ss.chunk, lk) : lk;
     causal = a.causal;
   }
   const int rows = lq * a.group;
-  bool waited = false;
 
   for (int r0 = blockIdx.z * R; r0 < rows; r0 += gridDim.z * R) {
     // Q^T: row g of each row tile, the columns that this thread loads of K.
@@ -915,7 +907,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
         for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     least = __reduce_min_sync(0xffffffffu, least);
 
-    for (int k = k0 + warp * kStepKeys; k < k1; k += kStepWarps * kStepKeys) {
+    for (int k = k0 + (warp - first_warp) * kStepKeys; k < k1; k += WARPS * kStepKeys) {
       // K: keys g, g + 8; V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, columns 8 g of each 64
       uint4 kr[2][D / 32], vr[4][D / 64];
 #pragma unroll
@@ -999,11 +991,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
     }
     allow_dependent();  // join_kernel looks its row up meanwhile
     // The warps' parts to shared memory, added in order.
-    __syncthreads();
-    if (SHARED && sp.slots == 0 && !waited) {
-      wait_for_predecessor();
-      waited = true;
-    }
+    if (kHeads == 1) __syncthreads(); else __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1022,30 +1010,30 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
           dst[1] = o[n][i][2 + e];
         }
       }
-    __syncthreads();
-    for (int r = warp; r < R && r0 + r < rows; r += kStepWarps) {
+    if (kHeads == 1) __syncthreads(); else __syncwarp();
+    for (int r = warp - first_warp; r < R && r0 + r < rows; r += WARPS) {
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sh_m[w][r]);
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sh_m[first_warp + w][r]);
       const float sub = top == -INFINITY ? 0.0f : top;
-      float f[kStepWarps], sum = 0.0f;
+      float f[WARPS], sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) {
-        f[w] = ex2(sh_m[w][r] - sub);
-        sum = fmaf(sh_l[w][r], f[w], sum);
+      for (int w = 0; w < WARPS; ++w) {
+        f[w] = ex2(sh_m[first_warp + w][r] - sub);
+        sum = fmaf(sh_l[first_warp + w][r], f[w], sum);
       }
       float y[D / 32];
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         y[c] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kStepWarps; ++w) y[c] = fmaf(sh_o[w][r][c * 32 + lane], f[w], y[c]);
+        for (int w = 0; w < WARPS; ++w) y[c] = fmaf(sh_o[first_warp + w][r][c * 32 + lane], f[w], y[c]);
       }
       const int row = r0 + r;
       if constexpr (SHARED) {
         const int64_t all = (int64_t)a.total_q * a.heads;
         const int64_t at = (int64_t)(qs + row / a.group) * a.heads + kv_head * a.group + row % a.group;
-        if (of_prefix || (!split && sp.slots > 0)) {
+        if (of_prefix || !split) {
           float* to = of_prefix ? sp.part_o + index * all * D : sp.own_o;
           float2* to_ml = of_prefix ? sp.part_ml + index * all : sp.own_ml;
 #pragma unroll
@@ -1053,7 +1041,6 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
           if (lane == 0) to_ml[at] = make_float2(top, sum);
           continue;
         }
-        if (!split) add_prefix<D>(sp, all, at, lane, top, sum, y);
       }
       if (split) {
         const int64_t at = ((first_part(ks, ss.chunk) + index) * a.kv_heads + kv_head) * ss.max_rows + row;
@@ -1062,7 +1049,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
         if (lane == 0) ss.part_ml[at] = make_float2(top, sum);
       } else {
         const int token = row / a.group;
-        const int seen = SHARED ? 1 : causal ? min(token + lk - lq + 1, lk) : lk;
+        const int seen = causal ? min(token + lk - lq + 1, lk) : lk;
         const float inv = 1.0f / sum;
         bf16* dst = a.out + ((int64_t)(qs + token) * a.heads + kv_head * a.group + row % a.group) * D;
 #pragma unroll
@@ -1070,16 +1057,12 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
       }
     }
   }
-  if (SHARED && sp.slots == 0 && !waited) wait_for_predecessor();  // a sequence without queries
 }
 
 // The parts of the sequences whose keys were split: a block a row, a thread a
 // column and every THREADS / D-th part; the groups' sums are added in order.
-//
-// SHARED: behind a prefix, whose parts are joined as well: for every row where
-// the step kernel made them, else for the sequences that were split.
-template <int D, int THREADS, bool SHARED>
-__global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepShape ss) {
   constexpr int kGroups = THREADS / D;
   __shared__ float sh_y[kGroups][D], sh_l[kGroups];
   const int lane = threadIdx.x & 31;
@@ -1097,41 +1080,27 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
   const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
   const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
   const int pieces = (int)((lk + (int64_t)ss.chunk - 1) / ss.chunk);
-  const bool split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
-  if (!(split || (SHARED && sp.slots > 0)) || tok < qs || tok >= qs + lq) {
+  if (pieces <= 1 || (int64_t)lq * a.group > ss.max_rows || tok < qs || tok >= qs + lq) {
     wait_for_predecessor();
     return;
   }
   const int row = (tok - qs) * a.group + head % a.group;
-  const int seen = SHARED ? 1 : a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
+  const int seen = a.causal ? min(tok - qs + lk - lq + 1, lk) : lk;
   const int64_t stride = (int64_t)a.kv_heads * ss.max_rows;
   const int64_t at = (first_part(ks, ss.chunk) * a.kv_heads + head / a.group) * ss.max_rows + row;
-  const int64_t all = (int64_t)a.total_q * a.heads;
-  // part p: the sequence's own, then the prefix's
-  const int own = split ? pieces : 1, parts = SHARED ? own + sp.chunks : own;
-  const auto part_ml = [&](int p) -> float2 {
-    if (SHARED && p >= own) return sp.part_ml[(p - own) * all + item];
-    if (SHARED && !split) return sp.own_ml[item];
-    return ss.part_ml[at + p * stride];
-  };
-  const auto part_o = [&](int p) -> float {
-    if (SHARED && p >= own) return sp.part_o[((p - own) * all + item) * D + col];
-    if (SHARED && !split) return sp.own_o[item * D + col];
-    return ss.part_o[(at + p * stride) * D + col];
-  };
   wait_for_predecessor();
   float top = -INFINITY;
-  for (int p = lane; p < parts; p += 32) top = fmaxf(top, part_ml(p).x);
+  for (int p = lane; p < pieces; p += 32) top = fmaxf(top, ss.part_ml[at + p * stride].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float sub = top == -INFINITY ? 0.0f : top;
   float y = 0.0f, sum = 0.0f;
 #pragma unroll 8
-  for (int p = group; p < parts; p += kGroups) {
-    const float2 ml = part_ml(p);
+  for (int p = group; p < pieces; p += kGroups) {
+    const float2 ml = ss.part_ml[at + p * stride];
     const float f = ex2(ml.x - sub);
     sum = fmaf(ml.y, f, sum);
-    y = fmaf(part_o(p), f, y);
+    y = fmaf(ss.part_o[(at + p * stride) * D + col], f, y);
   }
   sh_y[group][col] = y;
   if (col == 0) sh_l[group] = sum;
@@ -1143,6 +1112,63 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
     sum += sh_l[w];
   }
   a.out[item * D + col] = __float2bfloat16_rn(seen > 0 ? y * (1.0f / sum) : 0.0f);
+}
+
+// The parts of every row behind a prefix, the prefix's and then its sequence's
+// own, added in that order: a warp a row, D / 32 columns a lane.
+constexpr int kJoinRows = 8;
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinRows) join_prefix_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
+  using V = typename std::conditional<D == 128, float4, float2>::type;
+  constexpr int kEach = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t all = (int64_t)a.total_q * a.heads, item = (int64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
+  const int tok = (int)(min(item, all - 1) / a.heads), head = (int)(min(item, all - 1) % a.heads);
+  int b = 0, n = a.seqs;  // the last sequence that starts at or before the token
+  while (n > 1) {
+    const int stride = (n + 31) / 32, at = b + lane * stride;
+    const int hits = __popc(__ballot_sync(0xffffffffu, at < b + n && a.cu_q[at] <= tok));
+    const int step = max(hits - 1, 0) * stride;
+    n = min(stride, n - step);
+    b += step;
+  }
+  const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
+  const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
+  const int pieces = (int)((lk + (int64_t)ss.chunk - 1) / ss.chunk);
+  const bool split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
+  const int64_t at = (first_part(ks, ss.chunk) * a.kv_heads + head / a.group) * ss.max_rows + (tok - qs) * a.group + head % a.group;
+  const int64_t stride = split ? (int64_t)a.kv_heads * ss.max_rows : 0;
+  const float2* own_ml = split ? ss.part_ml + at : sp.own_ml + item;
+  const float* own_o = split ? ss.part_o + at * D : sp.own_o + item * D;
+  const int own = split ? pieces : 1, parts = sp.chunks + own;
+  wait_for_predecessor();
+  if (item >= all || tok < qs || tok >= qs + lq) return;  // tokens past the last offset have their zeros
+  const auto ml_of = [&](int p) { return p < sp.chunks ? sp.part_ml[p * all + item] : own_ml[(p - sp.chunks) * stride]; };
+  float top = -INFINITY;
+  for (int p = lane; p < parts; p += 32) top = fmaxf(top, ml_of(p).x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float sub = top == -INFINITY ? 0.0f : top;
+  float y[kEach], sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kEach; ++c) y[c] = 0.0f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = ml_of(p);
+    const float* o = p < sp.chunks ? sp.part_o + (p * all + item) * D : own_o + (p - sp.chunks) * stride * D;
+    const V v = reinterpret_cast<const V*>(o)[lane];
+    const float f = ex2(ml.x - sub);
+    sum = fmaf(ml.y, f, sum);
+    const float* x = reinterpret_cast<const float*>(&v);
+#pragma unroll
+    for (int c = 0; c < kEach; ++c) y[c] = fmaf(x[c], f, y[c]);
+  }
+  const float inv = 1.0f / sum;
+  uint32_t out[kEach / 2];
+#pragma unroll
+  for (int c = 0; c < kEach / 2; ++c) out[c] = cvt2(y[2 * c] * inv, y[2 * c + 1] * inv);
+  using W = typename std::conditional<D == 128, uint2, uint32_t>::type;
+  reinterpret_cast<W*>(a.out + item * D)[lane] = *reinterpret_cast<const W*>(out);
 }
 
 // ------------------------------------------------------------------ host
@@ -1225,20 +1251,31 @@ int launch_step(const Args& a, const Plan& p, const StepPrefix& sp, void* worksp
   const int most_rows = sp.slots > 0 && a.total_q * a.group > p.max_rows ? a.total_q * a.group : p.max_rows;
   const int nt = most_rows <= 8 ? 1 : 2;
   const dim3 grid((unsigned)(p.slots + sp.slots), (unsigned)a.kv_heads, (unsigned)((most_rows + 8 * nt - 1) / (8 * nt)));
-  const int st = launch(SHARED ? "attention_shared (steps)" : "attention_packed (steps)",
-                        nt == 1 ? step_kernel<D, 1, SHARED> : step_kernel<D, 2, SHARED>, grid, 32 * kStepWarps, 0, stream, 1,
-                        SHARED && sp.slots == 0, a, ss, sp);
-  if (st || (p.bytes == 0 && sp.slots == 0)) return st;
   const int64_t rows = (int64_t)a.total_q * a.heads;
-  LR_REQUIRE(rows <= INT32_MAX, "attention_packed: too many rows");
+  LR_REQUIRE(rows <= INT32_MAX, "attention: too many rows");
+  const StepPrefix none{};
+  if constexpr (SHARED) {
+    // one warp a head where that fills the GPU's 16 warps an SM
+    const bool narrow = (int64_t)p.slots * a.kv_heads >= 16 * sm_count();
+    dim3 all = grid;
+    all.x += 1;  // the block that waits for prompt_kernel
+    if (narrow) all.y = (unsigned)((a.kv_heads + kStepWarps - 1) / kStepWarps);
+    const auto kernel = nt == 1 ? (narrow ? step_kernel<D, 1, 1, true> : step_kernel<D, 1, kStepWarps, true>)
+                                : (narrow ? step_kernel<D, 2, 1, true> : step_kernel<D, 2, kStepWarps, true>);
+    const int st = launch("attention_shared (steps)", kernel, all, 32 * kStepWarps, 0, stream, 1, sp.slots == 0, a, ss, sp);
+    if (st) return st;
+    return launch("attention_shared (join)", join_prefix_kernel<D>, dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)),
+                  32 * kJoinRows, 0, stream, 1, true, a, ss, sp);
+  }
+  const int st = launch("attention_packed (steps)", nt == 1 ? step_kernel<D, 1, kStepWarps, false> : step_kernel<D, 2, kStepWarps, false>,
+                        grid, 32 * kStepWarps, 0, stream, 1, false, a, ss, none);
+  if (st || p.bytes == 0) return st;
   // a thread takes about eight parts at most: one token against 32768 keys 33.8 us with 256 threads, 30.2 us with 512
   // (64 requests of a few parts each, 139 us, lose 5 us to the larger blocks)
-  const int parts_each = p.slots / a.seqs + sp.chunks;
-  const auto join =
-      parts_each > 32 ? join_kernel<D, 1024, SHARED> : parts_each > 8 ? join_kernel<D, 512, SHARED> : join_kernel<D, 128, SHARED>;
+  const int parts_each = p.slots / a.seqs;
+  const auto join = parts_each > 32 ? join_kernel<D, 1024> : parts_each > 8 ? join_kernel<D, 512> : join_kernel<D, 128>;
   const unsigned threads = parts_each > 32 ? 1024 : parts_each > 8 ? 512 : 128;
-  return launch(SHARED ? "attention_shared (join)" : "attention_packed (join)", join, dim3((unsigned)rows), threads, 0, stream, 1,
-                true, a, ss, sp);
+  return launch("attention_packed (join)", join, dim3((unsigned)rows), threads, 0, stream, 1, true, a, ss);
 }
 
 // How a call behind a prefix is laid out.
@@ -1264,7 +1301,13 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
   } else {
     const int64_t head_parts = (group + kRows - 1) / kRows, tile_heads = (group + head_parts - 1) / head_parts;
     const int64_t tokens = 2 * (kRows / tile_heads);
-    want = sm_count() / ((total_q + tokens - 1) / tokens * kv_heads * head_parts);
+    const int64_t blocks = (total_q + tokens - 1) / tokens * kv_heads * head_parts, tiles = (prefix + kKeys - 1) / kKeys;
+    // step_kernel runs on the SMs that this leaves, and on all of them afterwards: the parts should end when both together
+    // would, a key tile taking about 2.2 us and a block 8 more, and the sequences' own keys going by at 6 TB/s.
+    const double together = blocks * tiles * 2.2 / sm_count() + (double)total_k * kv_heads * head_dim * 4 / 6e6;
+    const int64_t each = together > 8 + 2.2 ? (int64_t)((together - 8) / 2.2) : 1;
+    want = (tiles + each - 1) / each;
+    if (want > sm_count() / blocks) want = sm_count() / blocks;
     p.chunk = kKeys;
   }
   if (want < 1) want = 1;
@@ -1274,7 +1317,7 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
   const int64_t row_bytes = (head_dim + 2) * 4, all = total_q * group * kv_heads;
   p.own_at = p.prefix_at + p.chunks * all * row_bytes;
   p.own_at = (p.own_at + 31) / 32 * 32;
-  p.bytes = p.own_at + (p.step ? all * row_bytes : 0);
+  p.bytes = p.own_at + all * row_bytes;
   return p;
 }
 
