@@ -47,17 +47,18 @@ def _check_stack(name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.T
         if t.dtype != torch.bfloat16 or t.ndim != 3:
             raise ValueError(f"{name}: {what} must be a bf16 tensor of three dimensions, got {t.dtype} {tuple(t.shape)}")
     count, rank, width = down.shape
-    if up.shape[0] != count or up.shape[2] != rank or up.device != down.device:
+    up_count, outputs, up_rank = up.shape
+    if up_count != count or up_rank != rank or up.get_device() != down.get_device():
         raise ValueError(f"{name}: down [adapters, rank, in] and up [adapters, out, rank] disagree: {tuple(down.shape)}, {tuple(up.shape)}")
-    if count == 0 or width == 0 or up.shape[1] == 0:
+    if count == 0 or width == 0 or outputs == 0:
         raise ValueError(f"{name}: no adapters, or empty ones")
     if rank == 0 or rank % 8 or rank > MOST_RANK:
         raise ValueError(f"{name}: the rank must be a multiple of 8 up to {MOST_RANK} (pad with zeros), got {rank}")
     if width % 8:
         raise ValueError(f"{name}: the input width must be a multiple of 8, got {width}")
-    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count or scale.device != down.device):
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count or scale.get_device() != down.get_device()):
         raise ValueError(f"{name}: scale must hold {count} fp32 values on the adapters' device")
-    return count, rank, width, up.shape[1]
+    return count, rank, width, outputs
 
 
 def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
@@ -70,32 +71,38 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     Any order will do, tokens of one adapter side by side are fastest. ``out`` may be ``base`` itself; it must not overlap
     x, nor base in any other way."""
     count, rank, width, outputs = _check_stack("add_adapters", down, up, scale)
-    device = down.device
+    device = down.get_device()
     for what, t, columns in (("base", base, outputs), ("x", x, width)):
-        if t.dtype != torch.bfloat16 or t.ndim != 2 or t.shape[1] != columns or t.device != device:
+        if t.dtype != torch.bfloat16 or t.ndim != 2 or t.shape[1] != columns or t.get_device() != device:
             raise ValueError(f"add_adapters: {what} must be a bf16 [tokens, {columns}] tensor on the adapters' device, "
                              f"got {t.dtype} {tuple(t.shape)}")
     tokens = x.shape[0]
     if base.shape[0] != tokens:
         raise ValueError(f"add_adapters: base and x differ in tokens: {base.shape[0]}, {tokens}")
-    if index.dtype != torch.int32 or index.shape != (tokens,) or index.device != device:
+    if index.dtype != torch.int32 or index.ndim != 1 or index.shape[0] != tokens or index.get_device() != device:
         raise ValueError("add_adapters: index must be int32 [tokens] on the adapters' device")
+    if device < 0:
+        raise ValueError("add_adapters: expected CUDA tensors")
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return add_adapters(base, x, down, up, index, scale, out=out)
     if out is None:
-        out = torch.empty(tokens, outputs, dtype=torch.bfloat16, device=device)
-    elif (out.dtype != torch.bfloat16 or out.shape != base.shape or out.device != device or out.stride(1) != 1
+        out = torch.empty_like(base, memory_format=torch.contiguous_format)
+    elif (out.dtype != torch.bfloat16 or out.shape != base.shape or out.get_device() != device or out.stride(1) != 1
           or (tokens > 1 and out.stride(0) < outputs)):
         raise ValueError("add_adapters: out must be a bf16 tensor of base's shape with contiguous rows that do not overlap")
     down, up, index = down.contiguous(), up.contiguous(), index.contiguous()
     if scale is not None:
         scale = scale.contiguous()
-    if base.stride(1) != 1 or base.stride(0) < 0:
-        base = base.contiguous()
-    x_stride = x.stride(0)
-    if x.stride(1) != 1 or x_stride % 8 or x_stride < width or x.data_ptr() % 16:
+    base_stride, one = base.stride()
+    if one != 1:
+        base, base_stride = base.contiguous(), outputs
+    x_stride, one = x.stride()
+    if one != 1 or x_stride % 8 or x_stride < width or x.data_ptr() % 16:
         x, x_stride = x.clone(memory_format=torch.contiguous_format), width
-    need = _workspace_bytes(down.get_device(), tokens, width, outputs, rank, count) if down.is_cuda else 0
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    check(_lib.load().lr_adapters(x.data_ptr(), x_stride, base.data_ptr(), base.stride(0), down.data_ptr(), up.data_ptr(),
+    need = _workspace_bytes(device, tokens, width, outputs, rank, count)
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(_lib.load().lr_adapters(x.data_ptr(), x_stride, base.data_ptr(), base_stride, down.data_ptr(), up.data_ptr(),
                                   ptr(scale), index.data_ptr(), tokens, width, outputs, rank, count, out.data_ptr(),
                                   max(out.stride(0), outputs), ptr(workspace), need, stream_of(x)), "add_adapters")
     return out

@@ -800,6 +800,44 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// The last sequence of which before(its first key, its first query, its number) holds, with both its ranges. One round of
+// loads, four candidates a lane, up to 127 sequences, two up to 2047.
+struct Ranges {
+  int ks, ke, qs, qe, b;
+};
+template <typename Before>
+__device__ __forceinline__ Ranges find_ranges(const Args& a, int lane, Before before) {
+  const auto key = [&](int i) { return clamped(a.cu_k, min(i, a.seqs), a.total_k); };
+  const auto query = [&](int i) { return clamped(a.cu_q, min(i, a.seqs), a.total_q); };
+  int lo = 0;
+  if (a.seqs > 127) {
+    int64_t stride = 64;  // the answer lies in [lo, lo + 32 stride)
+    while (32 * stride < a.seqs) stride *= 32;
+    for (;; stride /= 32) {
+      const int64_t at = lo + lane * stride;
+      const bool there = at < a.seqs;
+      const int i = there ? (int)at : 0;
+      const int hits = __popc(__ballot_sync(0xffffffffu, there && before(key(i), query(i), i)));
+      lo += max(hits - 1, 0) * (int)stride;
+      if (stride == 64) break;
+    }
+  }
+  int k[4], q[4], hits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = key(lo + 32 * i + lane), q[i] = query(lo + 32 * i + lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = lo + 32 * i + lane;
+    hits += __popc(__ballot_sync(0xffffffffu, at < a.seqs && before(k[i], q[i], at)));
+  }
+  const int b = min(max(hits - 1, 0), 126);  // as many hold where offsets do not go down
+  const auto pick = [&](const int(&v)[4], int at) {
+    const int i = at >> 5;
+    return __shfl_sync(0xffffffffu, i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3], at & 31);
+  };
+  return Ranges{pick(k, b), pick(k, b + 1), pick(q, b), pick(q, b + 1), lo + b};
+}
+
 // What a prefix in front of every sequence adds to the step kernel.
 struct StepPrefix {
   const bf16 *k, *v;
@@ -823,9 +861,11 @@ struct StepPrefix {
 // the GPU: a block is then that many heads side by side, and no warp waits for
 // another.
 template <int D, int NT, int WARPS, bool SHARED>
-__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
+__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (WARPS == 1 && D == 64 ? 3 : 4) : 2) step_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   constexpr int R = 8 * NT;
   constexpr int kHeads = kStepWarps / WARPS;
+  // Steps whose keys are under way together: 64 columns are half as many bytes, and a warp alone has no other to wait with.
+  constexpr int kUnder = WARPS == 1 && D == 64 && NT == 1 ? 2 : 1;
   __shared__ float sh_m[kStepWarps][R], sh_l[kStepWarps][R];
   __shared__ float sh_o[kStepWarps][R][D + 4];
   if (SHARED && blockIdx.x == gridDim.x - 1) {
@@ -859,9 +899,15 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
     k0 = index * sp.chunk;
     k1 = min(k0 + sp.chunk, lk);
   } else {
-    const int b = find_sequence(a.cu_k, a.seqs - 1, a.total_k, ss.chunk, slot, lane);
-    ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
-    qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
+    int b;
+    if constexpr (SHARED) {
+      const Ranges r = find_ranges(a, lane, [&](int k, int, int at) { return (int)((uint32_t)k / (uint32_t)ss.chunk) + at <= slot; });
+      b = r.b, ks = r.ks, lk = max(r.ke - ks, 0), qs = r.qs, lq = max(r.qe - qs, 0);
+    } else {
+      b = find_sequence(a.cu_k, a.seqs - 1, a.total_k, ss.chunk, slot, lane);
+      ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
+      qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
+    }
     index = slot - (int)((uint32_t)ks / (uint32_t)ss.chunk) - b;
     const int pieces = max((int)((lk + (int64_t)ss.chunk - 1) / ss.chunk), 1);
     // a sequence with more rows than the parts have room for is not split
@@ -907,85 +953,94 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) step_kernel(
         for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     least = __reduce_min_sync(0xffffffffu, least);
 
-    for (int k = k0 + (warp - first_warp) * kStepKeys; k < k1; k += WARPS * kStepKeys) {
+    for (int kk = k0 + (warp - first_warp) * kStepKeys; kk < k1; kk += kUnder * WARPS * kStepKeys) {
       // K: keys g, g + 8; V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, columns 8 g of each 64
-      uint4 kr[2][D / 32], vr[4][D / 64];
+      uint4 kr[kUnder][2][D / 32], vr[kUnder][4][D / 64];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bf16* src = keys + (int64_t)(ks + min(k + g + 8 * h, k1 - 1)) * k_ts + (int64_t)kv_head * k_hs + t * 8;
+      for (int u = 0; u < kUnder; ++u) {
+        const int k = kk + u * WARPS * kStepKeys;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) kr[h][c] = ld_stream(src + c * 32);
-      }
+        for (int h = 0; h < 2; ++h) {
+          const bf16* src = keys + (int64_t)(ks + min(k + g + 8 * h, k1 - 1)) * k_ts + (int64_t)kv_head * k_hs + t * 8;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int key = k + 2 * t + (h & 1) + (h >> 1) * 8;
-        const bf16* src = values + (int64_t)(ks + min(key, k1 - 1)) * v_ts + (int64_t)kv_head * v_hs + g * 8;
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          vr[h][c] = ld_stream(src + c * 64);
-          if (key >= k1) vr[h][c] = make_uint4(0u, 0u, 0u, 0u);
+          for (int c = 0; c < D / 32; ++c) kr[u][h][c] = ld_stream(src + c * 32);
         }
-      }
-      uint32_t pb[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < 4; ++h) {
+          const int key = k + 2 * t + (h & 1) + (h >> 1) * 8;
+          const bf16* src = values + (int64_t)(ks + min(key, k1 - 1)) * v_ts + (int64_t)kv_head * v_hs + g * 8;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          mma_16816(s, kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, q[n][c][0], q[n][c][1]);
-          mma_16816(s, kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, q[n][c][2], q[n][c][3]);
-        }
-        // s[e], s[2 + e]: keys k + g, k + g + 8 of row 2 t + e
-        const bool masked = k + kStepKeys > least;
-        float top[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[e] *= a.scale_log2;
-          s[2 + e] *= a.scale_log2;
-          if (masked && k + g >= see[n][e]) s[e] = -INFINITY;
-          if (masked && k + g + 8 >= see[n][e]) s[2 + e] = -INFINITY;
-          top[e] = fmaxf(s[e], s[2 + e]);
-        }
-        // as above: the maximum moves when it would grow by more than 2^8
-        if (__any_sync(0xffffffffu, top[0] > m[n][0] + 8.0f || top[1] > m[n][1] + 8.0f)) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], off));
-            const float mn = fmaxf(m[n][e], top[e]);
-            const float alpha = mn == -INFINITY ? 1.0f : ex2(m[n][e] - mn);
-            m[n][e] = mn;
-            l[n][e] *= alpha;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              o[n][i][e] *= alpha;
-              o[n][i][2 + e] *= alpha;
-            }
+          for (int c = 0; c < D / 64; ++c) {
+            vr[u][h][c] = ld_stream(src + c * 64);
+            if (key >= k1) vr[u][h][c] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float sub = m[n][e] == -INFINITY ? 0.0f : m[n][e];
-          s[e] = ex2(s[e] - sub);
-          s[2 + e] = ex2(s[2 + e] - sub);
-          l[n][e] += s[e] + s[2 + e];
-        }
-        pb[n][0] = transpose8x8(cvt2(s[0], s[1]));
-        pb[n][1] = transpose8x8(cvt2(s[2], s[3]));
       }
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const uint32_t v0[4] = {vr[0][c].x, vr[0][c].y, vr[0][c].z, vr[0][c].w};
-        const uint32_t v1[4] = {vr[1][c].x, vr[1][c].y, vr[1][c].z, vr[1][c].w};
-        const uint32_t v2[4] = {vr[2][c].x, vr[2][c].y, vr[2][c].z, vr[2][c].w};
-        const uint32_t v3[4] = {vr[3][c].x, vr[3][c].y, vr[3][c].z, vr[3][c].w};
+      for (int u = 0; u < kUnder; ++u) {
+        const int k = kk + u * WARPS * kStepKeys;
+        if (u > 0 && k >= k1) break;
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // output rows g and g + 8 of the MMA are columns 8 g + 2 i and + 1
-          const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
-          const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
+        for (int n = 0; n < NT; ++n) {
+          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816(o[n][c * 4 + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          for (int c = 0; c < D / 32; ++c) {
+            mma_16816(s, kr[u][0][c].x, kr[u][1][c].x, kr[u][0][c].y, kr[u][1][c].y, q[n][c][0], q[n][c][1]);
+            mma_16816(s, kr[u][0][c].z, kr[u][1][c].z, kr[u][0][c].w, kr[u][1][c].w, q[n][c][2], q[n][c][3]);
+          }
+          // s[e], s[2 + e]: keys k + g, k + g + 8 of row 2 t + e
+          const bool masked = k + kStepKeys > least;
+          float top[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[e] *= a.scale_log2;
+            s[2 + e] *= a.scale_log2;
+            if (masked && k + g >= see[n][e]) s[e] = -INFINITY;
+            if (masked && k + g + 8 >= see[n][e]) s[2 + e] = -INFINITY;
+            top[e] = fmaxf(s[e], s[2 + e]);
+          }
+          // as above: the maximum moves when it would grow by more than 2^8
+          if (__any_sync(0xffffffffu, top[0] > m[n][0] + 8.0f || top[1] > m[n][1] + 8.0f)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], off));
+              const float mn = fmaxf(m[n][e], top[e]);
+              const float alpha = mn == -INFINITY ? 1.0f : ex2(m[n][e] - mn);
+              m[n][e] = mn;
+              l[n][e] *= alpha;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                o[n][i][e] *= alpha;
+                o[n][i][2 + e] *= alpha;
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float sub = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+            s[e] = ex2(s[e] - sub);
+            s[2 + e] = ex2(s[2 + e] - sub);
+            l[n][e] += s[e] + s[2 + e];
+          }
+          pb[n][0] = transpose8x8(cvt2(s[0], s[1]));
+          pb[n][1] = transpose8x8(cvt2(s[2], s[3]));
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint32_t v0[4] = {vr[u][0][c].x, vr[u][0][c].y, vr[u][0][c].z, vr[u][0][c].w};
+          const uint32_t v1[4] = {vr[u][1][c].x, vr[u][1][c].y, vr[u][1][c].z, vr[u][1][c].w};
+          const uint32_t v2[4] = {vr[u][2][c].x, vr[u][2][c].y, vr[u][2][c].z, vr[u][2][c].w};
+          const uint32_t v3[4] = {vr[u][3][c].x, vr[u][3][c].y, vr[u][3][c].z, vr[u][3][c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // output rows g and g + 8 of the MMA are columns 8 g + 2 i and + 1
+            const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410), a1 = __byte_perm(v0[i], v1[i], 0x7632);
+            const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410), a3 = __byte_perm(v2[i], v3[i], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(o[n][c * 4 + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
         }
       }
     }
@@ -1120,20 +1175,12 @@ constexpr int kJoinRows = 8;
 template <int D>
 __global__ void __launch_bounds__(32 * kJoinRows) join_prefix_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   using V = typename std::conditional<D == 128, float4, float2>::type;
-  constexpr int kEach = D / 32;
+  constexpr int kEach = D / 32, kAhead = 16;  // parts whose values are under way together
   const int lane = threadIdx.x & 31;
   const int64_t all = (int64_t)a.total_q * a.heads, item = (int64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
   const int tok = (int)(min(item, all - 1) / a.heads), head = (int)(min(item, all - 1) % a.heads);
-  int b = 0, n = a.seqs;  // the last sequence that starts at or before the token
-  while (n > 1) {
-    const int stride = (n + 31) / 32, at = b + lane * stride;
-    const int hits = __popc(__ballot_sync(0xffffffffu, at < b + n && a.cu_q[at] <= tok));
-    const int step = max(hits - 1, 0) * stride;
-    n = min(stride, n - step);
-    b += step;
-  }
-  const int qs = clamped(a.cu_q, b, a.total_q), lq = max(clamped(a.cu_q, b + 1, a.total_q) - qs, 0);
-  const int ks = clamped(a.cu_k, b, a.total_k), lk = max(clamped(a.cu_k, b + 1, a.total_k) - ks, 0);
+  const Ranges r = find_ranges(a, lane, [&](int, int q, int) { return q <= tok; });
+  const int qs = r.qs, lq = max(r.qe - qs, 0), ks = r.ks, lk = max(r.ke - ks, 0);
   const int pieces = (int)((lk + (int64_t)ss.chunk - 1) / ss.chunk);
   const bool split = pieces > 1 && (int64_t)lq * a.group <= ss.max_rows;
   const int64_t at = (first_part(ks, ss.chunk) * a.kv_heads + head / a.group) * ss.max_rows + (tok - qs) * a.group + head % a.group;
@@ -1143,25 +1190,42 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_prefix_kernel(const Args 
   const int own = split ? pieces : 1, parts = sp.chunks + own;
   wait_for_predecessor();
   if (item >= all || tok < qs || tok >= qs + lq) return;  // tokens past the last offset have their zeros
-  const auto ml_of = [&](int p) { return p < sp.chunks ? sp.part_ml[p * all + item] : own_ml[(p - sp.chunks) * stride]; };
-  float top = -INFINITY;
-  for (int p = lane; p < parts; p += 32) top = fmaxf(top, ml_of(p).x);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const float sub = top == -INFINITY ? 0.0f : top;
-  float y[kEach], sum = 0.0f;
+  float top = -INFINITY, sum = 0.0f, y[kEach];
 #pragma unroll
   for (int c = 0; c < kEach; ++c) y[c] = 0.0f;
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = ml_of(p);
-    const float* o = p < sp.chunks ? sp.part_o + (p * all + item) * D : own_o + (p - sp.chunks) * stride * D;
-    const V v = reinterpret_cast<const V*>(o)[lane];
-    const float f = ex2(ml.x - sub);
-    sum = fmaf(ml.y, f, sum);
-    const float* x = reinterpret_cast<const float*>(&v);
+  // 32 parts at a time: a lane has one's maximum and sum
+  for (int p0 = 0; p0 < parts; p0 += 32) {
+    const int here = min(parts - p0, 32), mine = p0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (mine < parts) ml = mine < sp.chunks ? sp.part_ml[mine * all + item] : own_ml[(mine - sp.chunks) * stride];
+    V v[kAhead];
+    const auto value = [&](int p) {
+      const float* o = p < sp.chunks ? sp.part_o + (p * all + item) * D : own_o + (p - sp.chunks) * stride * D;
+      return reinterpret_cast<const V*>(o)[lane];
+    };
 #pragma unroll
-    for (int c = 0; c < kEach; ++c) y[c] = fmaf(x[c], f, y[c]);
+    for (int i = 0; i < kAhead; ++i)
+      if (i < here) v[i] = value(p0 + i);
+    float most = fmaxf(top, ml.x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    const float sub = most == -INFINITY ? 0.0f : most, again = ex2(top - sub), weight = ex2(ml.x - sub);
+    sum *= again;
+#pragma unroll
+    for (int c = 0; c < kEach; ++c) y[c] *= again;
+    top = most;
+    for (int p = 0; p < here; p += kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (p + i >= here) break;
+        const float f = __shfl_sync(0xffffffffu, weight, p + i);
+        sum = fmaf(__shfl_sync(0xffffffffu, ml.y, p + i), f, sum);
+        const float* x = reinterpret_cast<const float*>(&v[i]);
+#pragma unroll
+        for (int c = 0; c < kEach; ++c) y[c] = fmaf(x[c], f, y[c]);
+        if (p + i + kAhead < here) v[i] = value(p0 + p + i + kAhead);
+      }
+    }
   }
   const float inv = 1.0f / sum;
   uint32_t out[kEach / 2];
@@ -1175,11 +1239,12 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_prefix_kernel(const Args 
 // How a call is laid out, from what the host knows: token and sequence counts.
 struct Plan {
   bool step;
+  bool narrow;  // one warp to a slot and head
   int chunk, slots, max_rows;
   int64_t parts;  // room for parts, 0 where no sequence can be long enough to be split
   int64_t bytes;  // of workspace
 };
-Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t kv_heads, int64_t head_dim) {
+Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t kv_heads, int64_t head_dim, bool shared = false) {
   Plan p{};
   const int64_t queries = (total_q + seqs - 1) / seqs;  // a sequence, on average
   p.step = queries * group <= 64;
@@ -1191,6 +1256,10 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   // Shorter pieces cost more at the join than they save; up to 512 keys none is made (300 keys: one kernel takes 6.8 us, two
   // 7.7; 1000 keys in pieces of 256, 512, 1024: 9.1, 11.7, 16.1 us).
   if (chunk < 256) chunk = total_k <= 512 ? 512 : 256;
+  // Behind a prefix, where a warp takes a slot and head alone, 128 keys (64 requests of 64 to 1024 own keys: 35.5 us, 41.8 with
+  // 256; four warps a slot 41.5 and 38.5).
+  p.narrow = shared && (total_k / 128 + seqs) * kv_heads >= 8 * sm_count();
+  if (p.narrow && total_k < (1 << 23)) chunk = 128;
   p.chunk = (int)chunk;
   p.slots = (int)(total_k / chunk + seqs);
   int64_t most = 1;
@@ -1255,13 +1324,11 @@ int launch_step(const Args& a, const Plan& p, const StepPrefix& sp, void* worksp
   LR_REQUIRE(rows <= INT32_MAX, "attention: too many rows");
   const StepPrefix none{};
   if constexpr (SHARED) {
-    // one warp a head where that fills the GPU's 16 warps an SM
-    const bool narrow = (int64_t)p.slots * a.kv_heads >= 16 * sm_count();
     dim3 all = grid;
     all.x += 1;  // the block that waits for prompt_kernel
-    if (narrow) all.y = (unsigned)((a.kv_heads + kStepWarps - 1) / kStepWarps);
-    const auto kernel = nt == 1 ? (narrow ? step_kernel<D, 1, 1, true> : step_kernel<D, 1, kStepWarps, true>)
-                                : (narrow ? step_kernel<D, 2, 1, true> : step_kernel<D, 2, kStepWarps, true>);
+    if (p.narrow) all.y = (unsigned)((a.kv_heads + kStepWarps - 1) / kStepWarps);
+    const auto kernel = nt == 1 ? (p.narrow ? step_kernel<D, 1, 1, true> : step_kernel<D, 1, kStepWarps, true>)
+                                : (p.narrow ? step_kernel<D, 2, 1, true> : step_kernel<D, 2, kStepWarps, true>);
     const int st = launch("attention_shared (steps)", kernel, all, 32 * kStepWarps, 0, stream, 1, sp.slots == 0, a, ss, sp);
     if (st) return st;
     return launch("attention_shared (join)", join_prefix_kernel<D>, dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)),
@@ -1289,7 +1356,7 @@ struct SharedPlan {
 SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t prefix, int64_t group, int64_t kv_heads,
                        int64_t head_dim) {
   SharedPlan p{};
-  p.own = plan(seqs, total_q, total_k, group, kv_heads, head_dim);
+  p.own = plan(seqs, total_q, total_k, group, kv_heads, head_dim, true);
   p.parts = p.own.step;
   if (!p.parts) return p;
   const int64_t rows = total_q * group;
@@ -1303,9 +1370,9 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
     const int64_t tokens = 2 * (kRows / tile_heads);
     const int64_t blocks = (total_q + tokens - 1) / tokens * kv_heads * head_parts, tiles = (prefix + kKeys - 1) / kKeys;
     // step_kernel runs on the SMs that this leaves, and on all of them afterwards: the parts should end when both together
-    // would, a key tile taking about 2.2 us and a block 8 more, and the sequences' own keys going by at 6 TB/s.
-    const double together = blocks * tiles * 2.2 / sm_count() + (double)total_k * kv_heads * head_dim * 4 / 6e6;
-    const int64_t each = together > 8 + 2.2 ? (int64_t)((together - 8) / 2.2) : 1;
+    // would, a key tile taking about 1.65 us and a block 8 more, and the sequences' own keys going by at 4.5 TB/s.
+    const double together = blocks * tiles * 1.65 / sm_count() + (double)total_k * kv_heads * head_dim * 4 / 4.5e6;
+    const int64_t each = together > 8 + 1.65 ? (int64_t)((together - 8) / 1.65) + 1 : 1;
     want = (tiles + each - 1) / each;
     if (want > sm_count() / blocks) want = sm_count() / blocks;
     p.chunk = kKeys;
