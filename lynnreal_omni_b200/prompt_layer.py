@@ -10,6 +10,18 @@ residual. Norms, SwiGLU and residuals are the kernels of the W8A8 path.
     plan = pack([len(p) for p in prompts], "cuda")    # offsets and positions, made once for all layers
     for layer in layers:
         x = layer(x, plan, inv_freq, factor)
+
+Prompts that all continue one text (an instruction, a template) share its keys and values, and each request may have
+low-rank adapters of its own on the projections (``AdaptedLinear`` in place of ``Fp4Linear``):
+
+    prefixes = []
+    for layer in layers:                              # once for all batches behind this text
+        t, kv = layer.read_prefix(t, inv_freq, factor)
+        prefixes.append(kv)
+    plan = pack([len(p) for p in prompts], "cuda", start=len(text))
+    index = token_adapters(adapter_of_each_prompt, [len(p) for p in prompts], "cuda")
+    for layer, kv in zip(layers, prefixes):
+        x = layer(x, plan, inv_freq, factor, prefix=kv, index=index)
 """
 from __future__ import annotations
 
@@ -19,7 +31,8 @@ from typing import NamedTuple
 import torch
 
 from . import kernels as K
-from .attention import attention_packed
+from .adapters import AdaptedLinear
+from .attention import attention_packed, attention_shared
 from .fp4 import Fp4Linear
 from .rotary import rope
 
@@ -28,22 +41,25 @@ __all__ = ["PackedPrompts", "pack", "PromptLayer"]
 
 class PackedPrompts(NamedTuple):
     cu_seqlens: torch.Tensor  # int32 [prompts + 1]
-    positions: torch.Tensor   # int32 [tokens], from 0 in each prompt
+    positions: torch.Tensor   # int32 [tokens], from `start` in each prompt
 
 
-def pack(lengths, device="cuda") -> PackedPrompts:
-    """Offsets and positions of prompts of these lengths, one after another."""
+def pack(lengths, device="cuda", *, start: int = 0) -> PackedPrompts:
+    """Offsets and positions of prompts of these lengths, one after another; ``start``: the first token's position in
+    each (the length of a shared prefix)."""
     if not lengths or min(lengths) < 0:
         raise ValueError("pack: expected the lengths of one or more prompts")
+    if start < 0:
+        raise ValueError("pack: start must not be negative")
     n = torch.tensor(lengths, dtype=torch.int64)
     cu = torch.cat((torch.zeros(1, dtype=torch.int64), n.cumsum(0)))
-    positions = torch.arange(int(cu[-1])) - torch.repeat_interleave(cu[:-1], n)
+    positions = torch.arange(int(cu[-1])) - torch.repeat_interleave(cu[:-1], n) + start
     return PackedPrompts(cu.to(device=device, dtype=torch.int32), positions.to(device=device, dtype=torch.int32))
 
 
 class PromptLayer:
-    """One layer. qkv, out, gate_up, down: ``Fp4Linear``; norm weights bf16 [hidden]; ``gate_up`` gives the SwiGLU's
-    value and gate halves side by side as ``kernels._swiglu`` takes them."""
+    """One layer. qkv, out, gate_up, down: ``Fp4Linear``, or ``AdaptedLinear`` on one; norm weights bf16 [hidden];
+    ``gate_up`` gives the SwiGLU's value and gate halves side by side as ``kernels._swiglu`` takes them."""
 
     def __init__(self, qkv: Fp4Linear, out: Fp4Linear, gate_up: Fp4Linear, down: Fp4Linear, norm1: torch.Tensor,
                  norm2: torch.Tensor, *, heads: int, kv_heads: int, eps: float = 1e-6):
@@ -72,13 +88,36 @@ class PromptLayer:
         return cls(linear((heads + 2 * kv_heads) * head_dim, hidden), linear(hidden, heads * head_dim),
                    linear(2 * inner, hidden), linear(hidden, inner), norm(), norm(), heads=heads, kv_heads=kv_heads)
 
-    def __call__(self, x: torch.Tensor, prompts: PackedPrompts, inv_freq: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
-        """bf16 [tokens, hidden] -> the same."""
+    def __call__(self, x: torch.Tensor, prompts: PackedPrompts, inv_freq: torch.Tensor, factor: float = 1.0, *, prefix=None,
+                 index: torch.Tensor | None = None) -> torch.Tensor:
+        """bf16 [tokens, hidden] -> the same. prefix: the (keys, values) that ``read_prefix`` gave, in front of every prompt;
+        index: int32 [tokens], each token's adapter on the ``AdaptedLinear`` projections (None: they go without)."""
+        cu = prompts.cu_seqlens
+        if prefix is None:
+            return self._run(x, prompts.positions, inv_freq, factor, lambda q, k, v: attention_packed(q, k, v, cu), index)
+        return self._run(x, prompts.positions, inv_freq, factor, lambda q, k, v: attention_shared(q, k, v, *prefix, cu), index)
+
+    def read_prefix(self, x: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0):
+        """One text on its own, without adapters: bf16 [tokens, hidden] -> (the same for the next layer, (keys, values) bf16
+        [tokens, kv_heads, D] for the prompts that continue it)."""
+        kept = []
+
+        def attend(q, k, v):
+            kept.extend((k, v.contiguous()))  # rope's keys are a tensor of their own; the values a view of the projection
+            return attention_packed(q, k, v, prompts.cu_seqlens)
+
+        prompts = pack([x.shape[0]], x.device)
+        return self._run(x, prompts.positions, inv_freq, factor, attend, None), tuple(kept)
+
+    def _run(self, x, positions, inv_freq, factor, attend, index):
+        def project(linear, rows):
+            return linear(rows, index) if isinstance(linear, AdaptedLinear) else linear(rows)
+
         h, hk, d = self.heads, self.kv_heads, self.head_dim
-        qkv = self.qkv(K._rms_adaln(x, self.norm1, None, None, 0, 0))
+        qkv = project(self.qkv, K._rms_adaln(x, self.norm1, None, None, 0, 0))
         q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split([h * d, hk * d, hk * d], 1))
-        q, k = rope(q, k, prompts.positions, inv_freq, factor=factor)
-        context = attention_packed(q, k, v, prompts.cu_seqlens)
-        x = K._gated_residual(x, self.out(context.flatten(1)), None, None, 0)
-        inner = K._swiglu(self.gate_up(K._rms_adaln(x, self.norm2, None, None, 0, 0)))
-        return K._gated_residual(x, self.down(inner), None, None, 0)
+        q, k = rope(q, k, positions, inv_freq, factor=factor)
+        context = attend(q, k, v)
+        x = K._gated_residual(x, project(self.out, context.flatten(1)), None, None, 0)
+        inner = K._swiglu(project(self.gate_up, K._rms_adaln(x, self.norm2, None, None, 0, 0)))
+        return K._gated_residual(x, project(self.down, inner), None, None, 0)
