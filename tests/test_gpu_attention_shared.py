@@ -97,6 +97,25 @@ def test_many_sequences(seqs):
     check(300, lengths, lengths, 2, 1, 64, seed=seqs)
 
 
+@pytest.mark.parametrize("seqs", [127, 128, 129, 2047, 2048, 2049, 66000])
+def test_very_many_sequences(seqs):
+    """One token and, for two sequences of three, one own key each: every round of the look-up of a slot and a token."""
+    g = torch.Generator().manual_seed(seqs)
+    lk = torch.tensor([0 if i % 3 == 1 else 1 for i in range(seqs)])
+    q, k, v = (torch.randn(n, 1, 64, generator=g).bfloat16().to(DEV) for n in (seqs, int(lk.sum()), int(lk.sum())))
+    pk, pv = prefix_tensors(37, 1, 64)
+    cu_q, cu_k = torch.arange(seqs + 1, dtype=torch.int32), torch.cat((torch.zeros(1, dtype=torch.int64), lk.cumsum(0))).int()
+    got = attention_shared(q, k, v, pk, pv, cu_q.to(DEV), cu_k.to(DEV))
+    assert _lib.device_status() == 0
+    qd, (kd, vd) = q[:, 0].double(), (torch.zeros(seqs, 64, dtype=torch.float64, device=DEV) for _ in range(2))
+    there = (lk == 1).to(DEV)
+    kd[there], vd[there] = k[:, 0].double(), v[:, 0].double()
+    own = ((qd * kd).sum(-1, keepdim=True) / 8).masked_fill(~there[:, None], -math.inf)
+    p = torch.cat((qd @ pk[:, 0].double().t() / 8, own), 1).softmax(-1)
+    ref, size = (p[:, :-1] @ x + p[:, -1:] * y for x, y in ((pv[:, 0].double(), vd), (pv[:, 0].double().abs(), vd.abs())))
+    compare(got[:, 0], (ref, size))
+
+
 def test_long():
     check(20000, [1, 1], [5, 700], 8, 1, 128, seed=1)
     check(40000, [1] * 20, [30] * 20, 8, 2, 64, seed=2)
