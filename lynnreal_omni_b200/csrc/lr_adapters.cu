@@ -152,7 +152,8 @@ template <int N>
 struct Shrink {
   static constexpr int kTogether = N <= 32 ? 4 : N == 64 ? 2 : 1;
   static constexpr int kX = kShrinkRows * 128, kStage = kX + kTogether * N * 128;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = N == 16 ? 4 : 6;
+  static constexpr int kBlocks = N == 16 ? 2 : 1;  // an SM
   static constexpr int kBars = kStages * kStage;  // full, empty, done; TMEM address, abort flag
   static_assert(kBars >= N * kShrinkRows * 4, "the sums fit the ring");
   static constexpr size_t kSmem = 1024 + kBars + (2 * kStages + 1) * 8 + 8;
@@ -204,6 +205,9 @@ __global__ void __launch_bounds__(kShrinkThreads)
   groups.check(a);
   const int row = ((warp & 3) * 32) + lane;  // of the sums' warps
   const int mine = warp >= 2 && first + row < a.tokens ? a.index[first + row] : -1;
+  __shared__ float scales[kShrinkRows];
+  __shared__ int8_t slots[kShrinkRows];  // each row's adapter among a pass's, -1: none of them
+  if (warp >= 2) scales[row] = a.scale && adapter_of(a, mine) ? a.scale[mine] : 1.0f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -268,7 +272,8 @@ __global__ void __launch_bounds__(kShrinkThreads)
     } else {
       ok = ok && warp_wait(smem_u32(done), pass & 1u, watch, lane);
       tc_fence_after();
-      const float scale = a.scale && slot >= 0 ? a.scale[mine] : 1.0f;
+      slots[row] = (int8_t)slot;
+      const float scale = scales[row];
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       bf16* dst = a.inner + (int64_t)(first + row) * a.padded;
       for (int i = 0; i < together; ++i) {
@@ -294,20 +299,19 @@ __global__ void __launch_bounds__(kShrinkThreads)
     if (parts > 1) {
       __syncwarp();
       cluster_sync_all();
-      // this block's share of the columns, eight at a time
-      if (slot >= 0) {
-        const float scale = a.scale ? a.scale[mine] : 1.0f;
-        for (int c = part * 8; c < N; c += parts * 8) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-          for (int p = 0; p < parts; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += cluster_load(sums + (c + i) * kShrinkRows + row, p);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= scale;
-          *reinterpret_cast<uint4*>(a.inner + (int64_t)(first + row) * a.padded + c) = pack8(v);
+      // this block's share of the sums, two columns of a row at a time
+      const int share = kShrinkRows * N / 2 / parts;
+#pragma unroll 4
+      for (int i = part * share + (int)threadIdx.x; i < (part + 1) * share; i += kShrinkThreads) {
+        const int r = i % kShrinkRows, c = i / kShrinkRows * 2;
+        if (slots[r] < 0) continue;
+        const float* from = sums + c * kShrinkRows + r;
+        float v0 = 0.0f, v1 = 0.0f;
+        for (int p = 0; p < parts; ++p) {
+          v0 += cluster_load(from, p);
+          v1 += cluster_load(from + kShrinkRows, p);
         }
+        *reinterpret_cast<uint32_t*>(a.inner + (int64_t)(first + r) * a.padded + c) = cvt2(v0 * scales[r], v1 * scales[r]);
       }
       fence_async_smem();  // the next pass's copies write where the sums were
       __syncwarp();
@@ -438,8 +442,8 @@ __device__ __forceinline__ void unpack_row(float (&acc)[4][4], int h, const uint
 template <int KS>
 struct Few {
   static constexpr int kTile = 16 * 16 * KS;                      // inner values of 16 tokens
-  static constexpr int kSteps = KS == 1 ? 4 : KS <= 4 ? 2 : 1;    // of the first product whose loads are under way together
-  static constexpr int kAhead = KS == 1 ? 4 : KS == 2 ? 2 : 1;
+  static constexpr int kSteps = KS == 1 ? 4 : KS == 2 ? 2 : 1;    // of the first product whose loads are under way together
+  static constexpr int kAhead = KS == 1 ? 4 : KS == 2 ? 2 : KS == 4 ? 3 : 1;
   static constexpr int kLine = KS >= 4 ? 16 * KS + 32 : 16 * KS;  // inner rows side by side in different banks
   static constexpr int kBlocks = KS <= 2 ? 2 : 1;                 // an SM
   static constexpr size_t kSmem = (kWarps + 1) * kTile * 4 + 16 * kLine * 2;
@@ -556,13 +560,15 @@ __global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const A
   }
 }
 
-// Many tokens: tiles of 64 neighbours by 32 columns a warp, dealt out in runs down
-// the columns, so that a warp keeps its weights while the adapter stays the same.
-// A warp has a ring of tiles of its own in shared memory, which bulk copies fill
-// and empty: nothing but bytes in flight makes this kernel fast. (Base rows through
-// registers, the next tile's on their way meanwhile: 12240 tokens to 24576, rank
-// 32, 400 us, a third of the memory's rate.) Rows in shared memory are 64 bytes
-// long and two of them fill the banks.
+// Many tokens: tiles of 64 neighbours by 32 columns a warp. A warp has a ring of
+// tiles of its own in shared memory, which bulk copies fill and empty: nothing but
+// bytes in flight, and whole rows, make this kernel fast. 12240 tokens to 24576 at
+// rank 32, both products: 223 us, 0.93 of the measured copy rate (this kernel 0.97);
+// base rows through registers, the next tile's on their way, 457 us; through the
+// rings, but runs of tiles down the columns, 272 us. Blocks therefore take the tiles
+// of a row of tiles in turn; where the grid is a multiple of their number a warp
+// keeps its columns, and its weights while the adapter stays the same. Rows in
+// shared memory are 64 bytes long: two of them fill the banks.
 constexpr int kExpandRows = 64;
 constexpr int kSlotBytes = kExpandRows * 64;
 template <int KS>
@@ -600,39 +606,53 @@ __global__ void __launch_bounds__(kThreads, Expand<KS>::kBlocks)
   }
   __syncthreads();
   const bool el = elect_one();
-  const int tiles = (a.tokens + kExpandRows - 1) / kExpandRows;
-  const int64_t items = (int64_t)tiles * ((a.outputs + kThreads - 1) / kThreads);
-  const int64_t begin = items * blockIdx.x / gridDim.x;
-  const int count = (int)(items * (blockIdx.x + 1) / gridDim.x - begin);
+  // Items go along the rows and are dealt out in turn, so that the blocks together work on whole rows.
+  const int blocks = (a.outputs + kThreads - 1) / kThreads;
+  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks;
+  const int count = (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const int step_tile = gridDim.x / blocks, step_block = gridDim.x % blocks;
+  const auto advance = [&](int& tile, int& block) {
+    tile += step_tile;
+    block += step_block;
+    if (block >= blocks) block -= blocks, ++tile;
+  };
   // the next tile to be fetched, and the one in hand
-  int fetch_tile = (int)(begin % tiles), fetch_column = (int)(begin / tiles) * kThreads + warp * 32, fetched = 0;
-  int tile = fetch_tile, column = fetch_column;
+  int fetch_tile = blockIdx.x / blocks, fetch_block = blockIdx.x % blocks, fetched = 0;
+  int tile = fetch_tile, block = fetch_block;
   const auto fetch = [&] {
-    if (fetched < count && fetch_column < a.outputs && el) {
+    const int fetch_column = fetch_block * kThreads + warp * 32;
+    if (fetched < count && el) {
       const uint32_t s = (uint32_t)fetched % kSlots, bar = smem_u32(&full[s]);
-      mbar_expect_tx(bar, kSlotBytes);
-      tma_load_2d(smem_u32(ring + s * kSlotBytes), &map_base, bar, fetch_column, fetch_tile * kExpandRows);
+      if (fetch_column < a.outputs) {
+        mbar_expect_tx(bar, kSlotBytes);
+        tma_load_2d(smem_u32(ring + s * kSlotBytes), &map_base, bar, fetch_column, fetch_tile * kExpandRows);
+      } else {
+        mbar_arrive(bar);  // nothing to come
+      }
     }
     ++fetched;
-    if (++fetch_tile == tiles) fetch_tile = 0, fetch_column += kThreads;
+    advance(fetch_tile, fetch_block);
   };
   for (int s = 0; s < kSlots; ++s) fetch();
+  bool ok = true;
+  const auto wait_for = [&](int i) {
+    const bool landed = warp_wait(smem_u32(&full[i % kSlots]), (uint32_t)(i / kSlots) & 1u, watch, lane);
+    __syncwarp();
+    return landed;
+  };
   Groups<2> groups;
   groups.load(a, tile * kExpandRows, lane);
   wait_for_predecessor();
   Up<KS> up;
   int kept = -1, kept_column = -1;  // whose weights `up` holds
-  bool ok = true;
   for (int i = 0; i < count; ++i) {
-    const int first = tile * kExpandRows, this_column = column;
+    const int first = tile * kExpandRows, this_column = block * kThreads + warp * 32;
     Groups<2> now = groups;
     now.check(a);
-    if (++tile == tiles) tile = 0, column += kThreads;
+    advance(tile, block);
     if (i + 1 < count) groups.load(a, tile * kExpandRows, lane);
-    const uint32_t s = (uint32_t)i % kSlots;
-    uint8_t* rows = ring + s * kSlotBytes;
-    const bool there = this_column < a.outputs;  // the last columns' warps may have none
-    if (there) {
+    uint8_t* rows = ring + i % kSlots * kSlotBytes;
+    if (this_column < a.outputs) {  // the last columns' warps may have none
       // Inner values do not depend on whose they are; they load before the base rows are there.
       Inner<KS> inner[kHeld];
       const auto load_inner = [&](int from) {
@@ -650,8 +670,7 @@ __global__ void __launch_bounds__(kThreads, Expand<KS>::kBlocks)
       bool any = all || now.next(adapter, members);
       if (all) members[0] = members[1] = 0xffffffffu, adapter = kept;
       bool held = true;  // the first kHeld tiles' inner values
-      if (!(ok = warp_wait(smem_u32(&full[s]), ((uint32_t)i / kSlots) & 1u, watch, lane))) break;
-      __syncwarp();
+      if (!(ok = wait_for(i))) break;
       while (any) {
         if (adapter != kept || this_column != kept_column) {
           kept = adapter, kept_column = this_column;
@@ -680,11 +699,11 @@ __global__ void __launch_bounds__(kThreads, Expand<KS>::kBlocks)
       }
       fence_async_smem();
       __syncwarp();
-      if (el) {
-        tma_store_2d(&map_out, smem_u32(rows), this_column, first);
-        bulk_commit();
-      }
+      if (el) tma_store_2d(&map_out, smem_u32(rows), this_column, first);
+    } else if (!(ok = wait_for(i))) {
+      break;
     }
+    if (el) bulk_commit();
     // The tile before this one has been stored: its slot takes the next.
     if (i > 0) {
       if (el) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -801,7 +820,7 @@ int launch_shrink(const Args& a, cudaStream_t stream) {
     return st;
   const int64_t tiles = (a.tokens + kShrinkRows - 1) / kShrinkRows;
   LR_REQUIRE(tiles <= 65535, "adapters: too many tokens");
-  const int parts = column_parts(a, tiles, 2 * sm_count(), 256);
+  const int parts = column_parts(a, tiles, C::kBlocks * sm_count(), 256);
   return tc::launch("adapters (inner rows)", shrink_kernel<N>, dim3((unsigned)parts, (unsigned)tiles), kShrinkThreads, C::kSmem, stream,
                     (unsigned)parts, false, mx, md, a);
 }
@@ -824,8 +843,12 @@ int launch_expand(const Args& a, bool vec, cudaStream_t stream) {
   if ((st = tc::make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.base, dims, base_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) ||
       (st = tc::make_map(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.out, dims, out_strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return st;
-  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks, most = Expand<KS>::kBlocks * sm_count();
-  return tc::launch("adapters (outputs)", expand_kernel<KS>, dim3((unsigned)(items < most ? items : most)), kThreads, Expand<KS>::kSmem,
+  const int64_t items = (int64_t)((a.tokens + kExpandRows - 1) / kExpandRows) * blocks;
+  int64_t grid = Expand<KS>::kBlocks * sm_count();
+  const int64_t whole = grid / blocks * blocks;  // the same columns for every tile of a block
+  if (whole * 8 >= grid * 7) grid = whole;
+  if (grid > items) grid = items;
+  return tc::launch("adapters (outputs)", expand_kernel<KS>, dim3((unsigned)grid), kThreads, Expand<KS>::kSmem,
                     stream, 1, true, mb, mo, a);
 }
 

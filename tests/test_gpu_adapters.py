@@ -97,6 +97,12 @@ def test_one_adapter_for_all_and_none_for_any(tokens):
     check(tokens, 256, 256, 32, 3, index=[-7] * tokens, scaled=False)
 
 
+@pytest.mark.parametrize("tokens,outputs,count", [(600, 25864, 3), (70, 77000, 1), (640, 256 * 100 + 8, 2)])
+def test_rows_that_the_grid_does_not_divide(tokens, outputs, count):
+    """Blocks whose columns change from tile to tile, some of them past the last."""
+    check(tokens, 64, outputs, 16, count, seed=outputs)
+
+
 def test_large():
     check(5000, 4096, 12288, 32, 3, index=[0] * 2000 + [-1] * 17 + [2] * 2983)
 
