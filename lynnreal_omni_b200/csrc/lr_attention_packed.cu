@@ -1172,10 +1172,10 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a, const StepS
 // The parts of every row behind a prefix, the prefix's and then its sequence's
 // own, added in that order: a warp a row, D / 32 columns a lane.
 constexpr int kJoinRows = 8;
-template <int D>
-__global__ void __launch_bounds__(32 * kJoinRows) join_prefix_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
+template <int D, int AHEAD>
+__global__ void __launch_bounds__(32 * kJoinRows, AHEAD <= 8 ? 4 : 2) join_prefix_kernel(const Args a, const StepShape ss, const StepPrefix sp) {
   using V = typename std::conditional<D == 128, float4, float2>::type;
-  constexpr int kEach = D / 32, kAhead = 16;  // parts whose values are under way together
+  constexpr int kEach = D / 32, kAhead = AHEAD;  // parts whose values are under way together
   const int lane = threadIdx.x & 31;
   const int64_t all = (int64_t)a.total_q * a.heads, item = (int64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
   const int tok = (int)(min(item, all - 1) / a.heads), head = (int)(min(item, all - 1) % a.heads);
@@ -1331,7 +1331,8 @@ int launch_step(const Args& a, const Plan& p, const StepPrefix& sp, void* worksp
                                 : (p.narrow ? step_kernel<D, 2, 1, true> : step_kernel<D, 2, kStepWarps, true>);
     const int st = launch("attention_shared (steps)", kernel, all, 32 * kStepWarps, 0, stream, 1, sp.slots == 0, a, ss, sp);
     if (st) return st;
-    return launch("attention_shared (join)", join_prefix_kernel<D>, dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)),
+    const auto join = sp.chunks + p.slots / a.seqs <= 8 ? join_prefix_kernel<D, 8> : join_prefix_kernel<D, 16>;
+    return launch("attention_shared (join)", join, dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)),
                   32 * kJoinRows, 0, stream, 1, true, a, ss, sp);
   }
   const int st = launch("attention_packed (steps)", nt == 1 ? step_kernel<D, 1, kStepWarps, false> : step_kernel<D, 2, kStepWarps, false>,
