@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (MODE == kPrefixPart) part = (int64_t)(w.k_row / px.chunk) * a.total_q * a.heads + at;
         } else if (MODE != kNoPrefix) {
           // A row that stands for nothing sees every key, so that its warp has no mask to test: 48 prompts of 1 to 512 tokens
-          // behind 1000 keys 183 us with no key, PENDING us with all.
+          // behind 1000 keys 183 us with no key, 167 us with all.
           seen = w.lk;
         }
       }
@@ -1248,7 +1248,7 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   Plan p{};
   const int64_t queries = (total_q + seqs - 1) / seqs;  // a sequence, on average
   p.step = queries * group <= 64;
-  if (!p.step) return p;
+  if (!p.step && !shared) return p;
   // slots for three waves of four CTAs an SM, for one whole wave when there is one sequence
   const int64_t want = (int64_t)sm_count() * 4 * (seqs > 1 ? 3 : 1) / kv_heads;
   int64_t chunk = (total_k + (want > 0 ? want : 1) - 1) / (want > 0 ? want : 1);
@@ -1358,27 +1358,40 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
                        int64_t head_dim) {
   SharedPlan p{};
   p.own = plan(seqs, total_q, total_k, group, kv_heads, head_dim, true);
-  p.parts = p.own.step;
-  if (!p.parts) return p;
   const int64_t rows = total_q * group;
+  const int64_t head_parts = (group + kRows - 1) / kRows, tile_heads = (group + head_parts - 1) / head_parts;
+  const int64_t tokens = 2 * (kRows / tile_heads), sms = sm_count();
+  const int64_t blocks = (total_q + tokens - 1) / tokens * kv_heads * head_parts, tiles = (prefix + kKeys - 1) / kKeys;
+  // The prefix in one piece needs a block for every `tokens` tokens, and part of one for each sequence. Where those leave
+  // most SMs idle it is cut as for single tokens, although the rows' parts then pass through memory (at about 4 TB/s, and
+  // 6 us for the join) and step_kernel takes 16 rows at a time (about 0.7 us for 16 keys, 8 warps an SM). A key tile takes
+  // about 1.65 us, a block 8 more. One prompt of 100 tokens behind 16384 keys: 223 us in one piece, 48 in parts; 16 of
+  // 100 behind 2048: 76 and 161.
+  const int64_t most = sms / blocks > 1 ? (sms / blocks < tiles ? sms / blocks : tiles) : 1;
+  if (!p.own.step) {
+    const double own_tiles = (double)total_k / seqs / kKeys + 1;
+    const int64_t whole = blocks + seqs * kv_heads * head_parts / 2;
+    const double whole_us = (double)((whole + sms - 1) / sms) * (8 + 1.65 * (tiles + own_tiles));
+    const double parts_us = (double)((blocks * most + sms - 1) / sms) * (8 + 1.65 * ((tiles + most - 1) / most)) + 6 +
+                            (double)rows * kv_heads * (most + 1) * (head_dim + 2) * 8 / 4e6 +
+                            (double)rows / 16 * (total_k / seqs / 16 + 1) * kv_heads * 0.7 / (8 * sms);
+    if (parts_us >= whole_us) return p;
+  }
+  p.parts = true;
   p.step = rows <= 16;
   int64_t want;  // parts
   if (p.step) {
-    want = (int64_t)sm_count() * 4 / kv_heads;
+    want = sms * 4 / kv_heads;
     p.chunk = 64;
   } else {
-    const int64_t head_parts = (group + kRows - 1) / kRows, tile_heads = (group + head_parts - 1) / head_parts;
-    const int64_t tokens = 2 * (kRows / tile_heads);
-    const int64_t blocks = (total_q + tokens - 1) / tokens * kv_heads * head_parts, tiles = (prefix + kKeys - 1) / kKeys;
     // step_kernel runs on the SMs that this leaves, and on all of them afterwards: the parts should end when both together
-    // would, a key tile taking about 1.65 us and a block 8 more, and the sequences' own keys going by at 4.5 TB/s.
-    const double together = blocks * tiles * 1.65 / sm_count() + (double)total_k * kv_heads * head_dim * 4 / 4.5e6;
+    // would, the sequences' own keys going by at 4.5 TB/s.
+    const double together = blocks * tiles * 1.65 / sms + (double)total_k * kv_heads * head_dim * 4 / 4.5e6;
     const int64_t each = together > 8 + 1.65 ? (int64_t)((together - 8) / 1.65) + 1 : 1;
     want = (tiles + each - 1) / each;
-    if (want > sm_count() / blocks) want = sm_count() / blocks;
+    if (want > most) want = most;
     p.chunk = kKeys;
   }
-  if (want < 1) want = 1;
   p.chunk = (int)(((prefix + want - 1) / want + p.chunk - 1) / p.chunk * p.chunk);
   p.chunks = (int)((prefix + p.chunk - 1) / p.chunk);
   p.prefix_at = (p.own.bytes + 31) / 32 * 32;

@@ -116,6 +116,15 @@ def test_very_many_sequences(seqs):
     compare(got[:, 0], (ref, size))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lq,lk", [([100], [100]), ([64] * 4, [64] * 4), ([30, 0, 200], [300, 5, 200]), ([33], [20]), ([90], [0])])
+def test_few_prompts_behind_a_long_prefix(lq, lk, causal, d):
+    """Prompts whose prefix is cut into parts because their own blocks would not fill the GPU."""
+    check(5000, lq, lk, 8, 2, d, causal, seed=d)
+    check(3001, lq, lk, 5, 5, d, causal, seed=d)
+
+
 def test_long():
     check(20000, [1, 1], [5, 700], 8, 1, 128, seed=1)
     check(40000, [1] * 20, [30] * 20, 8, 2, 64, seed=2)
