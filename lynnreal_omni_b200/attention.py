@@ -147,18 +147,16 @@ def attention_shared(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     Kernels are chosen by the average number of queries a sequence, as there."""
     device = query.get_device()
-    for name, t in (("query", query), ("key", key), ("value", value), ("prefix_key", prefix_key), ("prefix_value", prefix_value)):
-        if t.dtype != torch.bfloat16 or t.ndim != 3 or not t.is_cuda:
+    given = (query, key, value, prefix_key, prefix_value)
+    for t, name in zip(given, ("query", "key", "value", "prefix_key", "prefix_value")):
+        if t.dtype is not torch.bfloat16 or t.ndim != 3 or not t.is_cuda:
             raise ValueError(f"attention_shared: {name} must be a CUDA bf16 [tokens, heads, D] tensor")
         if t.get_device() != device:
             raise ValueError("attention_shared: query, keys and values are on different devices")
-    if device != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
-            return attention_shared(query, key, value, prefix_key, prefix_value, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale)
     tq, h, d = query.shape
-    tk, hk, dk = key.shape
-    prefix = prefix_key.shape[0]
-    if value.shape != key.shape or dk != d or prefix_value.shape != prefix_key.shape or prefix_key.shape[1:] != key.shape[1:]:
+    tk, hk, dk = shape = key.shape
+    prefix, *rest = prefix_shape = prefix_key.shape
+    if value.shape != shape or dk != d or prefix_value.shape != prefix_shape or rest != [hk, dk]:
         raise ValueError("attention_shared: query/key/value/prefix shapes disagree")
     if d not in (64, 128):
         raise ValueError(f"attention_shared: head_dim {d} (the kernel handles 64 and 128)")
@@ -172,20 +170,28 @@ def attention_shared(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         return attention_packed(query, key, value, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale)
     count = cu_seqlens_q.numel()
     for t in (cu_seqlens_q, cu_seqlens_k):
-        if t.dtype != torch.int32 or t.ndim != 1 or count < 2 or t.get_device() != device:
+        if t.dtype is not torch.int32 or t.ndim != 1 or count < 2 or t.get_device() != device:
             raise ValueError("attention_shared: cu_seqlens must be int32 [sequences + 1] on the query's device")
     if cu_seqlens_k.numel() != count:
         raise ValueError("attention_shared: cu_seqlens_q and cu_seqlens_k differ in sequences")
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return attention_shared(*given, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale)
+    operands, kept = [], []  # pointer, token and head stride of each; the copies among them
+    for t in given:
+        ts, hs, cs = t.stride()
+        at = t.data_ptr()
+        if cs != 1 or ts % 8 or hs % 8 or ts < d or hs < d or at % 16:  # as in _head_view
+            t = t.clone(memory_format=torch.contiguous_format)
+            kept.append(t)
+            at, ts, hs = t.data_ptr(), t.shape[1] * d, d
+        operands += (at, ts, hs)
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
-    (query, q_ts, q_hs), (key, k_ts, k_hs), (value, v_ts, v_hs) = _head_view(query), _head_view(key), _head_view(value)
-    (prefix_key, pk_ts, pk_hs), (prefix_value, pv_ts, pv_hs) = _head_view(prefix_key), _head_view(prefix_value)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    lib, seqs = _lib.load(), count - 1
-    need = _shared_workspace_bytes(device, seqs, tq, tk, prefix, h, hk, d)
+    need = _shared_workspace_bytes(device, count - 1, tq, tk, prefix, h, hk, d)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    check(lib.lr_attention_shared(
-        query.data_ptr(), q_ts, q_hs, key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, prefix_key.data_ptr(), pk_ts,
-        pk_hs, prefix_value.data_ptr(), pv_ts, pv_hs, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), seqs, tq, tk, prefix, h,
-        hk, d, bool(causal), sc, out.data_ptr(), ptr(workspace), need, stream_of(query)), "attention_shared")
+    check(_lib.load().lr_attention_shared(
+        *operands, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), count - 1, tq, tk, prefix, h, hk, d, bool(causal),
+        1.0 / math.sqrt(d) if scale is None else float(scale), out.data_ptr(), ptr(workspace), need, stream_of(query)),
+        "attention_shared")
     return out
