@@ -92,6 +92,8 @@ class PromptLayer:
                  index: torch.Tensor | None = None) -> torch.Tensor:
         """bf16 [tokens, hidden] -> the same. prefix: the (keys, values) that ``read_prefix`` gave, in front of every prompt;
         index: int32 [tokens], each token's adapter on the ``AdaptedLinear`` projections (None: they go without)."""
+        if index is not None and not any(isinstance(p, AdaptedLinear) for p in (self.qkv, self.out, self.gate_up, self.down)):
+            raise ValueError("PromptLayer: adapters are given, but no projection has any")
         cu = prompts.cu_seqlens
         if prefix is None:
             return self._run(x, prompts.positions, inv_freq, factor, lambda q, k, v: attention_packed(q, k, v, cu), index)

@@ -63,6 +63,17 @@ def test_whole_prompts(lengths, prefix, d):
     check(prefix, lengths, lengths, 4, 2, d, seed=sum(lengths))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("prefix", [1, 128, 333])
+def test_many_prompts(prefix, causal, d):
+    """Enough blocks that each takes the whole prefix before its own keys; some sequences without keys or queries."""
+    lq = [37 * i % 190 + 20 for i in range(60)]
+    lk = [0 if i % 7 == 3 else n + 50 * (i % 3) for i, n in enumerate(lq)]
+    lq[5] = lq[11] = 0
+    check(prefix, lq, lk, 6, 2, d, causal, seed=prefix)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("h,hk", [(1, 1), (3, 3), (3, 1), (5, 1), (6, 2), (7, 1), (12, 4), (32, 8), (16, 1), (48, 1), (128, 1),
                                   (130, 1), (200, 1)])
@@ -140,7 +151,8 @@ def test_flat_and_peaked_scores(spread, lq, lk):
         check(300, lq, lk, 4, 2, 64, scale=scale)
 
 
-CASES = [([40, 30, 60], [40, 30, 60]), ([1, 1, 1], [40, 30, 60]), ([1, 1, 1], [1500, 1430, 1160]), ([8] * 6, [50, 9, 400, 8, 20, 8])]
+CASES = [([40, 30, 60], [40, 30, 60]), ([1, 1, 1], [40, 30, 60]), ([1, 1, 1], [1500, 1430, 1160]), ([8] * 6, [50, 9, 400, 8, 20, 8]),
+         ([150, 130, 70] + [90] * 60, [150, 130, 70] + [90] * 60)]  # enough blocks to take the prefix in one piece
 
 
 @pytest.mark.parametrize("lq,lk", CASES)

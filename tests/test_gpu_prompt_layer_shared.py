@@ -119,6 +119,18 @@ def test_captured_step():
         assert torch.equal(out, layer(x, plan, inv_freq, prefix=prefix, index=index))
 
 
+@pytest.mark.gpu
+def test_refusals():
+    layer = PromptLayer.random(hidden=HIDDEN, heads=HEADS, kv_heads=KV_HEADS, inner=512, head_dim=D)
+    inv_freq, _ = rope_frequencies(D)
+    x, plan = rows(5, 1), pack([5])
+    with pytest.raises(ValueError, match="no projection has any"):
+        layer(x, plan, inv_freq, index=token_adapters([0], [5]))
+    key = torch.zeros(9, KV_HEADS + 1, D, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="disagree"):
+        layer(x, plan, inv_freq, prefix=(key, key))
+
+
 def test_pack_behind_a_prefix():
     cu, positions = pack([2, 0, 3], "cpu", start=7)
     assert cu.tolist() == [0, 2, 2, 5] and positions.tolist() == [7, 8, 7, 8, 9]
