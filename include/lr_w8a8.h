@@ -53,7 +53,7 @@ const char* lr_last_error(void);
  * output row was written from zeros); bit 3: offsets of packed sequences went
  * down or outside their tensor; bit 4: a token's adapter number was past the
  * last adapter (its row had none). Bit 1 also covers the bounded waits of the
- * attention and 4-bit GEMM kernels. Synchronises the device. */
+ * attention, 4-bit GEMM and adapter kernels. Synchronises the device. */
 int lr_device_status(unsigned int* bits, int clear);
 
 /* Arithmetic of the divisions and RMS reciprocal square roots of the

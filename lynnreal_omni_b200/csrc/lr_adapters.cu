@@ -434,11 +434,14 @@ __device__ __forceinline__ void unpack_row(float (&acc)[4][4], int h, const uint
 // Both products in one kernel: clusters stand for one adapter and their blocks for
 // every gridDim.x-th 256 columns. A cluster's blocks share the first product, every
 // warp 32 columns of x at a time, add their sums in a fixed order through shared
-// memory and have the inner rows in it at once. (A launch of its own for the inner
-// rows: one token 6144 to 18432 5.2 us and 18.4 us with the host, now 5.0 and 13.6.)
-// Weights and base rows of the second product load meanwhile, and then kAhead
-// strips ahead. An adapter's second cluster reads `down` again, from L2; grids are
-// one wave.
+// memory and have the inner rows in it at once. (With a launch of its own for the
+// inner rows 64 tokens of 64 adapters, 4096 to 12288 at rank 16, took 14.4 us and 18.4
+// us with the host, now 15.4 and 17.0; one token 18.4 us with the host, now 12.6.)
+// Weights and base rows of the second product load meanwhile, and then AHEAD strips
+// ahead: one where a block has one strip (one token 6144 to 18432: 6.0 us with four),
+// else kAhead. An adapter's second cluster reads `down` again, from L2; grids are
+// one wave. Bound by latency: list, first product, cluster and second product follow
+// one another.
 template <int KS>
 struct Few {
   static constexpr int kTile = 16 * 16 * KS;                      // inner values of 16 tokens
@@ -449,7 +452,7 @@ struct Few {
   static constexpr size_t kSmem = (kWarps + 1) * kTile * 4 + 16 * kLine * 2;
 };
 
-template <int KS, bool VEC>
+template <int KS, int AHEAD, bool VEC>
 __global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const Args a) {
   using C = Few<KS>;
   constexpr int NR = 2 * KS;
@@ -470,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const A
     const bool lo = first + g < count, hi = first + 8 + g < count;
     const int64_t t0 = list.token[lo ? first + g : first], t1 = list.token[hi ? first + 8 + g : first];
     // strips of columns under way, a ring
-    Up<KS> up[C::kAhead];
-    uint4 base[C::kAhead][2];
+    Up<KS> up[AHEAD];
+    uint4 base[AHEAD][2];
     const bf16 *weight = up_of(a, max(adapter, 0)), *b0 = a.base + t0 * a.base_stride, *b1 = a.base + t1 * a.base_stride;
     bf16 *o0 = a.out + t0 * a.out_stride, *o1 = a.out + t1 * a.out_stride;
     const auto load_strip = [&](int s, int column) {
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const A
     };
     if (KS <= 4) {  // else the registers are not there yet
 #pragma unroll
-      for (int s = 0; s < C::kAhead; ++s) load_strip(s, start + s * stride);
+      for (int s = 0; s < AHEAD; ++s) load_strip(s, start + s * stride);
     }
     if (adapter >= 0) {
       float acc[NR][4];
@@ -541,14 +544,14 @@ __global__ void __launch_bounds__(kThreads, Few<KS>::kBlocks) few_kernel(const A
     if (KS > 4) load_strip(0, start);
     for (int next = start; next < a.outputs;) {
 #pragma unroll
-      for (int s = 0; s < C::kAhead; ++s, next += stride) {
+      for (int s = 0; s < AHEAD; ++s, next += stride) {
         if (next >= a.outputs) break;
         const int mine = next + 8 * t;
         float acc[4][4];
         unpack_row(acc, 0, base[s][0]);
         unpack_row(acc, 1, base[s][1]);
         if (adapter >= 0) add_update<KS>(acc, up[s], inner, true, true);
-        load_strip(s, next + C::kAhead * stride);
+        load_strip(s, next + AHEAD * stride);
         if (lo) store_row<VEC>(o0 + mine, acc, 0, a.outputs - mine);
         if (hi) store_row<VEC>(o1 + mine, acc, 1, a.outputs - mine);
       }
@@ -789,16 +792,18 @@ int64_t workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank) {
 
 template <int KS>
 int launch_few(const Args& a, bool vec, cudaStream_t stream) {
-  const auto kernel = vec ? few_kernel<KS, true> : few_kernel<KS, false>;
-  static bool done[2][64] = {};
-  const int st = tc::configure_smem(kernel, Few<KS>::kSmem, done[vec]);
-  if (st) return st;
   const int tiles = (a.tokens + 15) / 16, chunks = (tiles + a.groups - 1) / a.groups;
   int blocks = Few<KS>::kBlocks * sm_count() / (a.groups * chunks);  // for one adapter's tile
   if (blocks > (a.outputs + kThreads - 1) / kThreads) blocks = (a.outputs + kThreads - 1) / kThreads;
   int parts = 1;
   while (parts < 8 && 2 * parts <= blocks && (int64_t)parts * kWarps * 32 < a.width) parts *= 2;
   blocks = blocks < 1 ? 1 : blocks / parts * parts;
+  const bool one = (int64_t)blocks * kThreads >= a.outputs;
+  const auto kernel = one ? (vec ? few_kernel<KS, 1, true> : few_kernel<KS, 1, false>)
+                          : (vec ? few_kernel<KS, Few<KS>::kAhead, true> : few_kernel<KS, Few<KS>::kAhead, false>);
+  static bool done[2][2][64] = {};
+  const int st = tc::configure_smem(kernel, Few<KS>::kSmem, done[one][vec]);
+  if (st) return st;
   const dim3 grid((unsigned)blocks, (unsigned)(a.groups + 1), (unsigned)chunks);
   return tc::launch("adapters (few tokens)", kernel, grid, kThreads, Few<KS>::kSmem, stream, (unsigned)parts, false, a);
 }
