@@ -3,18 +3,19 @@
 // (e < 0: out[t, :] = base[t, :]), where base is the shared projection's output.
 //
 // The first product makes the few inner values scale[e] down[e] x[t] of every
-// token, the second adds up[e] times them to the base row. Both are bound by memory: per byte of x or base a rank of 16 to 128 gives the tensor core 8 to
-// 64 products, so mma.sync is fast enough, and its operands come straight from
-// global memory, 16 bytes a load: a sum over columns does not mind their order,
-// and neither do the outputs of a tile, so what a thread loads at once are the
-// columns that it stands for.
+// token, the second adds up[e] times them to the base row. Both are bound by
+// memory: per byte of x or base a rank of 16 to 128 gives the tensor core 8 to 64
+// products, so mma.sync is fast enough (tcgen05 where many tokens stream through
+// shared memory anyway), and its operands come straight from global memory, 16
+// bytes a load: a sum over columns does not mind their order, and neither do the
+// outputs of a tile, so what a thread loads at once are the columns that it stands
+// for.
 //
 // Up to kFew tokens, where one token a request is usual, a block stands for one
 // adapter and lists its tokens first, so that every adapter in use is read about
 // once whatever the order: few_kernel, both products. More tokens are taken in
-// tiles of neighbours, by shrink_kernel and an expand kernel: for each
-// adapter that occurs in a tile the rows of the others are zeros, and their sums
-// are put back afterwards. Either way an infinity in one request's row or adapter
+// tiles of neighbours, by shrink_kernel and an expand kernel: for each adapter that
+// occurs in a tile the rows of the others are neither used nor changed. Either way an infinity in one request's row or adapter
 // reaches no other.
 #include "lr_common.cuh"
 #include "lr_host.h"
@@ -146,7 +147,10 @@ __device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
 // on the tensor core, 64 columns of both a stage. The cluster's blocks take every
 // gridDim.x-th 64 columns and add their sums in order through shared memory. Up to
 // kTogether adapters that occur among the tokens are taken in one pass over the
-// rows, each in columns of its own of tensor memory.
+// rows, each in columns of its own of tensor memory. Bound by memory where tokens
+// are many (12240 of 6144 columns, rank 32: 31 us, 0.73 of the measured copy rate;
+// with mma.sync and operands straight from global memory 47), else by its chain of
+// latencies (2500 tokens: 17 us, an adapter at a time 34).
 constexpr int kShrinkRows = 128;
 template <int N>
 struct Shrink {
