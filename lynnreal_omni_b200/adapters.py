@@ -43,9 +43,9 @@ def _workspace_bytes(device: int, tokens: int, width: int, outputs: int, rank: i
 
 def _check_stack(name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None):
     """(adapters, rank, width, outputs) of adapters that fit each other."""
-    for what, t in (("down", down), ("up", up)):
-        if t.dtype != torch.bfloat16 or t.ndim != 3:
-            raise ValueError(f"{name}: {what} must be a bf16 tensor of three dimensions, got {t.dtype} {tuple(t.shape)}")
+    if down.dtype is not torch.bfloat16 or down.ndim != 3 or up.dtype is not torch.bfloat16 or up.ndim != 3:
+        raise ValueError(f"{name}: down and up must be bf16 tensors of three dimensions, got {down.dtype} {tuple(down.shape)}, "
+                         f"{up.dtype} {tuple(up.shape)}")
     count, rank, width = down.shape
     up_count, outputs, up_rank = up.shape
     if up_count != count or up_rank != rank or up.get_device() != down.get_device():
@@ -56,7 +56,7 @@ def _check_stack(name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.T
         raise ValueError(f"{name}: the rank must be a multiple of 8 up to {MOST_RANK} (pad with zeros), got {rank}")
     if width % 8:
         raise ValueError(f"{name}: the input width must be a multiple of 8, got {width}")
-    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count or scale.get_device() != down.get_device()):
+    if scale is not None and (scale.dtype is not torch.float32 or scale.numel() != count or scale.get_device() != down.get_device()):
         raise ValueError(f"{name}: scale must hold {count} fp32 values on the adapters' device")
     return count, rank, width, outputs
 
@@ -72,14 +72,16 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     x, nor base in any other way."""
     count, rank, width, outputs = _check_stack("add_adapters", down, up, scale)
     device = down.get_device()
-    for what, t, columns in (("base", base, outputs), ("x", x, width)):
-        if t.dtype != torch.bfloat16 or t.ndim != 2 or t.shape[1] != columns or t.get_device() != device:
-            raise ValueError(f"add_adapters: {what} must be a bf16 [tokens, {columns}] tensor on the adapters' device, "
-                             f"got {t.dtype} {tuple(t.shape)}")
+    if base.dtype is not torch.bfloat16 or base.ndim != 2 or base.shape[1] != outputs or base.get_device() != device:
+        raise ValueError(f"add_adapters: base must be a bf16 [tokens, {outputs}] tensor on the adapters' device, got {base.dtype} "
+                         f"{tuple(base.shape)}")
+    if x.dtype is not torch.bfloat16 or x.ndim != 2 or x.shape[1] != width or x.get_device() != device:
+        raise ValueError(f"add_adapters: x must be a bf16 [tokens, {width}] tensor on the adapters' device, got {x.dtype} "
+                         f"{tuple(x.shape)}")
     tokens = x.shape[0]
     if base.shape[0] != tokens:
         raise ValueError(f"add_adapters: base and x differ in tokens: {base.shape[0]}, {tokens}")
-    if index.dtype != torch.int32 or index.ndim != 1 or index.shape[0] != tokens or index.get_device() != device:
+    if index.dtype is not torch.int32 or index.ndim != 1 or index.shape[0] != tokens or index.get_device() != device:
         raise ValueError("add_adapters: index must be int32 [tokens] on the adapters' device")
     if device < 0:
         raise ValueError("add_adapters: expected CUDA tensors")
@@ -91,7 +93,8 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     elif (out.dtype != torch.bfloat16 or out.shape != base.shape or out.get_device() != device or out.stride(1) != 1
           or (tokens > 1 and out.stride(0) < outputs)):
         raise ValueError("add_adapters: out must be a bf16 tensor of base's shape with contiguous rows that do not overlap")
-    down, up, index = down.contiguous(), up.contiguous(), index.contiguous()
+    if not (down.is_contiguous() and up.is_contiguous() and index.is_contiguous()):
+        down, up, index = down.contiguous(), up.contiguous(), index.contiguous()
     if scale is not None:
         scale = scale.contiguous()
     base_stride, one = base.stride()
