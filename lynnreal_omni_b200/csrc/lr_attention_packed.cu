@@ -1386,7 +1386,7 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
   p.step = rows <= 16;
   int64_t want;  // parts
   if (p.step) {
-    want = sms * 4 / kv_heads;
+    want = sms * 4 / kv_heads > 1 ? sms * 4 / kv_heads : 1;
     p.chunk = 64;
   } else {
     // step_kernel runs on the SMs that this leaves, and on all of them afterwards: the parts should end when both together

@@ -1,0 +1,29 @@
+"""CPU tests of how a call behind a shared prefix is laid out: accepted sizes give a workspace, none ends the process."""
+from __future__ import annotations
+
+import subprocess
+import sys
+
+import pytest
+
+from lynnreal_omni_b200 import _lib
+
+
+def needed(*sizes):
+    """lr_attention_shared_workspace_bytes(seqs, queries, own keys, prefix, heads, kv_heads, D)."""
+    return _lib.load().lr_attention_shared_workspace_bytes(*sizes)
+
+
+@pytest.mark.parametrize("kv_heads", [592, 593, 600, 4096, 65535])
+@pytest.mark.parametrize("queries", [1, 10, 16, 17])
+def test_many_key_heads(kv_heads, queries):
+    """More key/value heads than the GPU has places for blocks. In a process of its own: it used to divide by zero."""
+    code = ("import ctypes, sys\n"
+            f"need = ctypes.CDLL({str(_lib.LIBRARY)!r}).lr_attention_shared_workspace_bytes\n"
+            "need.restype, need.argtypes = ctypes.c_int64, [ctypes.c_int64] * 7\n"
+            f"print(need(1, {queries}, 10, 100, {kv_heads}, {kv_heads}, 128))")
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert got.returncode == 0, (got.returncode, got.stderr)
+    # at least the prefix's part and the own one of every row, at most one of each 64 keys of the prefix more
+    row = queries * kv_heads * (128 + 2) * 4
+    assert 2 * row <= int(got.stdout) <= 3 * row + 64
