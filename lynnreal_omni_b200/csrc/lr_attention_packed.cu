@@ -1249,6 +1249,7 @@ struct Plan {
   int64_t parts;  // room for parts, 0 where no sequence can be long enough to be split
   int64_t bytes;  // of workspace
 };
+constexpr int64_t kMostRows = 65535 * 8;
 Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t kv_heads, int64_t head_dim, bool shared = false) {
   Plan p{};
   const int64_t queries = (total_q + seqs - 1) / seqs;  // a sequence, on average
@@ -1269,7 +1270,8 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   p.slots = (int)(total_k / chunk + seqs);
   int64_t most = 1;
   while (most < queries) most *= 2;
-  p.max_rows = (int)(most * group);
+  // Behind a prefix prompts, too, come here: sequences with more rows than a grid's z has are not split, their blocks go on by grids.
+  p.max_rows = (int)(most * group < kMostRows ? most * group : kMostRows);
   p.parts = total_k > chunk ? 2 * total_k / chunk + 2 : 0;
   p.bytes = p.parts * kv_heads * p.max_rows * (head_dim + 2) * 4;
   return p;
@@ -1326,7 +1328,6 @@ int launch_step(const Args& a, const Plan& p, const StepPrefix& sp, void* worksp
   const int nt = most_rows <= 8 ? 1 : 2;
   const dim3 grid((unsigned)(p.slots + sp.slots), (unsigned)a.kv_heads, (unsigned)((most_rows + 8 * nt - 1) / (8 * nt)));
   const int64_t rows = (int64_t)a.total_q * a.heads;
-  LR_REQUIRE(rows <= INT32_MAX, "attention: too many rows");
   const StepPrefix none{};
   if constexpr (SHARED) {
     dim3 all = grid;
@@ -1411,6 +1412,7 @@ template <int D>
 int launch_shared(const Args& a, const SharedPlan& p, StepPrefix sp, void* workspace, cudaStream_t stream) {
   if (!p.parts) return launch_prompt<D, kWithPrefix>(a, sp, sm_count(), stream);
   const int64_t all = (int64_t)a.total_q * a.heads;
+  LR_REQUIRE(all <= INT32_MAX, "attention_shared: too many rows");  // of the join's and the steps' grids, before anything runs
   sp.chunk = p.chunk, sp.chunks = p.chunks, sp.slots = p.step ? p.chunks : 0;
   sp.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.prefix_at);
   sp.part_ml = reinterpret_cast<float2*>(sp.part_o + p.chunks * all * D);
@@ -1485,6 +1487,7 @@ extern "C" int lr_attention_packed(const void* q, int64_t q_token_stride, int64_
                        (float)((double)scale * 1.4426950408889634)};
   auto* s = static_cast<cudaStream_t>(stream);
   const packed::StepPrefix none{};
+  LR_REQUIRE(!p.step || total_q * heads <= INT32_MAX, "attention_packed: too many rows");
   if (p.step)
     return head_dim == 64 ? packed::launch_step<64, false>(a, p, none, workspace, s)
                           : packed::launch_step<128, false>(a, p, none, workspace, s);

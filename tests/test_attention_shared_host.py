@@ -27,3 +27,13 @@ def test_many_key_heads(kv_heads, queries):
     # at least the prefix's part and the own one of every row, at most one of each 64 keys of the prefix more
     row = queries * kv_heads * (128 + 2) * 4
     assert 2 * row <= int(got.stdout) <= 3 * row + 64
+
+
+def test_too_many_rows_are_refused_before_anything_runs():
+    """2^32 rows: no grid counts them. The pointers are never followed."""
+    seqs, heads, lib = 1 << 20, 4096, _lib.load()
+    need = needed(seqs, seqs, 0, 100, heads, heads, 64)
+    operand = (4096, heads * 64, 64)
+    status = lib.lr_attention_shared(*operand, *operand, *operand, *operand, *operand, 4096, 4096, seqs, seqs, 0, 100, heads, heads, 64, 1,
+                                     0.125, 4096, 4096, need, None)
+    assert status == _lib.LR_ERR_INVALID_ARGUMENT and b"rows" in lib.lr_last_error()

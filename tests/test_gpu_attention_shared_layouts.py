@@ -2,8 +2,12 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
-from test_gpu_attention_shared import check
+from lynnreal_omni_b200 import _lib
+from lynnreal_omni_b200.attention import attention_shared
+from test_gpu_attention_packed import compare, offsets, tensors
+from test_gpu_attention_shared import check, prefix_tensors, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -13,3 +17,14 @@ pytestmark = pytest.mark.gpu
 def test_many_key_heads(lq, lk, hk):
     """More key/value heads than the GPU has places for blocks."""
     check(100, lq, lk, hk, hk, 64, seed=hk)
+
+
+def test_more_rows_of_a_sequence_than_a_grid_has():
+    """One sequence whose rows, 16 a block, are more blocks than a grid's third dimension counts. A sample of them is compared."""
+    tokens, prefix, h, hk, d = 132572, 131072, 8, 2, 64
+    q, k, v = tensors([tokens], [0], h, hk, d, seed=4)
+    pk, pv = prefix_tensors(prefix, hk, d)
+    got = attention_shared(q, k, v, pk, pv, offsets([tokens]), offsets([0]))
+    assert _lib.device_status() == 0
+    some = torch.cat((torch.arange(40), torch.arange(65520, 65560), torch.arange(131050, 131090), torch.arange(tokens - 40, tokens))).to(q.device)
+    compare(got[some], reference(q[some], k, v, pk, pv, [len(some)], [0], True, d ** -0.5))
