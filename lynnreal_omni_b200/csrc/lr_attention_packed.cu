@@ -1262,16 +1262,33 @@ Plan plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t group, int64_t
   // Shorter pieces cost more at the join than they save; up to 512 keys none is made (300 keys: one kernel takes 6.8 us, two
   // 7.7; 1000 keys in pieces of 256, 512, 1024: 9.1, 11.7, 16.1 us).
   if (chunk < 256) chunk = total_k <= 512 ? 512 : 256;
-  // Behind a prefix, where a warp takes a slot and head alone, 128 keys (64 requests of 64 to 1024 own keys: 35.5 us, 41.8 with
-  // 256; four warps a slot 41.5 and 38.5).
-  p.narrow = shared && (total_k / 128 + seqs) * kv_heads >= 8 * sm_count();
-  if (p.narrow && total_k < (1 << 23)) chunk = 128;
-  p.chunk = (int)chunk;
-  p.slots = (int)(total_k / chunk + seqs);
   int64_t most = 1;
   while (most < queries) most *= 2;
   // Behind a prefix prompts, too, come here: sequences with more rows than a grid's z has are not split, their blocks go on by grids.
   p.max_rows = (int)(most * group < kMostRows ? most * group : kMostRows);
+  if (shared && p.step) {
+    // Behind a prefix a warp takes a slot and head alone where those are many, 128 keys each (64 requests of 64 to 1024 own
+    // keys: 35.5 us, 41.8 with 256; four warps a slot 41.5 and 38.5). A row's part is as many bytes as a key and value of one
+    // head, written and read: at least eight keys a row (58 requests of 8 tokens, up to 989 own keys, 32 rows a head: 93.6 us, 101
+    // with 128 keys; 64 of 8 tokens, up to 4045, 64 rows: 600 and 752), and no more slots than four waves of warps take (64 of one
+    // token, up to 16181 own keys: 330 and 372). Room for parts then stays below 26 % of the own keys and values.
+    p.narrow = (total_k / 128 + seqs) * kv_heads >= 8 * sm_count();
+    if (p.narrow) {
+      const int64_t waves = 4 * 16 * (int64_t)sm_count(), even = (total_k * kv_heads + waves - 1) / waves;
+      chunk = 8 * p.max_rows > 128 ? 8 * p.max_rows : 128;
+      chunk = ((chunk > even ? chunk : even) + 63) / 64 * 64;
+    }
+  } else if (shared) {
+    // Of prompts every 16 rows are blocks of their own, which mostly fill the GPU: as many slots as give it two blocks an SM (17
+    // queries, 32 / 8 heads, 32768 own keys: 172 us, 536 in one piece, 221 in pieces of 128), else one for every other sequence,
+    // which splits those far above the average.
+    const int64_t asking = seqs < total_q ? seqs : total_q, blocks = asking * kv_heads * ((queries * group + 15) / 16);
+    const int64_t pieces = 2 * sm_count() / blocks, slots = pieces > 1 ? asking * pieces : (asking + 1) / 2;
+    chunk = ((total_k + slots - 1) / slots + 63) / 64 * 64;
+    if (chunk < 256) chunk = total_k <= 512 ? 512 : 256;
+  }
+  p.chunk = (int)chunk;
+  p.slots = (int)(total_k / chunk + seqs);
   p.parts = total_k > chunk ? 2 * total_k / chunk + 2 : 0;
   p.bytes = p.parts * kv_heads * p.max_rows * (head_dim + 2) * 4;
   return p;
@@ -1369,18 +1386,20 @@ SharedPlan shared_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t p
   const int64_t tokens = 2 * (kRows / tile_heads), sms = sm_count();
   const int64_t blocks = (total_q + tokens - 1) / tokens * kv_heads * head_parts, tiles = (prefix + kKeys - 1) / kKeys;
   // The prefix in one piece needs a block for every `tokens` tokens, and part of one for each sequence. Where those leave
-  // most SMs idle it is cut as for single tokens, although the rows' parts then pass through memory (at about 4 TB/s, and
-  // 6 us for the join) and step_kernel takes 16 rows at a time (about 0.7 us for 16 keys, 8 warps an SM). A key tile takes
-  // about 1.65 us, a block 8 more. One prompt of 100 tokens behind 16384 keys: 223 us in one piece, 48 in parts; 16 of
-  // 100 behind 2048: 76 and 161.
+  // most SMs idle it is cut as for single tokens, although the rows' parts, those of the prefix and those of the own keys, then pass
+  // through memory (at about 4 TB/s, and 6 us for the join) and step_kernel takes 16 rows at a time, their keys from L2 for each
+  // (about 1.2 us for 16 keys, 8 warps an SM). A key tile takes about 1.65 us, a block 8 more. One prompt of 100 tokens behind 16384 keys:
+  // 223 us in one piece, 48 in parts; 16 of 100 behind 2048: 76 and 161; behind 8192, 17 queries against 32768 own keys: 482 and 172;
+  // 128 against 32768: 553 and 689; 128 against 8192: 227 and 177; 256 against 8192: 228 and 352.
   const int64_t most = sms / blocks > 1 ? (sms / blocks < tiles ? sms / blocks : tiles) : 1;
   if (!p.own.step) {
-    const double own_tiles = (double)total_k / seqs / kKeys + 1;
+    const double own_keys = (double)total_k / seqs, own_tiles = own_keys / kKeys + 1;
+    const double own_parts = own_keys > p.own.chunk ? own_keys / p.own.chunk + 1 : 1;
     const int64_t whole = blocks + seqs * kv_heads * head_parts / 2;
     const double whole_us = (double)((whole + sms - 1) / sms) * (8 + 1.65 * (tiles + own_tiles));
     const double parts_us = (double)((blocks * most + sms - 1) / sms) * (8 + 1.65 * ((tiles + most - 1) / most)) + 6 +
-                            (double)rows * kv_heads * (most + 1) * (head_dim + 2) * 8 / 4e6 +
-                            (double)rows / 16 * (total_k / seqs / 16 + 1) * kv_heads * 0.7 / (8 * sms);
+                            (double)rows * kv_heads * (most + own_parts) * (head_dim + 2) * 8 / 4e6 +
+                            (double)rows / 16 * (own_keys / 16 + 1) * kv_heads * 1.2 / (8 * sms);
     if (parts_us >= whole_us) return p;
   }
   p.parts = true;

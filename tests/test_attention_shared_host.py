@@ -1,6 +1,8 @@
 """CPU tests of how a call behind a shared prefix is laid out: accepted sizes give a workspace, none ends the process."""
 from __future__ import annotations
 
+import math
+import random
 import subprocess
 import sys
 
@@ -37,3 +39,33 @@ def test_too_many_rows_are_refused_before_anything_runs():
     status = lib.lr_attention_shared(*operand, *operand, *operand, *operand, *operand, 4096, 4096, seqs, seqs, 0, 100, heads, heads, 64, 1,
                                      0.125, 4096, 4096, need, None)
     assert status == _lib.LR_ERR_INVALID_ARGUMENT and b"rows" in lib.lr_last_error()
+
+
+def room(seqs, tq, tk, prefix, h, hk, d):
+    """A bound on the workspace: a few fp32 parts a row of queries, a quarter of the own keys and values, and what fills the GPU
+    (148 blocks of 256 rows of the prefix's parts; the places of a wave for the own keys' of few sequences)."""
+    row = (d + 2) * 4
+    return row * (8 * tq * h + 2 ** 18 + 256 * hk) + int(0.26 * 4 * tk * hk * d)
+
+
+def test_pieces_of_prompts_behind_long_own_keys():
+    """Queries against longer own keys: the workspace stays below what the call reads and writes."""
+    for sizes in ((1, 256, 8192, 8192, 32, 8, 128), (1, 128, 32768, 8192, 32, 8, 128), (1, 128, 131072, 512, 32, 8, 128),
+                  (1, 147, 972915, 26, 32, 2, 128), (64, 64 * 80, 64 * 1080, 32768, 64, 8, 128), (16, 16 * 17, 16 * 4017, 32768, 64, 8, 128),
+                  (512, 512 * 17, 512 * 4017, 32768, 64, 8, 128), (64, 64 * 8, 64 * 4096, 8192, 64, 8, 128), (1, 1, 1 << 23, 1000, 32, 8, 128)):
+        seqs, tq, tk, prefix, h, hk, d = sizes
+        assert needed(*sizes) <= (4 * tq * h * d + 4 * (tk + prefix) * hk * d) // 2, sizes
+
+
+def test_workspaces_over_the_whole_range():
+    rng = random.Random(7)
+
+    def spread(high):
+        return int(round(2 ** rng.uniform(0, math.log2(high))))
+
+    for _ in range(20000):
+        hk, group, d = spread(64), spread(128), rng.choice((64, 128))
+        seqs, tq = spread(4096), spread(1 << 17)
+        tk, prefix = rng.choice((0, spread(1 << 24))), spread(1 << 20)
+        sizes = (seqs, tq, tk, prefix, hk * group, hk, d)
+        assert needed(*sizes) <= room(*sizes), (sizes, needed(*sizes), room(*sizes))
