@@ -130,9 +130,12 @@ class AdaptedLinear(nn.Module):
         """From a list of (down [rank, in], up [out, rank], scale) of any ranks up to 128; ranks are padded with zeros."""
         if not adapters:
             raise ValueError("AdaptedLinear: no adapters")
+        for d, u, _ in adapters:
+            if (d.ndim != 2 or u.ndim != 2 or d.shape[0] != u.shape[1] or d.shape[1] != base.in_features
+                    or u.shape[0] != base.out_features):
+                raise ValueError(f"AdaptedLinear: expected (down [rank, {base.in_features}], up [{base.out_features}, rank], scale) for each "
+                                 f"adapter, got {tuple(d.shape)}, {tuple(u.shape)}")
         ranks = [d.shape[0] for d, _, _ in adapters]
-        if any(d.ndim != 2 or u.ndim != 2 or u.shape[1] != r for (d, u, _), r in zip(adapters, ranks)):
-            raise ValueError("AdaptedLinear: expected (down [rank, in], up [out, rank], scale) for each adapter")
         rank = max(8, -(-max(ranks) // 8) * 8)
         device = adapters[0][0].device
         down = torch.zeros(len(ranks), rank, base.in_features, dtype=torch.bfloat16, device=device)
