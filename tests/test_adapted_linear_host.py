@@ -8,7 +8,7 @@ from lynnreal_omni_b200.adapters import AdaptedLinear
 
 
 def ones(*shape):
-    return torch.ones(*shape, dtype=torch.bfloat16)
+    return torch.ones(shape, dtype=torch.bfloat16)
 
 
 @pytest.mark.parametrize("down,up", [((3, 1), (24, 3)), ((3, 64), (1, 3)), ((3, 32), (24, 3)), ((3, 64), (64, 3)), ((3,), (24, 3)), ((3, 64), (24,)),
