@@ -69,7 +69,9 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     [adapters, out, rank], rank a multiple of 8 up to 128; scale fp32 [adapters] (None: 1); index int32 [tokens] on the
     device, negative for no adapter (a number past the last adapter counts as none and raises bit 4 of the device status).
     Any order will do, tokens of one adapter side by side are fastest. ``out`` may be ``base`` itself; it must not overlap
-    x, nor base in any other way."""
+    x, nor base in any other way. There is no backward pass: an ``out`` that belongs to an autograd graph is refused."""
+    if out is not None and out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("add_adapters: out belongs to an autograd graph, whose gradients would miss the update; call it under torch.no_grad()")
     count, rank, width, outputs = _check_stack("add_adapters", down, up, scale)
     device = down.get_device()
     if base.dtype is not torch.bfloat16 or base.ndim != 2 or base.shape[1] != outputs or base.get_device() != device:
@@ -112,7 +114,8 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
 
 
 class AdaptedLinear(nn.Module):
-    """A shared projection and the adapters of its requests. ``base``: a layer from bf16 [..., in] to bf16 [..., out]."""
+    """A shared projection and the adapters of its requests, for inference. ``base``: a layer from bf16 [..., in] to a new bf16
+    [..., out] tensor, in which the update is made."""
 
     def __init__(self, base: nn.Module, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None = None):
         super().__init__()
