@@ -11,7 +11,7 @@ from __future__ import annotations
 
 from types import MethodType
 
-from .fusion import resolve_adaln_table
+from .fusion import refuse_adapters, resolve_adaln_table
 from .kernels import _gated_residual, _swiglu
 
 
@@ -27,6 +27,7 @@ def block_forward(self, hidden_states, temb, adaln_indices, rotary_emb, attentio
     """One DiT block: attention on the modulated input (slots 0, 1) -> gated
     residual (slot 2) -> SwiGLU FFN on the modulated residual (slots 3, 4) ->
     gated residual (slot 5)."""
+    refuse_adapters(self)
     table = resolve_adaln_table(self, temb)
     rows = table.view(table.shape[0], 6, -1)  # [table rows, slot, hidden]
     attended = self.attn(_modulated(hidden_states, self.norm1, rows, adaln_indices, 0), rotary_emb, attention_mask)

@@ -32,6 +32,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kernels as k
+from .adapters import AdaptedLinear
 from .attention import attention_bshd
 
 CACHE_ENTRIES = 16  # adaLN tables kept per block (oldest evicted first)
@@ -122,6 +123,18 @@ class FusedAttention:
 
 
 # ------------------------------------------------------------ block stages
+def refuse_adapters(block):
+    """A DiT block has no adapter numbers to call its projections with: an ``AdaptedLinear`` among them would go without its
+    adapters."""
+    net, held = block.ff.net, vars(block.attn)
+    held = held.get("_modules", held)  # without the search, and the error where there is none, that a module's attributes cost
+    out = held.get("to_out")
+    layers = (held.get("to_qkv"), held.get("to_q"), held.get("to_k"), held.get("to_v"), out and out[0], net[0].proj, net[2])
+    if any(isinstance(layer, AdaptedLinear) for layer in layers):
+        raise ValueError("a DiT block passes no adapter numbers to its projections: put the adapters' bases in their places and call "
+                         "add_adapters, or merge one adapter into the weight before it is quantised")
+
+
 def _int8_capable(layer, fused_quant: bool) -> bool:
     return fused_quant and hasattr(layer, "forward_quantized")
 
@@ -162,6 +175,7 @@ def _ffn_down(down, projected, fused_quant):
 def fused_block(self, hidden_states, temb, adaln_indices, rotary_emb, attention_mask=None, adaln_table=None):
     """One DiT block (model/fusion.py:61-98): adaLN table -> attention branch ->
     gated residual + FFN prologue -> FFN (SwiGLU) -> gated residual (slot 5)."""
+    refuse_adapters(self)
     table = resolve_adaln_table(self, temb, adaln_table)
     quant = self._lynnreal_fused_quant
     attention_out = self.attn(_attention_input(self, hidden_states, table, adaln_indices, quant),
