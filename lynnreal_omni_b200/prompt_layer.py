@@ -16,7 +16,7 @@ low-rank adapters of its own on the projections (``AdaptedLinear`` in place of `
 
     prefixes = []
     for layer in layers:                              # once for all batches behind this text
-        t, kv = layer.read_prefix(t, inv_freq, factor)
+        t, kv = layer.read_prefix(t, inv_freq, factor)  # index=: as the model with an adapter reads it
         prefixes.append(kv)
     plan = pack([len(p) for p in prompts], "cuda", start=len(text))
     index = token_adapters(adapter_of_each_prompt, [len(p) for p in prompts], "cuda")
@@ -92,16 +92,16 @@ class PromptLayer:
                  index: torch.Tensor | None = None) -> torch.Tensor:
         """bf16 [tokens, hidden] -> the same. prefix: the (keys, values) that ``read_prefix`` gave, in front of every prompt;
         index: int32 [tokens], each token's adapter on the ``AdaptedLinear`` projections (None: they go without)."""
-        if index is not None and not any(isinstance(p, AdaptedLinear) for p in (self.qkv, self.out, self.gate_up, self.down)):
-            raise ValueError("PromptLayer: adapters are given, but no projection has any")
         cu = prompts.cu_seqlens
         if prefix is None:
             return self._run(x, prompts.positions, inv_freq, factor, lambda q, k, v: attention_packed(q, k, v, cu), index)
         return self._run(x, prompts.positions, inv_freq, factor, lambda q, k, v: attention_shared(q, k, v, *prefix, cu), index)
 
-    def read_prefix(self, x: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0):
-        """One text on its own, without adapters: bf16 [tokens, hidden] -> (the same for the next layer, (keys, values) bf16
-        [tokens, kv_heads, D] for the prompts that continue it)."""
+    def read_prefix(self, x: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0, *, index: torch.Tensor | None = None):
+        """One text on its own: bf16 [tokens, hidden] -> (the same for the next layer, (keys, values) bf16 [tokens, kv_heads, D] for the
+        prompts that continue it). index: int32 [tokens], the adapter that reads the text (None: it is read without one, and prompts
+        with adapters of their own then see the keys and values of the model without them). A text that several adapters are to read is
+        read once for each, and their prompts are called apart."""
         kept = []
 
         def attend(q, k, v):
@@ -109,9 +109,12 @@ class PromptLayer:
             return attention_packed(q, k, v, prompts.cu_seqlens)
 
         prompts = pack([x.shape[0]], x.device)
-        return self._run(x, prompts.positions, inv_freq, factor, attend, None), tuple(kept)
+        return self._run(x, prompts.positions, inv_freq, factor, attend, index), tuple(kept)
 
     def _run(self, x, positions, inv_freq, factor, attend, index):
+        if index is not None and not any(isinstance(p, AdaptedLinear) for p in (self.qkv, self.out, self.gate_up, self.down)):
+            raise ValueError("PromptLayer: adapters are given, but no projection has any")
+
         def project(linear, rows):
             return linear(rows, index) if isinstance(linear, AdaptedLinear) else linear(rows)
 
