@@ -61,14 +61,20 @@ def _check_stack(name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.T
     return count, rank, width, outputs
 
 
+def _readable(weight: torch.Tensor) -> torch.Tensor:
+    """The weight as the kernels read it: contiguous from a 16-byte boundary."""
+    return weight if weight.is_contiguous() and weight.data_ptr() % 16 == 0 else weight.clone(memory_format=torch.contiguous_format)
+
+
 def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor,
                  scale: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 [tokens, out]: base plus every token's low-rank update.
 
     base bf16 [tokens, out] and x bf16 [tokens, in]: rows may be strided; down bf16 [adapters, rank, in], up bf16
-    [adapters, out, rank], rank a multiple of 8 up to 128; scale fp32 [adapters] (None: 1); index int32 [tokens] on the
-    device, negative for no adapter (a number past the last adapter counts as none and raises bit 4 of the device status).
-    Any order will do, tokens of one adapter side by side are fastest. ``out`` may be ``base`` itself; it must not overlap
+    [adapters, out, rank], rank a multiple of 8 up to 128 (copied at each call where they are not contiguous from a 16-byte
+    boundary); scale fp32 [adapters] (None: 1); index int32 [tokens] on the device, negative for no adapter (a number past the last
+    adapter counts as none and raises bit 4 of the device status). The inner values down[e] x[t] are summed in fp32, scaled and
+    rounded to bf16 for the second product; base and update are added in fp32 and rounded once. Any order will do, tokens of one adapter side by side are fastest. ``out`` may be ``base`` itself; it must not overlap
     x, nor base in any other way. There is no backward pass: an ``out`` that belongs to an autograd graph is refused."""
     if out is not None and out.requires_grad and torch.is_grad_enabled():
         raise ValueError("add_adapters: out belongs to an autograd graph, whose gradients would miss the update; call it under torch.no_grad()")
@@ -95,8 +101,10 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     elif (out.dtype != torch.bfloat16 or out.shape != base.shape or out.get_device() != device or out.stride(1) != 1
           or (tokens > 1 and out.stride(0) < outputs)):
         raise ValueError("add_adapters: out must be a bf16 tensor of base's shape with contiguous rows that do not overlap")
-    if not (down.is_contiguous() and up.is_contiguous() and index.is_contiguous()):
-        down, up, index = down.contiguous(), up.contiguous(), index.contiguous()
+    down_at, up_at = down.data_ptr(), up.data_ptr()
+    if (down_at | up_at) % 16 or not (down.is_contiguous() and up.is_contiguous() and index.is_contiguous()):
+        down, up, index = _readable(down), _readable(up), index.contiguous()
+        down_at, up_at = down.data_ptr(), up.data_ptr()
     if scale is not None:
         scale = scale.contiguous()
     base_stride, one = base.stride()
@@ -107,7 +115,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         x, x_stride = x.clone(memory_format=torch.contiguous_format), width
     need = _workspace_bytes(device, tokens, width, outputs, rank, count)
     workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    check(_lib.load().lr_adapters(x.data_ptr(), x_stride, base.data_ptr(), base_stride, down.data_ptr(), up.data_ptr(),
+    check(_lib.load().lr_adapters(x.data_ptr(), x_stride, base.data_ptr(), base_stride, down_at, up_at,
                                   ptr(scale), index.data_ptr(), tokens, width, outputs, rank, count, out.data_ptr(),
                                   max(out.stride(0), outputs), ptr(workspace), need, stream_of(x)), "add_adapters")
     return out
@@ -124,8 +132,8 @@ class AdaptedLinear(nn.Module):
             raise ValueError(f"AdaptedLinear: adapters of {width} to {outputs} beside a projection of {base.in_features} to "
                              f"{base.out_features}")
         self.base, self.in_features, self.out_features = base, width, outputs
-        self.register_buffer("down", down.contiguous())
-        self.register_buffer("up", up.contiguous())
+        self.register_buffer("down", _readable(down))
+        self.register_buffer("up", _readable(up))
         self.register_buffer("scale", scale)
 
     @classmethod

@@ -36,3 +36,21 @@ def test_an_infinity_gives_infinities(where, tokens, width, rank):
     assert bool((got[lost] == -math.inf).all())
     rest = ~lost
     compare(got[rest], reference(base[rest], x[rest], down, up, index[rest], scale))
+
+
+@pytest.mark.parametrize("tokens", [9, 640])
+def test_adapters_off_16_byte_boundaries(tokens):
+    """Contiguous weights that begin anywhere, as slices of one flat checkpoint do."""
+    base, x, down, up, index, scale = tensors(tokens, 128, 192, 16, 3)
+    expected = add_adapters(base, x, down, up, index, scale)
+    for left in (1, 4):
+        flat = torch.full((left + down.numel() + 3 + up.numel() + 5,), 7.0, device=DEV, dtype=torch.bfloat16)
+        d = flat[left:left + down.numel()].view(down.shape)
+        u = flat[left + down.numel() + 3:-5].view(up.shape)
+        d.copy_(down), u.copy_(up)
+        assert d.is_contiguous() and u.is_contiguous()
+        assert torch.equal(add_adapters(base, x, d, u, index, scale), expected)
+        assert torch.equal(add_adapters(base, x, d, up, index, scale), expected)
+        assert torch.equal(add_adapters(base, x, down, u, index, scale), expected)
+    odd = torch.cat((index[:1], index))[1:]
+    assert torch.equal(add_adapters(base, x, down, up, odd, scale), expected)
