@@ -51,6 +51,8 @@ def pack(lengths, device="cuda", *, start: int = 0) -> PackedPrompts:
         raise ValueError("pack: expected the lengths of one or more prompts")
     if start < 0:
         raise ValueError("pack: start must not be negative")
+    if start + max(lengths) > 2 ** 31:
+        raise ValueError(f"pack: positions from {start} on do not fit 32 bits")
     n = torch.tensor(lengths, dtype=torch.int64)
     cu = torch.cat((torch.zeros(1, dtype=torch.int64), n.cumsum(0)))
     positions = torch.arange(int(cu[-1])) - torch.repeat_interleave(cu[:-1], n) + start
