@@ -145,7 +145,8 @@ def attention_shared(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     keys and values are shared by all sequences, not copied; a single length for it, known to the host. Values of other
     sequences never reach a row; within a sequence, values of masked keys must be finite.
 
-    Kernels are chosen by the average number of queries a sequence, as there."""
+    Scores, softmax and sums are fp32; the probabilities, of at most 2^8 before they are divided by their sum, are rounded to bf16 for the
+    second product. Kernels are chosen by counts alone: the average number of queries and keys a sequence, and the prefix."""
     device = query.get_device()
     given = (query, key, value, prefix_key, prefix_value)
     for t, name in zip(given, ("query", "key", "value", "prefix_key", "prefix_value")):

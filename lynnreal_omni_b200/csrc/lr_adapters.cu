@@ -12,10 +12,13 @@
 // for.
 //
 // Up to kFew tokens, where one token a request is usual, a block stands for one
-// adapter and lists its tokens first, so that every adapter in use is read about
-// once whatever the order: few_kernel, both products. More tokens are taken in
-// tiles of neighbours, by shrink_kernel and an expand kernel: for each adapter that
-// occurs in a tile the rows of the others are neither used nor changed. Either way an infinity in one request's row or adapter
+// adapter and lists its tokens first: few_kernel, both products. Whatever the
+// tokens' order an adapter in use is read once for every 16 of them, from memory
+// once. The grid counts the adapters that are there: few in use out of many, or most
+// tokens with one of them, leave the other blocks idle and that one's 16 tokens
+// after one another. More tokens are taken in tiles of neighbours, by shrink_kernel and
+// an expand kernel: for each adapter that occurs in a tile the rows of the others are
+// neither used nor changed. Either way an infinity in one request's row or adapter
 // reaches no other.
 #include "lr_common.cuh"
 #include "lr_host.h"
@@ -836,6 +839,7 @@ int launch_shrink(const Args& a, cudaStream_t stream) {
   const int64_t tiles = (a.tokens + kShrinkRows - 1) / kShrinkRows;
   LR_REQUIRE(tiles <= 65535, "adapters: too many tokens");
   const int parts = column_parts(a, tiles, C::kBlocks * sm_count(), 256);
+  // The ordinary way: the expand kernels read base, the tokens' numbers and weights before they wait for this one.
   return tc::launch("adapters (inner rows)", shrink_kernel<N>, dim3((unsigned)parts, (unsigned)tiles), kShrinkThreads, C::kSmem, stream,
                     (unsigned)parts, false, mx, md, a);
 }

@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   };
   PromptItem first{};
   bool first_there = false;
-  if (MODE == kPrefixPart) allow_dependent();  // the step kernel, which waits for this one before it reads the parts
+  if (MODE == kPrefixPart) allow_dependent();  // step_kernel, a block of which waits for this one, so that the join finds both's parts
   if (warp == 3) first_there = prompt_item<MODE>(a, ps, px, item_index(0), lane, first);
   tc_fence_before();
   __syncthreads();
@@ -1329,6 +1329,8 @@ int launch_prompt(const Args& a, const StepPrefix& sp, int64_t most_blocks, cuda
     return st;
   static bool done[64] = {};
   if ((st = configure_smem(prompt_kernel<D, MODE>, C::kSmem, done))) return st;
+  // The ordinary way: behind its parts step_kernel is launched dependent, and reads operands and writes parts and rows of its own
+  // without waiting for this one.
   prompt_kernel<D, MODE><<<(unsigned)(items < most_blocks ? items : most_blocks), kPromptThreads, C::kSmem, stream>>>(
       mq, mk, mv, a, ps, mpk, mpv, px);
   return launch_status(MODE == kNoPrefix ? "attention_packed (prompts)" : "attention_shared (prompts)");

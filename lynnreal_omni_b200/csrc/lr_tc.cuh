@@ -245,10 +245,15 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 
 // ------------------------------------------------------------------ dependent launches
-// A kernel launched with launch_dependent may start when its predecessor's
-// blocks have all called allow_dependent (or ended); it must call
-// wait_for_predecessor, in every block, before it touches global memory or
-// ends: until then only its own set-up may run.
+// A kernel launched dependent may start when its predecessor's blocks have all
+// called allow_dependent (or ended). Until a block has called
+// wait_for_predecessor it must touch nothing that the predecessor writes, and
+// write nothing that the predecessor touches; of what is older only what was
+// complete before the predecessor began, which is everything if the predecessor was
+// launched the ordinary way, and nothing otherwise. Pairs that count on that say so
+// where the first one is launched. At least one block waits before it ends, so that
+// the kernel is not complete before its predecessor and what follows in the stream
+// is behind both.
 __device__ __forceinline__ void allow_dependent() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
