@@ -129,7 +129,9 @@ def refuse_adapters(block):
     net, held = block.ff.net, vars(block.attn)
     held = held.get("_modules", held)  # without the search, and the error where there is none, that a module's attributes cost
     out = held.get("to_out")
-    layers = (held.get("to_qkv"), held.get("to_q"), held.get("to_k"), held.get("to_v"), out and out[0], net[0].proj, net[2])
+    if hasattr(out, "__getitem__"):
+        out = out[0]
+    layers = (held.get("to_qkv"), held.get("to_q"), held.get("to_k"), held.get("to_v"), out, net[0].proj, net[2])
     if any(isinstance(layer, AdaptedLinear) for layer in layers):
         raise ValueError("a DiT block passes no adapter numbers to its projections: put the adapters' bases in their places and call "
                          "add_adapters, or merge one adapter into the weight before it is quantised")

@@ -70,3 +70,18 @@ def test_adapted_projections_are_refused(kind, place):
     rotary = (torch.zeros(3, HIDDEN), torch.zeros(3, HIDDEN))
     with pytest.raises(ValueError, match="adapter"):
         block.forward(x, None, torch.zeros(3, dtype=torch.int64), rotary)
+
+
+def test_an_output_projection_without_a_list_runs():
+    """The element-wise blocks keep their native attention, whatever it holds."""
+    block = block_of(True)
+    block.attn.to_out = linear(HIDDEN, HIDDEN)
+    elementwise_fusion.enable_elementwise_fusion(SimpleNamespace(transformer_blocks=[block], training=False))
+    table = torch.zeros(1, 6 * HIDDEN, dtype=torch.bfloat16)
+    block._lynnreal_adaln_cache, block._lynnreal_cache_key = {0: table}, SimpleNamespace(current=0)
+    args = torch.zeros(1, 3, HIDDEN, dtype=torch.bfloat16), None, torch.zeros(3, dtype=torch.int64), None
+    with pytest.raises(AssertionError, match="the block ran"):
+        block.forward(*args)
+    block.attn.to_out = AdaptedLinear.stack(block.attn.to_out, [(torch.zeros(8, HIDDEN), torch.zeros(HIDDEN, 8), 1.0)])
+    with pytest.raises(ValueError, match="adapter"):
+        block.forward(*args)
